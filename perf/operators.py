@@ -1,0 +1,351 @@
+"""Cases, plain forms and calls of the paged-cache append and of differential attention.
+
+Three operations of one layer, as a serving loop runs them:
+  append  esp_kv_append: the projection's queries, keys and values of the new tokens; queries and keys are rotated to their
+          positions, everything is rounded to 16 bits, keys and values also go into their slots of the paged cache;
+  step    esp_diff_forward with one new token per sequence over its cached keys;
+  rows    esp_diff_forward with many new tokens per sequence: prefill, a chunk behind a cached prefix, a draft tree.
+A differential head of HD dims holds two queries and two keys of HD / 2 dims and one value of HD dims:
+  O = out_scale * w * D / sqrt(mean D^2 + eps),  D = softmax(scale q1.k1) V - lambda_h softmax(scale q2.k2) V.
+"""
+import math
+
+import numpy as np
+import torch
+
+own = False
+
+DEV = "cuda"
+T16 = {"f16": torch.float16, "bf16": torch.bfloat16}
+EPS, OUT_SCALE = 1e-5, 0.45
+
+
+# ------------------------------------------------------------------------------------------------ cases
+def listed():
+    return [
+        # one token of one sequence enters the cache: the smallest call, launch latency
+        dict(name="append 1 token", op="append", rows=1, H=32, Hkv=8, HD=128, maps=2, rot=64, pairs="halves", src="bf16", dtype="bf16", pool="bf16", bt=16, pad=0),
+        # a decode batch over an 8-bit cache, part of the batch is padding
+        dict(name="append 257 tokens e4m3", op="append", rows=257, H=32, Hkv=8, HD=256, maps=2, rot=128, pairs="halves", src="bf16", dtype="bf16", pool="e4m3", bt=16, pad=9),
+        # a prompt: adjacent pairs, ordinary heads
+        dict(name="append 8192 tokens", op="append", rows=8192, H=32, Hkv=4, HD=128, maps=1, rot=128, pairs="adjacent", src="f16", dtype="f16", pool="f16", bt=16, pad=0),
+        # an odd prompt from an fp32 projection, a quarter of the 256 dims rotated
+        dict(name="append 5001 tokens f32", op="append", rows=5001, H=16, Hkv=2, HD=256, maps=1, rot=64, pairs="halves", src="f32", dtype="bf16", pool="bf16", bt=32, pad=1),
+        # a chat's next token: short context, latency
+        dict(name="step 1 x 1024", op="step", seqs=1, lo=1024, hi=1024, H=8, Hkv=2, HD=128, dtype="f16", pool="f16", bt=16),
+        # a serving batch of uneven lengths
+        dict(name="step 32 x 512..32768", op="step", seqs=32, lo=512, hi=32768, H=32, Hkv=4, HD=128, dtype="bf16", pool="bf16", bt=16),
+        # one long document over an 8-bit cache
+        dict(name="step 1 x 131072 e4m3", op="step", seqs=1, lo=131072, hi=131072, H=32, Hkv=8, HD=256, dtype="bf16", pool="e4m3", bt=16),
+        # few heads per key head, large pages, some sequences only just begun
+        dict(name="step 7 x 1..6001", op="step", seqs=7, lo=1, hi=6001, H=16, Hkv=8, HD=256, dtype="f16", pool="f16", bt=64),
+        # two prompts from nothing
+        dict(name="prefill 2 x 8192", op="rows", seqs=2, m_lo=8192, m_hi=8192, lo=0, hi=0, mask="causal", H=16, Hkv=4, HD=128, dtype="bf16", pool="bf16", bt=16),
+        # prompts of odd lengths, 256-dim heads
+        dict(name="prefill 5 x 33..4001 hd256", op="rows", seqs=5, m_lo=33, m_hi=4001, lo=0, hi=0, mask="causal", H=16, Hkv=4, HD=256, dtype="f16", pool="f16", bt=16),
+        # draft trees behind long prefixes
+        dict(name="tree 16 x (4096 + 16)", op="rows", seqs=16, m_lo=16, m_hi=16, lo=4096, hi=4096, mask="tree", H=32, Hkv=4, HD=128, dtype="bf16", pool="bf16", bt=16),
+        # the next chunk of a long prompt over an 8-bit cache
+        dict(name="chunk 700 behind 20001 e4m3", op="rows", seqs=1, m_lo=700, m_hi=700, lo=20001, hi=20001, mask="causal", H=32, Hkv=8, HD=128, dtype="f16", pool="e4m3", bt=16),
+    ]
+
+
+def log_int(rng, lo, hi):
+    return max(lo, min(hi, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+
+
+def draw(rng):
+    op = rng.choice(["append", "step", "rows"])
+    dtype = rng.choice(["f16", "bf16"])
+    pool = rng.choice([dtype, dtype, "e4m3"])
+    HD = rng.choice([128, 256])
+    Hkv = rng.choice([1, 2, 4, 8])
+    H = Hkv * rng.choice([1, 2, 4, 8])
+    bt = rng.choice([16, 32, 64])
+    if op == "append":
+        HD = rng.choice([64, 128, 256])
+        maps = rng.choice([1, 2])
+        rows = min(log_int(rng, 1, 16384), (40 << 20) // ((H + 2 * Hkv) * HD))
+        return dict(op="append", rows=rows, H=H, Hkv=Hkv, HD=HD, maps=maps, rot=HD // maps // rng.choice([1, 1, 2]), pairs=rng.choice(["halves", "adjacent"]),
+                    src=rng.choice([dtype, "f32"]), dtype=dtype, pool=pool, bt=bt, pad=rng.choice([0, 0, 1]) * (rows // 16))
+    if op == "step":
+        seqs = log_int(rng, 1, 64)
+        hi = min(log_int(rng, 16, 131072), (1 << 29) // (2 * Hkv * HD * seqs))
+        return dict(op="step", seqs=seqs, lo=max(1, hi // rng.choice([1, 4, 32])), hi=hi, H=H, Hkv=Hkv, HD=HD, dtype=dtype, pool=pool, bt=bt)
+    seqs = log_int(rng, 1, 16)
+    if rng.random() < 0.4:
+        m = rng.randint(4, 64)
+        hi = min(log_int(rng, 64, 16384), (1 << 28) // (2 * Hkv * HD * seqs))
+        return dict(op="rows", seqs=seqs, m_lo=m, m_hi=m, lo=max(1, hi // 2), hi=hi, mask="tree", H=H, Hkv=Hkv, HD=HD, dtype=dtype, pool=pool, bt=bt)
+    pairs = (1 << 30) // (H * seqs)  # rows x keys of one sequence and head: under the largest listed one's
+    m = min(log_int(rng, 16, 8192), math.isqrt(pairs))
+    pre = rng.choice([0, 0, 1]) * min(log_int(rng, 16, 16384), pairs // m)
+    return dict(op="rows", seqs=seqs, m_lo=max(1, m // rng.choice([1, 8])), m_hi=m, lo=pre // 2, hi=pre, mask="causal", H=H, Hkv=Hkv, HD=HD, dtype=dtype, pool=pool, bt=bt)
+
+
+def spread(n, lo, hi):
+    """n lengths between lo and hi, even on the logarithm, the long ones not all last."""
+    if n == 1:
+        return [hi]
+    if lo <= 0:
+        v = [round(hi * i / (n - 1)) for i in range(n)]
+    else:
+        v = [round(lo * (hi / lo) ** (i / (n - 1))) for i in range(n)]
+    return v[::2] + v[1::2][::-1]
+
+
+def tree_mask(m):
+    """Ancestor sets of a tree in which node i hangs under node (i - 1) // 2, as 0 / 1 [m, m]."""
+    a = np.zeros((m, m), dtype=bool)
+    for i in range(m):
+        if i:
+            a[i] = a[(i - 1) // 2]
+        a[i, i] = True
+    return a
+
+
+def lengths(c):
+    if c["op"] == "step":
+        return [1] * c["seqs"], spread(c["seqs"], c["lo"], c["hi"])
+    return spread(c["seqs"], c["m_lo"], c["m_hi"]), spread(c["seqs"], c["lo"], c["hi"])
+
+
+def work(c):
+    H, Hkv, HD = c["H"], c["Hkv"], c["HD"]
+    esz = 1 if c["pool"] == "e4m3" else 2
+    if c["op"] == "append":
+        rows, kept = c["rows"], c["rows"] - c["pad"]
+        wide = (H + 2 * Hkv) * HD
+        b = rows * wide * ((4 if c["src"] == "f32" else 2) + 2) + kept * 2 * Hkv * HD * esz + rows * 12 + 2 * c["rot"]
+        return {"bytes": b, "flops": rows * (H + Hkv) * c["maps"] * c["rot"] * 3}
+    ms, ps = lengths(c)
+    b = sum(ps) * 2 * Hkv * HD * esz + sum(ms) * (2 * H + 2 * Hkv) * HD * 2
+    seen = sum(m * p + (int(tree_mask(m).sum()) if c.get("mask") == "tree" else m * (m + 1) // 2) for m, p in zip(ms, ps))
+    return {"bytes": b, "flops": 6 * HD * H * seen}
+
+
+# ------------------------------------------------------------------------------------------------ inputs
+def pool_of(g, n_blocks, c):
+    """A cache whose pages all hold something, and - 8-bit - the scale of every page and key head."""
+    shape = (n_blocks, 2, c["bt"], c["Hkv"], c["HD"])
+    if c["pool"] != "e4m3":
+        return torch.empty(shape, dtype=T16[c["pool"]], device=DEV).normal_(generator=g), None
+    scales = torch.exp2(torch.rand((n_blocks, 2, c["Hkv"]), generator=g, device=DEV) * 6 - 4)
+    kv = torch.empty(shape, dtype=torch.uint8, device=DEV)
+    per = max(1, (1 << 26) // (2 * c["bt"] * c["Hkv"] * c["HD"]))
+    for at in range(0, n_blocks, per):
+        x = torch.randn((min(per, n_blocks - at),) + shape[1:], generator=g, device=DEV) / scales[at:at + per, :, None, :, None]
+        kv[at:at + per] = x.clamp_(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8)
+    return kv, scales
+
+
+def prepare(c, seed):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(seed)
+    cpu = np.random.default_rng(seed)
+    H, Hkv, HD, bt = c["H"], c["Hkv"], c["HD"], c["bt"]
+    st = {"c": c}
+
+    def normal(*shape, dtype=T16[c["dtype"]]):
+        return torch.empty(shape, dtype=dtype, device=DEV).normal_(generator=g)
+
+    if c["op"] == "append":
+        rows, src = c["rows"], torch.float32 if c["src"] == "f32" else T16[c["src"]]
+        # the fused projection of the new tokens: queries, keys, values side by side
+        st["X"] = normal(rows, (H + 2 * Hkv) * HD, dtype=src)
+        used = (rows + bt - 1) // bt
+        st["n_blocks"] = used + 3
+        st["pool"], st["scales"] = pool_of(g, st["n_blocks"] + 1, c)  # the last block is nobody's: the plain form drops padding rows there
+        order = cpu.permutation(st["n_blocks"])[:used]
+        at = np.arange(rows)
+        slots = np.stack([order[at // bt], at % bt], axis=1).astype(np.int32)
+        slots[cpu.permutation(rows)[:c["pad"]], 0] = -1
+        st["slots"] = torch.from_numpy(slots).to(DEV)
+        st["pos"] = torch.from_numpy((np.arange(rows) + int(cpu.integers(0, 100000))).astype(np.int32)).to(DEV)
+        half = c["rot"] // 2
+        st["inv_freq"] = torch.from_numpy((10000.0 ** (-np.arange(half) / half)).astype(np.float32)).to(DEV)
+        st["q"] = torch.empty((rows, H * HD), dtype=T16[c["dtype"]], device=DEV)
+        st["k"], st["v"] = (torch.empty((rows, Hkv * HD), dtype=T16[c["dtype"]], device=DEV) for _ in range(2))
+        if own:
+            from espetero_b200 import capi, host
+            dt = {"f16": capi.ESP_F16, "bf16": capi.ESP_BF16, "e4m3": capi.ESP_E4M3}
+            st["op"] = host.AttnOp(H, Hkv, HD, bt, dt[c["dtype"]], dt[c["pool"]], 1.0)
+            q, k, v = st["X"].split([H * HD, Hkv * HD, Hkv * HD], dim=1)
+            st["call"] = st["op"].append_call(Q=q, K=k, V=v, Qo=st["q"], Kb=st["k"], Vb=st["v"], kv=st["pool"], kv_scales=st["scales"], n_blocks=st["n_blocks"],
+                                              slots=st["slots"], pos=st["pos"], inv_freq=st["inv_freq"], maps=c["maps"], adjacent=c["pairs"] == "adjacent")
+        return st
+
+    ms, ps = lengths(c)
+    rows, d = sum(ms), HD // 2
+    st["Q"] = normal(rows, H * HD).mul_(1.5)  # scores with a spread of 1.5: attention that prefers some keys
+    st["Kb"], st["Vb"] = normal(rows, Hkv * HD), normal(rows, Hkv * HD)
+    st["O"] = torch.empty((rows, H * HD), dtype=T16[c["dtype"]], device=DEV)
+    pages = [(p + bt - 1) // bt for p in ps]
+    n_blocks = sum(pages) + 3
+    st["pool"], st["scales"] = pool_of(g, n_blocks, c)
+    blocks = cpu.permutation(n_blocks).astype(np.int32)[:max(1, sum(pages))]
+    st["blocks"] = torch.from_numpy(blocks).to(DEV)
+    st["lam"] = torch.rand(H, generator=g, device=DEV) * 0.6 + 0.2
+    st["w"] = 1 + 0.1 * torch.randn(HD, generator=g, device=DEV)
+    tab, base = np.cumsum([0] + pages[:-1]), np.cumsum([0] + ms[:-1])
+    st["scale"] = 1.0 / math.sqrt(d)
+    tree = c.get("mask") == "tree"
+    if tree:
+        st["seen"] = [tree_mask(m) for m in ms]
+        bits = np.concatenate([(s.astype(np.uint64) << np.arange(s.shape[0], dtype=np.uint64)[None, :]).sum(axis=1, dtype=np.uint64) for s in st["seen"]])
+        st["anc"] = torch.from_numpy(bits.view(np.int64)).to(DEV)
+    st["desc"] = torch.zeros((rows, 4), dtype=torch.int32, device=DEV)
+    # the same as padded index tables, for the plain form
+    M, P = max(ms), max(ps)
+    r = np.arange(M)[None, :]
+    st["row"] = torch.from_numpy(np.minimum(base[:, None] + r, rows - 1)).to(DEV)
+    st["row_ok"] = torch.from_numpy(r < np.array(ms)[:, None]).to(DEV)
+    j = np.arange(P)[None, :]
+    at = np.minimum(tab[:, None] + j // bt, len(blocks) - 1)
+    st["page"] = torch.from_numpy(blocks[at].astype(np.int64)).to(DEV)
+    st["in_page"] = torch.from_numpy(np.broadcast_to(j % bt, at.shape).copy()).to(DEV)
+    st["key_ok"] = torch.from_numpy(j < np.array(ps)[:, None]).to(DEV)
+    own_ok = np.zeros((len(ms), M, M), dtype=bool)
+    for b, m in enumerate(ms):
+        own_ok[b, :m, :m] = st["seen"][b] if tree else np.tril(np.ones((m, m), dtype=bool))
+    st["own_ok"] = torch.from_numpy(own_ok).to(DEV)
+    st["flat"] = torch.from_numpy(np.concatenate([b * M + np.arange(m) for b, m in enumerate(ms)])).to(DEV)
+    st["ms"], st["ps"], st["tab"], st["base"], st["n_blocks"] = ms, ps, tab, base, n_blocks
+    if own:
+        from espetero_b200 import capi, host
+        dt = {"f16": capi.ESP_F16, "bf16": capi.ESP_BF16, "e4m3": capi.ESP_E4M3}
+        trees = host.make_trees(ms, ps, tab)
+        tile_rows, opts = host.diff_plan_options(trees, H, Hkv, HD)
+        st["op"] = host.AttnOp(H, Hkv, HD, bt, dt[c["dtype"]], dt[c["pool"]], st["scale"], capi.ESP_ATTN_FLAG_ANC_MASK if tree else 0, tile_rows)
+        plan = host.plan_tiles(trees, Hkv, **opts)
+        st["call"] = st["op"].diff_call(plan, trees, st["Q"], st["Kb"], st["Vb"], st["O"], kv=st["pool"], kv_scales=st["scales"], blocks=st["blocks"], n_blocks=n_blocks,
+                                        desc=st["desc"], anc_mask=st["anc"] if tree else None, lam=st["lam"], norm_w=st["w"], eps=EPS, out_scale=OUT_SCALE)
+    return st
+
+
+# ------------------------------------------------------------------------------------------------ plain forms
+def rotated(x, cos, sin, half, pairs):
+    """x [rows, heads, maps, D]: the first 2 * half dims of every map turned by the row's angles."""
+    cos, sin, rest = cos[:, None, None, :], sin[:, None, None, :], x[..., 2 * half:]
+    if pairs == "adjacent":
+        a, b = x[..., 0:2 * half:2], x[..., 1:2 * half:2]
+        return torch.cat([torch.stack([a * cos - b * sin, b * cos + a * sin], dim=-1).flatten(-2), rest], dim=-1)
+    a, b = x[..., :half], x[..., half:2 * half]
+    return torch.cat([a * cos - b * sin, b * cos + a * sin, rest], dim=-1)
+
+
+def plain_append(st):
+    c = st["c"]
+    H, Hkv, HD, maps, half = c["H"], c["Hkv"], c["HD"], c["maps"], c["rot"] // 2
+    rows, t16 = c["rows"], T16[c["dtype"]]
+    angle = st["pos"].double()[:, None] * st["inv_freq"].double()[None, :]
+    cos, sin = torch.cos(angle).float(), torch.sin(angle).float()
+    X = st["X"].float()
+    q, k, v = X.split([H * HD, Hkv * HD, Hkv * HD], dim=1)
+    q = rotated(q.reshape(rows, H, maps, HD // maps), cos, sin, half, c["pairs"]).reshape(rows, H * HD).to(t16)
+    k = rotated(k.reshape(rows, Hkv, maps, HD // maps), cos, sin, half, c["pairs"]).reshape(rows, Hkv * HD).to(t16)
+    v = v.to(t16)
+    block = torch.where(st["slots"][:, 0] < 0, st["n_blocks"], st["slots"][:, 0]).long()
+    at = st["slots"][:, 1].long()
+    kv = torch.stack([k, v], dim=1).reshape(rows, 2, Hkv, HD)
+    if c["pool"] == "e4m3":
+        kv = (kv.float() / st["scales"][block][..., None]).clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8)
+    st["pool"][block, :, at] = kv
+    return q, k, v
+
+
+def plain_attention(st):
+    c = st["c"]
+    H, Hkv, HD, G = c["H"], c["Hkv"], c["HD"], c["H"] // c["Hkv"]
+    d, B = HD // 2, len(st["ms"])
+    M, P = st["row"].shape[1], st["page"].shape[1]
+    keys, vals = st["pool"][st["page"], 0, st["in_page"]], st["pool"][st["page"], 1, st["in_page"]]  # [B, P, Hkv, HD]
+    if c["pool"] == "e4m3":
+        keys = keys.view(torch.float8_e4m3fn).float() * st["scales"][st["page"], 0][..., None]
+        vals = vals.view(torch.float8_e4m3fn).float() * st["scales"][st["page"], 1][..., None]
+    keys = torch.cat([keys.float(), st["Kb"][st["row"]].float().reshape(B, M, Hkv, HD)], dim=1)
+    vals = torch.cat([vals.float(), st["Vb"][st["row"]].float().reshape(B, M, Hkv, HD)], dim=1).permute(0, 2, 1, 3)  # [B, Hkv, K, HD]
+    keys = keys.reshape(B, P + M, Hkv, 2, d).permute(3, 0, 2, 4, 1)  # [2, B, Hkv, d, K]
+    q = st["Q"][st["row"]].float().reshape(B, M, Hkv, G, 2, d).permute(4, 0, 2, 3, 1, 5).reshape(2, B, Hkv, G * M, d)
+    seen = torch.cat([st["key_ok"][:, None, :].expand(B, M, P), st["own_ok"]], dim=2)[:, None, None]  # [B, 1, 1, M, K]
+
+    def one_map(q, k):
+        s = (q @ k).mul_(st["scale"]).reshape(B, Hkv, G, M, P + M).masked_fill_(~seen, -math.inf)
+        top = s.amax(dim=-1, keepdim=True)
+        p = s.sub_(torch.where(top == -math.inf, 0.0, top)).exp_()
+        total = p.sum(dim=-1, keepdim=True)
+        o = (p.reshape(B, Hkv, G * M, P + M) @ vals).reshape(B, Hkv, G, M, HD)
+        return torch.where(total > 0, o / total, 0.0)
+
+    diff = one_map(q[0], keys[0]) - st["lam"].reshape(1, Hkv, G, 1, 1) * one_map(q[1], keys[1])
+    o = OUT_SCALE * st["w"] * diff / torch.sqrt(diff.square().mean(dim=-1, keepdim=True) + EPS)
+    o = o.permute(0, 3, 1, 2, 4).reshape(B * M, H * HD)
+    return o[st["flat"]].to(T16[c["dtype"]])
+
+
+def run(st):
+    c = st["c"]
+    if c["op"] == "append":
+        if own:
+            st["op"].kv_append(st["call"])
+            q, k, v = st["q"], st["k"], st["v"]
+        else:
+            q, k, v = plain_append(st)
+        pool = st["pool"][:st["n_blocks"]]
+        return {"q": q, "k": k, "v": v, "pool": pool.view(torch.float8_e4m3fn) if c["pool"] == "e4m3" else pool}
+    if own:
+        st["op"].diff_forward(st["call"])
+        return {"o": st["O"]}
+    return {"o": plain_attention(st)}
+
+
+# ------------------------------------------------------------------------------------------------ 64 bits
+def exact(c, seed):
+    st = prepare(c, seed)
+    H, Hkv, HD = c["H"], c["Hkv"], c["HD"]
+    if c["op"] == "append":
+        rows, maps, n = c["rows"], c["maps"], c["rot"] // 2
+        turn = torch.polar(torch.ones((), dtype=torch.float64, device=DEV), st["pos"].double()[:, None] * st["inv_freq"].double())[:, None, :]
+
+        def rot(x, heads):
+            x = x.double().reshape(rows, heads * maps, HD // maps).clone()
+            at = (slice(0, 2 * n, 2), slice(1, 2 * n, 2)) if c["pairs"] == "adjacent" else (slice(0, n), slice(n, 2 * n))
+            z = torch.complex(x[..., at[0]], x[..., at[1]]) * turn
+            x[..., at[0]], x[..., at[1]] = z.real, z.imag
+            return x.reshape(rows, heads * HD)
+
+        q, k = rot(st["X"][:, :H * HD], H), rot(st["X"][:, H * HD:(H + Hkv) * HD], Hkv)
+        v = st["X"][:, (H + Hkv) * HD:].double()
+        raw = st["pool"][:st["n_blocks"]]
+        pool = (raw.view(torch.float8_e4m3fn) if c["pool"] == "e4m3" else raw).double()
+        slots = st["slots"].cpu().numpy()
+        live = np.flatnonzero(slots[:, 0] >= 0)
+        b, s = torch.from_numpy(slots[live, 0].astype(np.int64)).to(DEV), torch.from_numpy(slots[live, 1].astype(np.int64)).to(DEV)
+        for which, x in ((0, k), (1, v)):
+            x = x[torch.from_numpy(live).to(DEV)].reshape(-1, Hkv, HD)
+            if c["pool"] == "e4m3":
+                x = (x / st["scales"][b, which].double()[..., None]).clamp(-448, 448)
+            pool[b, which, s] = x
+        return {"q": q, "k": k, "v": v, "pool": pool}
+    G, d = H // Hkv, HD // 2
+    out = torch.zeros((sum(st["ms"]), H, HD), dtype=torch.float64, device=DEV)
+    for b, (m, p) in enumerate(zip(st["ms"], st["ps"])):
+        r0 = int(st["base"][b])
+        pages = st["blocks"][int(st["tab"][b]):int(st["tab"][b]) + (p + c["bt"] - 1) // c["bt"]].long()
+        kept = st["pool"][pages].permute(1, 0, 2, 3, 4)  # [2, pages, bt, Hkv, HD]
+        if c["pool"] == "e4m3":
+            kept = kept.view(torch.float8_e4m3fn).double() * st["scales"][pages].double().permute(1, 0, 2)[:, :, None, :, None]
+        kept = kept.double().reshape(2, -1, Hkv, HD)[:, :p]
+        fresh = torch.stack([x[r0:r0 + m].double().reshape(m, Hkv, HD) for x in (st["Kb"], st["Vb"])])
+        every = torch.cat([kept, fresh], dim=1)
+        hidden = torch.from_numpy(st["seen"][b]).to(DEV).logical_not() if "seen" in st else torch.ones((m, m), device=DEV).triu(1).bool()
+        for h in range(H):
+            q = st["Q"][r0:r0 + m].double().reshape(m, H, 2, d)[:, h]
+            maps = []
+            for i in range(2):
+                s = q[:, i] @ every[0, :, h // G, i * d:(i + 1) * d].T * st["scale"]
+                s[:, p:][hidden] = -math.inf
+                maps.append(torch.softmax(s, dim=1))
+            dif = (maps[0] - st["lam"][h].double() * maps[1]) @ every[1, :, h // G]
+            out[r0:r0 + m, h] = OUT_SCALE * st["w"].double() * dif / torch.sqrt((dif * dif).mean(dim=1, keepdim=True) + EPS)
+    return {"o": out.reshape(-1, H * HD)}

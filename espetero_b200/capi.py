@@ -78,6 +78,19 @@ class PrepParams(C.Structure):
                 ("eps", C.c_float), ("qscale", C.c_float), ("bt", C.c_int32), ("reserved", C.c_int32), ("kv_base", C.c_uint64)]
 
 
+class AppendArgs(C.Structure):
+    _fields_ = [("Q", C.c_void_p), ("K", C.c_void_p), ("V", C.c_void_p), ("Qo", C.c_void_p), ("Kb", C.c_void_p), ("Vb", C.c_void_p),
+                ("kv", C.c_void_p), ("kv_scales", C.c_void_p), ("slots", C.c_void_p), ("pos", C.c_void_p), ("inv_freq", C.c_void_p),
+                ("q_src_ld", C.c_int64), ("k_src_ld", C.c_int64), ("v_src_ld", C.c_int64), ("rows", C.c_int32), ("src_f32", C.c_int32),
+                ("maps", C.c_int32), ("rot_half", C.c_int32), ("adjacent", C.c_int32), ("n_blocks", C.c_int32), ("qscale", C.c_float),
+                ("reserved", C.c_int32), ("p", Params)]
+
+
+class DiffArgs(C.Structure):
+    _fields_ = [("lam", C.c_void_p), ("norm_w", C.c_void_p), ("lam_ld", C.c_int32), ("eps", C.c_float), ("out_scale", C.c_float),
+                ("reserved", C.c_int32)]
+
+
 class ProfileEntry(C.Structure):
     _fields_ = [("kernel", C.c_char * 32), ("launches", C.c_uint32), ("gpu_ms", C.c_float)]
 
@@ -129,6 +142,11 @@ PROTOTYPES = {
                                    C.POINTER(C.c_int32), C.POINTER(C.c_int32), C.c_int32, C.c_int32, C.c_uint64, C.c_uint64,
                                    C.c_void_p, C.c_int32, C.c_uint64]),
     "esp_attn_prep": (C.c_int, [C.c_void_p] * 14 + [C.c_int32, C.POINTER(PrepParams)]),
+    "esp_kv_append": (C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(AppendArgs)]),
+    "esp_diff_forward": (C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(Args), C.POINTER(DiffArgs)]),
+    "esp_diff_parts_floats": (C.c_size_t, [C.POINTER(Shape), C.c_int32]),
+    "esp_diff_plan_opts": (C.c_int, [C.POINTER(Shape), C.POINTER(Tree), C.c_int32, C.POINTER(PlanOpts)]),
+    "esp_diff_lambda": (C.c_int, [C.c_void_p] * 5 + [C.c_int32] * 3 + [C.c_float, C.c_void_p]),
     "esp_kv_save": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32,
                               C.POINTER(Params)]),
     "esp_kv_copy_blocks": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.POINTER(Params), C.c_uint64,

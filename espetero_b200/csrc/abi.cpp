@@ -141,8 +141,7 @@ int check_shape(const esp_attn_shape& s) {
   return ESP_OK;
 }
 
-int check_params(const esp_attn_ctx* c, const esp_attn_params& p) {
-  const esp_attn_shape& s = c->shape;
+int check_params(const esp_attn_shape& s, const esp_attn_params& p) {
   if (p.H != s.H || p.Hkv != s.Hkv || p.bt != s.bt) return fail(ESP_ERR_INVALID, "params: H/Hkv/bt (%d/%d/%d) differ from the context's (%d/%d/%d)", p.H, p.Hkv, p.bt, s.H, s.Hkv, s.bt);
   if (p.q_ld < s.H * s.HD || p.q_ld % 8) return fail(ESP_ERR_INVALID, "params: q_ld=%d (>= H*HD, multiple of 8)", p.q_ld);
   if (p.kv_ld < s.Hkv * s.HD || p.kv_ld % 16) return fail(ESP_ERR_INVALID, "params: kv_ld=%d (>= Hkv*HD, multiple of 16)", p.kv_ld);
@@ -150,6 +149,8 @@ int check_params(const esp_attn_ctx* c, const esp_attn_params& p) {
   if ((s.flags & ESP_ATTN_FLAG_GATE) && (p.g_ld < s.H * 2 * s.HD || p.g_ld % 4)) return fail(ESP_ERR_INVALID, "params: g_ld=%d (>= 2*H*HD, multiple of 4)", p.g_ld);
   return ESP_OK;
 }
+
+int check_params(const esp_attn_ctx* c, const esp_attn_params& p) { return check_params(c->shape, p); }
 
 bool windowed_lists(const esp_attn_args& a) { return a.qsa_tlist != nullptr; }
 
@@ -1103,6 +1104,172 @@ int esp_kv_copy_blocks(esp_attn_ctx* c, void* stream, void* kv, const int32_t* p
   if ((region_elems * esz) % 16) return fail(ESP_ERR_INVALID, "esp_kv_copy_blocks: region size must be a multiple of 16 bytes");
   const cudaError_t e = esp::launch_kv_copy_blocks(kv, pairs, n_pairs, *p, region_elems, n_layers, esz, static_cast<cudaStream_t>(stream), &c->launches);
   if (e != cudaSuccess) return cuda_fail(e, "kv_copy_blocks");
+  return ESP_OK;
+}
+
+}  // extern "C"
+
+// Host-side checks of the two calls below; nothing is launched when one fails.
+int esp::check_kv_append(const esp_attn_shape& s, const esp_kv_append_args& a) {
+  if (a.rows < 0) return fail(ESP_ERR_INVALID, "esp_kv_append: rows=%d", a.rows);
+  if (a.rows == 0) return ESP_OK;
+  if (!a.K || !a.V || (a.Q && !a.Qo)) return fail(ESP_ERR_INVALID, "esp_kv_append: null K / V, or queries without Qo");
+  if (!a.kv && !(a.Kb && a.Vb)) return fail(ESP_ERR_INVALID, "esp_kv_append: keys and values need the pool or both Kb and Vb");
+  if (a.src_f32 != 0 && a.src_f32 != 1) return fail(ESP_ERR_INVALID, "esp_kv_append: src_f32=%d", a.src_f32);
+  if (a.maps != 1 && a.maps != 2) return fail(ESP_ERR_INVALID, "esp_kv_append: maps=%d (1 or 2)", a.maps);
+  if (a.rot_half < 0 || 2 * int64_t(a.rot_half) > s.HD / a.maps) return fail(ESP_ERR_INVALID, "esp_kv_append: rot_half=%d (2 * rot_half <= %d)", a.rot_half, s.HD / a.maps);
+  if (a.rot_half > 0 && (!a.pos || !a.inv_freq)) return fail(ESP_ERR_INVALID, "esp_kv_append: a rotation needs pos and inv_freq");
+  const int64_t ssz = a.src_f32 ? 4 : 2;
+  const struct { const void* p; int64_t ld, heads, align; const char* name; } src[3] = {
+      {a.Q, a.q_src_ld, s.H, ssz, "Q"}, {a.K, a.k_src_ld, s.Hkv, ssz, "K"}, {a.V, a.v_src_ld, s.Hkv, ssz, "V"}};
+  for (const auto& x : src) {
+    if (!x.p) continue;
+    if (x.ld < x.heads * s.HD) return fail(ESP_ERR_INVALID, "esp_kv_append: %s rows are %lld elements apart, %lld heads of %d need more", x.name, (long long)x.ld, (long long)x.heads, s.HD);
+    if (reinterpret_cast<uintptr_t>(x.p) % uintptr_t(x.align)) return fail(ESP_ERR_INVALID, "esp_kv_append: %s is not aligned to its type", x.name);
+  }
+  for (const void* q : {static_cast<const void*>(a.Qo), static_cast<const void*>(a.Kb), static_cast<const void*>(a.Vb)})
+    if (reinterpret_cast<uintptr_t>(q) & 1) return fail(ESP_ERR_INVALID, "esp_kv_append: outputs must be aligned to their type");
+  // an output may lie on its source only where every element keeps its place
+  const struct { const void* src; const void* dst; int64_t src_ld, dst_ld; const char* name; } pairs[3] = {
+      {a.Q, a.Qo, a.q_src_ld, a.p.q_ld, "Qo on Q"}, {a.K, a.Kb, a.k_src_ld, a.p.kv_ld, "Kb on K"}, {a.V, a.Vb, a.v_src_ld, a.p.kv_ld, "Vb on V"}};
+  for (const auto& x : pairs)
+    if (x.src && x.src == x.dst && (a.src_f32 || (a.rows > 1 && x.src_ld != x.dst_ld)))
+      return fail(ESP_ERR_INVALID, "esp_kv_append: %s needs 16-bit sources and equal row strides", x.name);
+  if (int rc = check_params(s, a.p)) return rc;
+  if (a.kv) {
+    if (!a.slots || a.n_blocks <= 0) return fail(ESP_ERR_INVALID, "esp_kv_append: a pool needs slots and n_blocks");
+    if (!aligned16(a.kv) || (reinterpret_cast<uintptr_t>(a.slots) & 7)) return fail(ESP_ERR_INVALID, "esp_kv_append: the pool must be 16-byte aligned, slots 8-byte aligned");
+    if (s.kv_dtype == ESP_E4M3 && !a.kv_scales) return fail(ESP_ERR_INVALID, "esp_kv_append: E4M3 pool needs kv_scales");
+  }
+  return ESP_OK;
+}
+
+int esp::check_diff_pass(const esp_attn_shape& s, int TR, bool deep, const esp_attn_args& a, const esp_diff_args& d) {
+  if (s.flags & ESP_ATTN_FLAG_GATE) return fail(ESP_ERR_UNSUPPORTED, "esp_diff_forward: no output gate");
+  if (a.window || a.ring || a.bidi || a.qsa_tlist) return fail(ESP_ERR_UNSUPPORTED, "esp_diff_forward: no sliding windows, rings, image rows or sparse lists");
+  if (a.lse) return fail(ESP_ERR_INVALID, "esp_diff_forward: two maps have no one log-sum-exp: lse must be NULL");
+  if (!d.lam || (d.lam_ld != 0 && d.lam_ld < s.H)) return fail(ESP_ERR_INVALID, "esp_diff_forward: lam is null, or lam_ld=%d (0, or >= H=%d)", d.lam_ld, s.H);
+  if (!(d.eps >= 0.0f) || !(d.out_scale == d.out_scale)) return fail(ESP_ERR_INVALID, "esp_diff_forward: eps / out_scale");
+  if (!aligned16(d.norm_w)) return fail(ESP_ERR_INVALID, "esp_diff_forward: norm_w must be 16-byte aligned");
+  if (int rc = check_params(s, a.p)) return rc;
+  return esp::validate_pass(s, TR, deep, a);
+}
+
+// The entry points below may be called with another device current: they launch on their context's.
+namespace {
+struct DeviceScope {
+  int before = -1;
+  cudaError_t err;
+  explicit DeviceScope(int device) {
+    err = cudaGetDevice(&before);
+    if (err == cudaSuccess && before != device) err = cudaSetDevice(device);
+    else before = -1;
+  }
+  ~DeviceScope() {
+    if (before >= 0) cudaSetDevice(before);
+  }
+};
+}  // namespace
+
+extern "C" {
+
+int esp_kv_append(esp_attn_ctx* c, void* stream, const esp_kv_append_args* ap) {
+  if (!c || !ap) return fail(ESP_ERR_INVALID, "esp_kv_append: null argument");
+  const esp_kv_append_args& a = *ap;
+  const esp_attn_shape& s = c->shape;
+  if (int rc = esp::check_kv_append(s, a)) return rc;
+  if (a.rows == 0) return ESP_OK;
+  const bool fp8 = s.kv_dtype == ESP_E4M3;
+  DeviceScope dev(c->device);
+  if (dev.err != cudaSuccess) return cuda_fail(dev.err, "esp_kv_append: device");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  ProfScope prof(c, st, "kv_append");
+  const cudaError_t e = esp::launch_kv_append(esp::AppendArgs{a, c->d_status}, s.HD, s.q_dtype, fp8 && a.kv, st, &c->launches);
+  if (e != cudaSuccess) return cuda_fail(e, "kv_append");
+  return ESP_OK;
+}
+
+size_t esp_diff_parts_floats(const esp_attn_shape* s, int32_t n_parts) { return 2 * esp_attn_parts_floats(s, n_parts); }
+
+int esp_diff_plan_opts(const esp_attn_shape* s, const esp_attn_tree* trees, int32_t n_trees, esp_plan_opts* o) {
+  if (!s || !o || n_trees < 0 || (!trees && n_trees > 0)) return fail(ESP_ERR_INVALID, "esp_diff_plan_opts: null or negative argument");
+  if (s->H <= 0 || s->Hkv <= 0 || s->H % s->Hkv) return fail(ESP_ERR_INVALID, "esp_diff_plan_opts: H=%d Hkv=%d", s->H, s->Hkv);
+  int64_t cached = 0, fresh = 0;
+  bool single = true;
+  for (int i = 0; i < n_trees; ++i) {
+    const esp_attn_tree& t = trees[i];
+    if (t.M < 0 || t.P < 0) return fail(ESP_ERR_INVALID, "esp_diff_plan_opts: tree %d has a negative field", i);
+    single = single && t.M == 1;
+    cached += int64_t(t.P) * t.M, fresh += int64_t(t.M) * t.M / 2;
+  }
+  *o = esp_plan_opts{};
+  o->mode = ESP_PLAN_B200, o->min_chunk = 32, o->max_parts = 64;
+  const int G = s->H / s->Hkv;
+  if (single) {
+    o->tile_rows = 8, o->groups = 148 * 4, o->split = 1 << 20;
+    return ESP_OK;
+  }
+  if (cached <= 2 * fresh) {  // mostly its own rows: 128-row tiles, one head each, nothing split
+    o->tile_rows = 128, o->groups = 148, o->split = 0;
+    return ESP_OK;
+  }
+  int c = 8;  // heads per tile
+  while (c > 1 && (c > G || G % c)) c >>= 1;
+  o->tile_rows = 128 / c, o->groups = std::max(1, 148 * c / G), o->split = 1 << 20;
+  return ESP_OK;
+}
+
+int esp_diff_forward(esp_attn_ctx* c, void* stream, const esp_attn_args* ap, const esp_diff_args* dp) {
+  if (!c || !ap || !dp) return fail(ESP_ERR_INVALID, "esp_diff_forward: null argument");
+  const esp_attn_args& a = *ap;
+  const esp_attn_shape& s = c->shape;
+  if (int rc = esp::check_diff_pass(s, c->tile_rows, c->opt_validate != 0, a, *dp)) return rc;
+  ++c->pass_count;
+  if (c->fail_every > 0 && a.n_rows >= 64 && c->pass_count % uint64_t(c->fail_every) == 0)
+    return fail(ESP_ERR_INJECTED, "differential attention pass failed: injected (ESPETERO_FAIL_PASS)");
+  if (a.n_tiles == 0) return ESP_OK;
+  DeviceScope dev(c->device);
+  if (dev.err != cudaSuccess) return cuda_fail(dev.err, "esp_diff_forward: device");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+
+  esp::DiffArgs d{};
+  esp::KernelArgs& k = d.k;
+  k.Q = a.Q, k.Kb = a.Kb, k.Vb = a.Vb, k.kv = a.kv, k.kv_scales = a.kv_scales, k.blocks = a.blocks;
+  k.desc = (s.flags & ESP_ATTN_FLAG_ANC_MASK) ? nullptr : a.desc;
+  k.anc_mask = (s.flags & ESP_ATTN_FLAG_ANC_MASK) ? a.anc_mask : nullptr;
+  k.O = a.O, k.parts = a.parts, k.tiles = a.tiles, k.trees = a.trees, k.jobs = a.jobs, k.status = c->d_status, k.counters = c->d_status + 64;
+  k.p = a.p, k.HD = s.HD, k.G = c->G, k.tile_rows = c->tile_rows, k.n_tiles = a.n_tiles;
+  k.q_dtype = s.q_dtype, k.kv_dtype = s.kv_dtype, k.n_blocks = a.n_blocks, k.scale = s.scale;
+  k.n_trees = a.n_trees, k.n_block_entries = a.n_block_entries;
+  d.lam = dp->lam, d.norm_w = dp->norm_w, d.lam_ld = dp->lam_ld, d.eps = dp->eps, d.out_scale = dp->out_scale;
+
+  cudaError_t e;
+  {
+    c->last_kernel = "diff_general";
+    ProfScope prof(c, st, c->last_kernel);
+    e = esp::launch_diff_general(d, st, &c->launches);
+  }
+  if (e != cudaSuccess) return cuda_fail(e, c->last_kernel);
+  if (a.n_jobs > 0) {
+    esp::DiffCombineArgs m{d, a.n_jobs, c->tile_rows};
+    if (a.jobs_host) {
+      m.rows_max = 1;
+      for (int i = 0; i < a.n_jobs; ++i) m.rows_max = std::max(m.rows_max, a.jobs_host[i].rows);
+    }
+    ProfScope prof(c, st, "diff_combine");
+    e = esp::launch_diff_combine(m, st, &c->launches);
+    if (e != cudaSuccess) return cuda_fail(e, "diff_combine");
+  }
+  return ESP_OK;
+}
+
+int esp_diff_lambda(void* stream, const float* q1, const float* k1, const float* q2, const float* k2, int32_t H, int32_t dim, int32_t ld,
+                    float lambda_init, float* lam) {
+  if (H < 0 || dim <= 0 || (ld != 0 && ld < dim)) return fail(ESP_ERR_INVALID, "esp_diff_lambda: H=%d dim=%d ld=%d (0, or >= dim)", H, dim, ld);
+  if (H == 0) return ESP_OK;
+  if (!q1 || !k1 || !q2 || !k2 || !lam) return fail(ESP_ERR_INVALID, "esp_diff_lambda: null pointer");
+  const cudaError_t e = esp::launch_diff_lambda(q1, k1, q2, k2, H, dim, ld, lambda_init, lam, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "diff_lambda");
   return ESP_OK;
 }
 

@@ -198,11 +198,39 @@ struct PrepArgs {
   esp_attn_prep_params p;
 };
 
+// kv_append: rotation, cast and the paged write of the new tokens' projection.
+struct AppendArgs {
+  esp_kv_append_args a;
+  int* status;
+};
+cudaError_t launch_kv_append(const AppendArgs& a, int32_t HD, int32_t q_dtype, bool fp8_pool, cudaStream_t stream, uint64_t* launches);
+
+// Differential attention: what the attention kernels get, and how a row is finished. Records hold two maps per
+// (part, kv head, row, head): record_of(...) * (HD + 2) floats into `parts`.
+struct DiffArgs {
+  KernelArgs k;
+  const float* lam;
+  const float* norm_w;
+  int32_t lam_ld;
+  float eps, out_scale;
+};
+struct DiffCombineArgs {
+  DiffArgs d;
+  int32_t n_jobs, rows_max;
+};
+cudaError_t launch_diff_general(const DiffArgs& a, cudaStream_t stream, uint64_t* launches);
+cudaError_t launch_diff_combine(const DiffCombineArgs& a, cudaStream_t stream, uint64_t* launches);
+cudaError_t launch_diff_lambda(const float* q1, const float* k1, const float* q2, const float* k2, int32_t H, int32_t dim, int32_t ld,
+                               float lambda_init, float* lam, cudaStream_t stream);
+
 // Host-side checks of a pass before anything is launched (the checks run_forest makes,
 // src/model/impl/forest.h:2136-2280): pointers, alignment, and - with `deep` - every tree, tile and
 // combine job of the host mirrors against the row, block-table and record counts of `a`.
 // Returns ESP_OK or a negative esp_status with the message set.
 int validate_pass(const esp_attn_shape& s, int tile_rows, bool deep, const esp_attn_args& a);
+
+int check_kv_append(const esp_attn_shape& s, const esp_kv_append_args& a);
+int check_diff_pass(const esp_attn_shape& s, int tile_rows, bool deep, const esp_attn_args& a, const esp_diff_args& d);
 
 // Launch with programmatic stream serialization: the grid may be scheduled while the previous
 // kernel of the stream drains; the kernel orders itself with griddepcontrol.wait.

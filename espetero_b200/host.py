@@ -60,6 +60,31 @@ def plan_window(trees: np.ndarray, groups: int, split: int = 512, rows: int = 8,
     return Plan(tiles[:nt.value], jobs[:nj.value], np_.value, pr.value)
 
 
+def make_trees(rows, cached, tables) -> np.ndarray:
+    """Tree records of a pass whose tree i has rows[i] rows behind cached[i] keys, block list at tables[i]."""
+    trees = np.zeros(len(rows), dtype=TREE_DT)
+    trees["M"], trees["P"], trees["table"] = rows, cached, tables
+    trees["base"] = np.cumsum([0] + [int(m) for m in rows[:-1]])
+    return trees
+
+
+def diff_plan_options(trees: np.ndarray, H: int, Hkv: int, HD: int):
+    """esp_diff_plan_opts: (tile_rows for the context, keyword arguments for plan_tiles)."""
+    o = capi.PlanOpts()
+    shape = capi.Shape(H, Hkv, HD)
+    trees = np.ascontiguousarray(trees, dtype=TREE_DT)
+    capi.check(capi.load().esp_diff_plan_opts(C.byref(shape), trees.ctypes.data_as(C.POINTER(capi.Tree)), len(trees), C.byref(o)))
+    return o.tile_rows, dict(mode=o.mode, split=o.split, min_chunk=o.min_chunk, groups=o.groups, tile_rows=o.tile_rows, max_parts=o.max_parts)
+
+
+@dataclass
+class Call:
+    """Arguments of one call and what they point to (device tensors, host records), kept alive together."""
+    args: C.Structure
+    more: C.Structure | None
+    keep: tuple
+
+
 def _dev(arr: np.ndarray | None, device, pin: bool = False):
     if arr is None:
         return None
@@ -272,6 +297,62 @@ class AttnOp:
         capi.check(self.lib.esp_attn_prep(self.ctx, C.c_void_p(s), _ptr(X), _ptr(qn_w), _ptr(kn_w), _ptr(pos), _ptr(inv_freq),
                                           _ptr(rope_sel), _ptr(Q), _ptr(Kb), _ptr(Vb), _ptr(ktab), _ptr(kv), _ptr(kv_scales),
                                           X.shape[0], C.byref(pp)))
+
+    def append_call(self, Q, K, V, Qo=None, Kb=None, Vb=None, kv=None, kv_scales=None, n_blocks=0, slots=None, pos=None, inv_freq=None,
+                    maps=1, adjacent=False, qscale=1.0, kv_base=0) -> Call:
+        """Arguments of esp_kv_append from device tensors: Q / K / V are [rows, heads * HD] with any row stride, 16-bit or fp32."""
+        s, a = self.shape, capi.AppendArgs()
+        a.Q, a.K, a.V, a.Qo, a.Kb, a.Vb = (_ptr(t) for t in (Q, K, V, Qo, Kb, Vb))
+        a.kv, a.kv_scales, a.slots, a.pos, a.inv_freq = (_ptr(t) for t in (kv, kv_scales, slots, pos, inv_freq))
+        a.q_src_ld, a.k_src_ld, a.v_src_ld = 0 if Q is None else Q.stride(0), K.stride(0), V.stride(0)
+        a.rows, a.src_f32, a.maps, a.adjacent = K.shape[0], int(K.dtype == torch.float32), maps, int(adjacent)
+        a.rot_half, a.n_blocks, a.qscale = 0 if inv_freq is None else inv_freq.numel(), n_blocks, qscale
+        a.p = capi.Params(s.H, s.Hkv, s.H * s.HD if Qo is None else Qo.stride(0), s.Hkv * s.HD, 2 * s.H * s.HD, s.bt, kv_base)
+        return Call(a, None, (Q, K, V, Qo, Kb, Vb, kv, kv_scales, slots, pos, inv_freq))
+
+    def kv_append(self, call: Call, stream: int | None = None):
+        """esp_kv_append on torch's current stream (or the given cudaStream_t)."""
+        s = torch.cuda.current_stream(self.device).cuda_stream if stream is None else stream
+        capi.check(self.lib.esp_kv_append(self.ctx, C.c_void_p(s), C.byref(call.args)))
+
+    def diff_call(self, plan: Plan, trees: np.ndarray, Q, Kb, Vb, O, kv=None, kv_scales=None, blocks=None, n_blocks=0, desc=None,
+                  anc_mask=None, lam=None, lam_ld=0, norm_w=None, eps=0.0, out_scale=1.0, kv_base=0, parts=None, scratch=None) -> Call:
+        """Arguments of esp_diff_forward from a plan and device tensors; `parts` (and, over an E4M3 pool, the scratch of
+        multi-row passes) are allocated unless given."""
+        s, a = self.shape, capi.Args()
+        trees = np.ascontiguousarray(trees, dtype=TREE_DT)
+        tiles_dev, trees_dev, jobs_dev = (_dev(x, self.device) if len(x) else None for x in (plan.tiles, trees, plan.jobs))
+        if parts is None and plan.n_parts:
+            parts = torch.empty(int(self.lib.esp_diff_parts_floats(C.byref(s), plan.n_parts)), dtype=torch.float32, device=self.device)
+        if scratch is None and s.kv_dtype == E4M3 and blocks is not None and bool((trees["M"] > 1).any()) and bool((trees["P"] > 0).any()):
+            scratch = torch.empty(int(self.lib.esp_attn_dequant_scratch_bytes(C.byref(s), blocks.numel())), dtype=torch.uint8, device=self.device)
+        a.Q, a.Kb, a.Vb, a.O, a.kv, a.kv_scales, a.blocks, a.desc, a.anc_mask, a.parts = (
+            _ptr(t) for t in (Q, Kb, Vb, O, kv, kv_scales, blocks, desc, anc_mask, parts))
+        a.tiles, a.trees, a.jobs = _ptr(tiles_dev), _ptr(trees_dev), _ptr(jobs_dev)
+        a.tiles_host = plan.tiles.ctypes.data if len(plan.tiles) else None
+        a.trees_host = trees.ctypes.data
+        a.jobs_host = plan.jobs.ctypes.data if len(plan.jobs) else None
+        a.n_tiles, a.n_trees, a.n_jobs, a.n_rows, a.n_parts = len(plan.tiles), len(trees), len(plan.jobs), Q.shape[0], plan.n_parts
+        a.n_blocks, a.n_block_entries = n_blocks, 0 if blocks is None else blocks.numel()
+        if scratch is not None:
+            a.dequant_scratch, a.dequant_scratch_bytes = scratch.data_ptr(), scratch.numel()
+        a.p = capi.Params(s.H, s.Hkv, Q.stride(0), s.Hkv * s.HD, 2 * s.H * s.HD, s.bt, kv_base)
+        d = capi.DiffArgs(_ptr(lam), _ptr(norm_w), lam_ld, eps, out_scale)
+        return Call(a, d, (plan, trees, tiles_dev, trees_dev, jobs_dev, parts, scratch, Q, Kb, Vb, O, kv, kv_scales, blocks, desc, anc_mask, lam, norm_w))
+
+    def diff_forward(self, call: Call, stream: int | None = None):
+        """esp_diff_forward on torch's current stream (or the given cudaStream_t)."""
+        s = torch.cuda.current_stream(self.device).cuda_stream if stream is None else stream
+        capi.check(self.lib.esp_diff_forward(self.ctx, C.c_void_p(s), C.byref(call.args), C.byref(call.more)))
+
+    def diff_lambda(self, q1, k1, q2, k2, lambda_init: float, H: int | None = None, stream: int | None = None):
+        """esp_diff_lambda: [H, dim] vectors, or one [dim] vector for every head."""
+        s = torch.cuda.current_stream(self.device).cuda_stream if stream is None else stream
+        n = self.shape.H if H is None else H
+        lam = torch.empty(n, dtype=torch.float32, device=self.device)
+        ld = 0 if q1.dim() == 1 else q1.stride(0)
+        capi.check(self.lib.esp_diff_lambda(C.c_void_p(s), _ptr(q1), _ptr(k1), _ptr(q2), _ptr(k2), n, q1.shape[-1], ld, lambda_init, _ptr(lam)))
+        return lam
 
     def kv_save(self, dp: DevicePass, entries: np.ndarray, stream: int | None = None):
         s = torch.cuda.current_stream(self.device).cuda_stream if stream is None else stream

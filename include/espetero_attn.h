@@ -451,6 +451,86 @@ int esp_attn_prep(esp_attn_ctx* ctx, void* stream, const float* X, const float* 
                   const int32_t* pos, const float* inv_freq, const int32_t* rope_sel, void* Q, void* Kb, void* Vb,
                   const int32_t* ktab, void* kv, const float* kv_scales, int32_t rows, const esp_attn_prep_params* p);
 
+/* ---- kv_append: the same step for models without a norm on queries and keys, and for differential heads (below). One
+ * launch takes the new tokens' projection, turns queries and keys to their positions, rounds everything once to the
+ * context's q_dtype and writes keys and values into their slots of the paged cache.
+ * Sources: 16-bit rows of q_dtype or (src_f32) fp32 rows; row strides q_src_ld / k_src_ld / v_src_ld in elements, heads HD
+ * apart, so Q, K and V may be column ranges of one fused projection. Any alignment of their element type and any stride is
+ * taken; 16-byte aligned rows are read fastest.
+ * Rotation: each of the `maps` parts of a head (1, or 2 for differential heads; D = HD / maps dims) is rotated by itself:
+ * pairs (f, f + rot_half), or with `adjacent` (2 f, 2 f + 1), f < rot_half, by the angle pos[row] * inv_freq[f], which is
+ * formed exactly (any int32 position); dims from 2 * rot_half on pass through. rot_half = 0: no rotation (pos and inv_freq
+ * are not read). Queries are then multiplied by qscale.
+ * Outputs: Qo (rows q_ld apart), and - each optional, but together at least the pool or both of Kb and Vb - Kb / Vb (rows
+ * kv_ld apart: the batch keys of the attention pass that follows) and the pool. slots: (block, position in block) per row;
+ * block -1 = the row (padding, say) is not stored, though its Qo / Kb / Vb rows are written. A slot outside [0, n_blocks) x [0, bt)
+ * is not written and sets the status word (esp_attn_check_status). Two rows with one slot: one of them is kept, unspecified
+ * which. E4M3 pools take the code of the rounded 16-bit value with the block's scale, exactly as esp_kv_save would.
+ * In place: Qo may be Q, Kb may be K and Vb may be V where type and row stride agree; other overlaps are not allowed.
+ * Limits: HD <= 512, 2 * rot_half <= HD / maps. Nothing is allocated; one launch. */
+typedef struct esp_kv_append_args {
+  const void* Q;          /* [rows] x H heads, or NULL: keys and values only */
+  const void* K;          /* [rows] x Hkv heads */
+  const void* V;
+  void* Qo;               /* [rows][p.q_ld]; needed with Q */
+  void* Kb;               /* [rows][p.kv_ld], or NULL */
+  void* Vb;
+  void* kv;               /* pool, or NULL */
+  const float* kv_scales; /* ESP_E4M3: [n_blocks][2][Hkv] */
+  const int32_t* slots;   /* int2 per row: block, position in block; needed with kv */
+  const int32_t* pos;     /* [rows] */
+  const float* inv_freq;  /* [rot_half] */
+  int64_t q_src_ld, k_src_ld, v_src_ld;
+  int32_t rows;
+  int32_t src_f32;        /* 1: Q, K, V are fp32; 0: q_dtype */
+  int32_t maps;           /* 1 or 2 */
+  int32_t rot_half;
+  int32_t adjacent;
+  int32_t n_blocks;       /* blocks of this layer's pool region */
+  float qscale;
+  int32_t reserved;
+  esp_attn_params p;      /* H, Hkv, q_ld, kv_ld, bt, kv_base (g_ld is not read) */
+} esp_kv_append_args;
+int esp_kv_append(esp_attn_ctx* ctx, void* stream, const esp_kv_append_args* args);
+
+/* ---- Differential attention: a head is the difference of two softmax maps over one value head,
+ *   D_h = softmax(scale * q1 . k1) V - lam_h * softmax(scale * q2 . k2) V,
+ *   O_h = out_scale * norm_w * D_h / sqrt(mean(D_h^2) + eps)       (norm_w NULL: out_scale * D_h),
+ * over the paged cache and the forest passes of this library. HD counts the dims of a whole head: queries and keys hold
+ * [map 1 | map 2] of HD / 2 dims each, values HD dims, so the pool, its planner, its blocks and its checkpoints are those of an
+ * ordinary layer (esp_kv_append with maps = 2 writes it), and shape.scale multiplies products of HD / 2 dims.
+ * esp_diff_forward takes the plan and the arguments of esp_attn_forward with these differences:
+ *  - `parts` holds two records per (part, kv head, row, head), map 1's then map 2's: esp_diff_parts_floats;
+ *  - lse must be NULL (two maps have no one log-sum-exp), the shape must not carry ESP_ATTN_FLAG_GATE, and window, ring,
+ *    bidi and the sparse-attention arguments must be 0 / NULL (ESP_ERR_UNSUPPORTED);
+ *  - tiles are never planned again: esp_diff_plan_opts says which tile height (a property of the context) and planner options
+ *    suit a pass; every plan of esp_attn_plan is right, some are slow (see below).
+ * A row that sees no key gets zeros. Rows that no tile covers are left as they were. Keys behind a tree's last row and pool
+ * rows past P are never mixed in, whatever they hold; keys that another row of the same tree sees must be finite.
+ * Kernels: "diff_decode" (all trees have one row, G <= 8, HD 128 or 256, pages of 16 n keys), "diff_umma" (HD 128) and
+ * "diff_umma_pair" (HD 256) for tiles of 128 / c rows, c heads, c <= G (16-bit pools; E4M3 pools through dequant_scratch as in
+ * esp_attn_forward, and passes without cached keys), "diff_general" for everything else, plus "diff_combine" for split plans.
+ * esp_attn_last_kernel names the first of these. Sums, maxima and the difference are fp32; softmax weights are rounded to the
+ * pass's 16-bit type (fp16 over E4M3 pools in diff_decode) before they meet V. */
+typedef struct esp_diff_args {
+  const float* lam;    /* lam[row * lam_ld + h]: per head, lam_ld = 0, or per row and head, lam_ld >= H */
+  const float* norm_w; /* [HD], or NULL: no norm */
+  int32_t lam_ld;
+  float eps;           /* >= 0 */
+  float out_scale;
+  int32_t reserved;
+} esp_diff_args;
+int esp_diff_forward(esp_attn_ctx* ctx, void* stream, const esp_attn_args* args, const esp_diff_args* diff);
+/* Floats of `parts` for n_parts records. */
+size_t esp_diff_parts_floats(const esp_attn_shape* shape, int32_t n_parts);
+/* Planner options for a pass (pure host): opts->tile_rows is also the tile_rows its context wants. Reads H, Hkv and HD of the
+ * shape. */
+int esp_diff_plan_opts(const esp_attn_shape* shape, const esp_attn_tree* trees_host, int32_t n_trees, esp_plan_opts* opts);
+/* lam[h] = exp(q1_h . k1_h) - exp(q2_h . k2_h) + lambda_init for h < H, from the layer's learned vectors ([H][dim] fp32, rows
+ * ld elements apart; ld = 0: one vector for every head). Once per model load. One launch. */
+int esp_diff_lambda(void* stream, const float* q1, const float* k1, const float* q2, const float* k2, int32_t H, int32_t dim, int32_t ld,
+                    float lambda_init, float* lam);
+
 /* kv_save (40_attention.metal:875-889; forest.h:2935-2947). With an ESP_E4M3
  * pool the rows are quantised with the destination block's scale from kv_scales. */
 int esp_kv_save(esp_attn_ctx* ctx, void* stream, const void* Kb, const void* Vb, void* kv, const float* kv_scales,

@@ -400,6 +400,10 @@ int esp_attn_create(esp_attn_ctx** out, int device, const esp_attn_shape* shape)
     delete c;
     return cuda_fail(e, "tcgen05 kernel setup");
   }
+  if ((e = esp::diff_decode_setup()) != cudaSuccess) {
+    delete c;
+    return cuda_fail(e, "differential kernel setup");
+  }
   if ((e = cudaMalloc(reinterpret_cast<void**>(&c->d_status), kStatusBytes)) != cudaSuccess) {
     delete c;
     return cuda_fail(e, "cudaMalloc(status word)");
@@ -1243,8 +1247,18 @@ int esp_diff_forward(esp_attn_ctx* c, void* stream, const esp_attn_args* ap, con
   k.n_trees = a.n_trees, k.n_block_entries = a.n_block_entries;
   d.lam = dp->lam, d.norm_w = dp->norm_w, d.lam_ld = dp->lam_ld, d.eps = dp->eps, d.out_scale = dp->out_scale;
 
+  bool single = a.trees_host != nullptr && a.tiles_host != nullptr;
+  for (int i = 0; single && i < a.n_trees; ++i) single = a.trees_host[i].M == 1;
+  const bool decode = single && c->opt_attn_gqa && esp::diff_decode_supports(s.HD, c->G, s.bt) && a.kv != nullptr && a.n_blocks > 0 &&
+                      (size_t(a.p.kv_ld) * elem_bytes(s.kv_dtype)) % 128 == 0 && (a.p.kv_base * elem_bytes(s.kv_dtype)) % 128 == 0;
+
   cudaError_t e;
-  {
+  if (decode) {
+    if (int rc = pool_tensor_map(c, a)) return rc;
+    c->last_kernel = "diff_decode";
+    ProfScope prof(c, st, c->last_kernel);
+    e = esp::launch_diff_decode(d, c->pool_map, st, &c->launches);
+  } else {
     c->last_kernel = "diff_general";
     ProfScope prof(c, st, c->last_kernel);
     e = esp::launch_diff_general(d, st, &c->launches);

@@ -85,6 +85,41 @@ def test_general(case, split):
     _check(w, "diff_general", options=GENERAL, tile_rows=8, plan_opts=dict(split=split, groups=4096 if split else 1))
 
 
+LENGTHS = [0, 1, 15, 16, 17, 31, 64, 65, 333, 1024]
+
+
+@gpu
+@pytest.mark.parametrize("HD", [128, 256])
+@pytest.mark.parametrize("heads", [(4, 4), (4, 2), (3, 1), (8, 2), (5, 1), (16, 2)], ids=lambda x: "H%d/%d" % x)
+@pytest.mark.parametrize("types", [(wl.F16, None), (wl.BF16, None), (wl.F16, wl.E4M3), (wl.BF16, wl.E4M3)], ids=["f16", "bf16", "f16-e4m3", "bf16-e4m3"])
+@pytest.mark.parametrize("split", [0, 32], ids=["whole", "split"])
+def test_decode(HD, heads, types, split):
+    w = wl.make_pass("decode", HD + heads[0], [(n, 1) for n in LENGTHS], heads[0], heads[1], HD, 48 if split else 16, types[0], types[1], scale=(HD // 2) ** -0.5)
+    _check(w, "diff_decode", plan_opts=dict(split=split, groups=4096 if split else 1))
+
+
+@gpu
+def test_decode_long_and_hidden_from_itself():
+    w = wl.make_pass("long", 3, [(40000, 1), (9, 1)], 8, 2, 128, 16, wl.BF16, scale=0.125)
+    _check(w, "diff_decode")
+    w = wl.make_pass("hidden", 3, [(100, 1), (0, 1), (0, 1)], 8, 2, 128, 16, wl.BF16, scale=0.125, mask="tree")
+    w.anc_mask[:2] = 0
+    O, _ = _check(w, "diff_decode")
+    assert O[0].any() and not O[1].any() and O[2].any()
+
+
+@gpu
+@pytest.mark.parametrize("pool", [None, wl.E4M3], ids=["16-bit", "e4m3"])
+def test_decode_reports_a_block_outside_the_pool(pool):
+    """The page table's contents are seen by no host check: the kernel reads a block that exists instead and says so."""
+    for options in (None, GENERAL):
+        w = wl.make_pass("bad page", 3, [(100, 1), (50, 1)], 8, 2, 128, 16, wl.BF16, pool, scale=0.125)
+        for bad in (-1, w.n_blocks, 2 ** 30):
+            w.blocks[2] = bad
+            with pytest.raises(capi.EspError, match="bad block id"):
+                _launch(w, *_weights(w, 1), options=options)
+
+
 @gpu
 def test_no_norm_per_row_lambda_and_norm_of_nothing():
     w = wl.make_pass("plain", 5, [(70, 4), (0, 1)], 8, 2, 128, 16, wl.BF16, scale=0.125)

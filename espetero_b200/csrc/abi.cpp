@@ -400,7 +400,7 @@ int esp_attn_create(esp_attn_ctx** out, int device, const esp_attn_shape* shape)
     delete c;
     return cuda_fail(e, "tcgen05 kernel setup");
   }
-  if ((e = esp::diff_decode_setup()) != cudaSuccess) {
+  if ((e = esp::diff_decode_setup()) != cudaSuccess || (e = esp::diff_umma_setup()) != cudaSuccess) {
     delete c;
     return cuda_fail(e, "differential kernel setup");
   }
@@ -1252,12 +1252,42 @@ int esp_diff_forward(esp_attn_ctx* c, void* stream, const esp_attn_args* ap, con
   const bool decode = single && c->opt_attn_gqa && esp::diff_decode_supports(s.HD, c->G, s.bt) && a.kv != nullptr && a.n_blocks > 0 &&
                       (size_t(a.p.kv_ld) * elem_bytes(s.kv_dtype)) % 128 == 0 && (a.p.kv_base * elem_bytes(s.kv_dtype)) % 128 == 0;
 
+  // Multi-row tiles: the tcgen05 kernels, over 16-bit pages. An E4M3 pool is widened into the caller's scratch first, as for
+  // esp_attn_forward; a pass that reads no cached key does not care about the pool's type.
+  bool cached = false, page_starts = a.tiles_host != nullptr && a.trees_host != nullptr;
+  for (int i = 0; page_starts && i < a.n_tiles; ++i) {
+    cached = cached || a.tiles_host[i].k1 > a.tiles_host[i].k0;
+    page_starts = a.tiles_host[i].k0 % esp::kDecodeKeyBlock == 0;
+  }
+  const bool fp8_pool = s.kv_dtype == ESP_E4M3 && cached;
+  const size_t widened_bytes = size_t(std::max(a.n_block_entries, 0)) * 2 * size_t(a.p.bt) * size_t(a.p.kv_ld) * 2;
+  const bool widen = fp8_pool && a.dequant_scratch != nullptr && a.n_block_entries > 0 && (reinterpret_cast<uintptr_t>(a.dequant_scratch) & 127) == 0 &&
+                     a.dequant_scratch_bytes >= widened_bytes + ((size_t(a.n_block_entries) * 4 + 127) / 128) * 128;
+  const bool umma = !decode && c->opt_attn_umma && page_starts && esp::diff_umma_supports(s.HD, c->G, c->tile_rows, s.bt) && (!fp8_pool || widen) &&
+                    a.p.kv_ld % 64 == 0 && (s.kv_dtype == ESP_E4M3 || a.p.kv_base % 64 == 0);
+
   cudaError_t e;
   if (decode) {
     if (int rc = pool_tensor_map(c, a)) return rc;
     c->last_kernel = "diff_decode";
     ProfScope prof(c, st, c->last_kernel);
     e = esp::launch_diff_decode(d, c->pool_map, st, &c->launches);
+  } else if (umma) {
+    esp_attn_args w = a;  // the pass as the kernel sees it: a 16-bit pool, or none
+    if (widen) {
+      int32_t* identity = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(a.dequant_scratch) + widened_bytes);
+      ProfScope prof(c, st, "kv_dequant");
+      e = esp::launch_kv_dequant(a.kv, a.kv_scales, a.blocks, a.n_block_entries, a.dequant_scratch, identity, a.p, s.HD, a.n_blocks, s.q_dtype, st, &c->launches);
+      if (e != cudaSuccess) return cuda_fail(e, "kv_dequant");
+      w.kv = a.dequant_scratch, w.blocks = identity, w.n_blocks = a.n_block_entries, w.p.kv_base = 0;
+      k.blocks = identity, k.n_blocks = a.n_block_entries, k.p.kv_base = 0;
+    } else if (!cached) {
+      w.kv = nullptr;
+    }
+    if (int rc = umma_tensor_maps(c, w)) return rc;
+    c->last_kernel = "diff_umma";
+    ProfScope prof(c, st, c->last_kernel);
+    e = esp::launch_diff_umma(d, c->upool_map, c->kb_map, c->vb_map, st, &c->launches);
   } else {
     c->last_kernel = "diff_general";
     ProfScope prof(c, st, c->last_kernel);

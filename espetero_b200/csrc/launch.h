@@ -223,6 +223,11 @@ cudaError_t launch_diff_general(const DiffArgs& a, cudaStream_t stream, uint64_t
 bool diff_decode_supports(int32_t HD, int32_t G, int32_t bt);
 cudaError_t diff_decode_setup();
 cudaError_t launch_diff_decode(const DiffArgs& a, const CUtensorMap& pool_map, cudaStream_t stream, uint64_t* launches);
+// tcgen05 kernels: 16-bit pools (or none read), tiles of 16 .. 128 rows; maps as flash_umma's.
+bool diff_umma_supports(int32_t HD, int32_t G, int32_t tile_rows, int32_t bt);
+cudaError_t diff_umma_setup();
+cudaError_t launch_diff_umma(const DiffArgs& a, const CUtensorMap& pool_map, const CUtensorMap& kb_map, const CUtensorMap& vb_map, cudaStream_t stream,
+                             uint64_t* launches);
 cudaError_t launch_diff_combine(const DiffCombineArgs& a, cudaStream_t stream, uint64_t* launches);
 cudaError_t launch_diff_lambda(const float* q1, const float* k1, const float* q2, const float* k2, int32_t H, int32_t dim, int32_t ld,
                                float lambda_init, float* lam, cudaStream_t stream);

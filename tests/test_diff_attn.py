@@ -108,6 +108,77 @@ def test_decode_long_and_hidden_from_itself():
     assert O[0].any() and not O[1].any() and O[2].any()
 
 
+TC = {128: "diff_umma"}
+# name, trees (P, M), H, Hkv, bt, pool, mask, tile_rows, split
+ROWS_CASES = [
+    ("prefill", [(0, 1), (0, 15), (0, 128), (0, 129), (0, 300)], 4, 2, 16, None, "causal", 128, 0),
+    ("one head", [(0, 257)], 1, 1, 16, None, "causal", 128, 0),
+    ("chunk", [(48, 130), (500, 77), (129, 1), (0, 64)], 8, 2, 32, None, "causal", 128, 0),
+    ("chunk split", [(1000, 130), (500, 77)], 8, 2, 16, None, "causal", 128, 128),
+    ("tree", [(300, 16), (0, 64), (17, 33)], 16, 2, 16, None, "tree", 16, 0),
+    ("tree split", [(1030, 16), (600, 12), (64, 3)], 16, 2, 16, None, "tree", 16, 96),
+    ("tree of 4 heads", [(260, 40)], 12, 3, 48, None, "tree", 32, 0),
+    ("tree of 2 heads", [(260, 64), (0, 5)], 4, 2, 16, None, "tree", 64, 64),
+    ("forest", [(100, 400), (0, 261)], 4, 2, 16, None, "forest", 128, 0),
+    ("e4m3 chunk", [(333, 140), (16, 9)], 8, 2, 16, wl.E4M3, "causal", 128, 0),
+    ("e4m3 tree split", [(700, 16), (90, 7)], 8, 1, 16, wl.E4M3, "tree", 16, 64),
+    ("e4m3 prefill", [(0, 140)], 8, 2, 16, wl.E4M3, "causal", 128, 0),
+]
+
+
+@gpu
+@pytest.mark.parametrize("HD", sorted(TC))
+@pytest.mark.parametrize("dt", [wl.F16, wl.BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("case", ROWS_CASES, ids=[c[0] for c in ROWS_CASES])
+def test_rows_on_tensor_cores(case, dt, HD):
+    name, trees, H, Hkv, bt, pool, mask, tile_rows, split = case
+    w = wl.make_pass(name, len(name) + HD, trees, H, Hkv, HD, bt, dt, pool, scale=(HD // 2) ** -0.5, mask=mask)
+    if pool == wl.E4M3 and w.kv.size:
+        _widened(w)
+    _check(w, TC[HD], tile_rows=tile_rows, plan_opts=dict(split=split, groups=4096 if split else 1))
+
+
+def _widened(w):
+    """The widening pass rounds code * scale to 16 bits: scales that make it exact (powers of two) keep that out of the bound."""
+    scales = np.exp2(np.round(np.log2(w.kv_scales))).astype(np.float32)
+    w.kv_scales = scales
+
+
+@gpu
+@pytest.mark.parametrize("HD", sorted(TC))
+def test_rows_over_e4m3_without_scratch(HD):
+    w = wl.make_pass("no scratch", 4, [(64, 9)], 8, 2, HD, 16, wl.BF16, wl.E4M3, scale=0.125)
+    _check(w, "diff_general", tile_rows=128, plan_opts=dict(split=0), scratch=False)
+
+
+@gpu
+@pytest.mark.parametrize("HD", sorted(TC))
+def test_rows_with_scores_that_grow(HD):
+    """Rows whose maximum rises by more than 2^8 from block to block: the accumulators are rescaled."""
+    w = wl.make_pass("growing", 4, [(0, 600)], 2, 1, HD, 16, wl.F16, scale=(HD // 2) ** -0.5)
+    K = wl.from_bits16(w.Kb, wl.F16) * (0.05 + np.arange(600)[:, None] / 60.0).astype(np.float32)
+    w.Kb = wl.to_bits16(K.astype(np.float32), wl.F16)
+    _check(w, TC[HD], tile_rows=128)
+
+
+@gpu
+@pytest.mark.parametrize("HD", sorted(TC))
+def test_mixed_rows_in_one_pass(HD):
+    """Single tokens beside a prompt and a chunk: one plan, one kernel."""
+    w = wl.make_pass("mixed", 4, [(333, 1), (0, 200), (1, 1), (64, 30), (0, 1)], 8, 4, HD, 16, wl.BF16, scale=(HD // 2) ** -0.5)
+    _check(w, TC[HD])
+
+
+@gpu
+@pytest.mark.parametrize("HD", sorted(TC))
+def test_rows_report_a_block_outside_the_pool(HD):
+    w = wl.make_pass("bad page", 3, [(300, 20)], 8, 2, HD, 16, wl.BF16, scale=0.125)
+    for bad in (-1, w.n_blocks, 2 ** 30):
+        w.blocks[2] = bad
+        with pytest.raises(capi.EspError, match="bad block id"):
+            _launch(w, *_weights(w, 1), tile_rows=128)
+
+
 @gpu
 @pytest.mark.parametrize("pool", [None, wl.E4M3], ids=["16-bit", "e4m3"])
 def test_decode_reports_a_block_outside_the_pool(pool):

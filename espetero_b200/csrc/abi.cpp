@@ -1252,8 +1252,8 @@ int esp_diff_forward(esp_attn_ctx* c, void* stream, const esp_attn_args* ap, con
   const bool decode = single && c->opt_attn_gqa && esp::diff_decode_supports(s.HD, c->G, s.bt) && a.kv != nullptr && a.n_blocks > 0 &&
                       (size_t(a.p.kv_ld) * elem_bytes(s.kv_dtype)) % 128 == 0 && (a.p.kv_base * elem_bytes(s.kv_dtype)) % 128 == 0;
 
-  // Multi-row tiles: the tcgen05 kernels, over 16-bit pages. An E4M3 pool is widened into the caller's scratch first, as for
-  // esp_attn_forward; a pass that reads no cached key does not care about the pool's type.
+  // Multi-row tiles: the tcgen05 kernels, over 16-bit pages. The codes of an E4M3 pool are widened into the caller's
+  // scratch first (the scales stay apart); a pass that reads no cached key does not care about the pool's type.
   bool cached = false, page_starts = a.tiles_host != nullptr && a.trees_host != nullptr;
   for (int i = 0; page_starts && i < a.n_tiles; ++i) {
     cached = cached || a.tiles_host[i].k1 > a.tiles_host[i].k0;
@@ -1273,21 +1273,19 @@ int esp_diff_forward(esp_attn_ctx* c, void* stream, const esp_attn_args* ap, con
     ProfScope prof(c, st, c->last_kernel);
     e = esp::launch_diff_decode(d, c->pool_map, st, &c->launches);
   } else if (umma) {
-    esp_attn_args w = a;  // the pass as the kernel sees it: a 16-bit pool, or none
+    esp_attn_args w = a;  // the pool as the kernel sees it: 16-bit pages, or none
     if (widen) {
-      int32_t* identity = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(a.dequant_scratch) + widened_bytes);
-      ProfScope prof(c, st, "kv_dequant");
-      e = esp::launch_kv_dequant(a.kv, a.kv_scales, a.blocks, a.n_block_entries, a.dequant_scratch, identity, a.p, s.HD, a.n_blocks, s.q_dtype, st, &c->launches);
-      if (e != cudaSuccess) return cuda_fail(e, "kv_dequant");
-      w.kv = a.dequant_scratch, w.blocks = identity, w.n_blocks = a.n_block_entries, w.p.kv_base = 0;
-      k.blocks = identity, k.n_blocks = a.n_block_entries, k.p.kv_base = 0;
+      ProfScope prof(c, st, "diff_widen");
+      e = esp::launch_diff_widen(k, a.dequant_scratch, a.n_block_entries, st, &c->launches);
+      if (e != cudaSuccess) return cuda_fail(e, "diff_widen");
+      w.kv = a.dequant_scratch, w.n_blocks = a.n_block_entries, w.p.kv_base = 0;
     } else if (!cached) {
       w.kv = nullptr;
     }
     if (int rc = umma_tensor_maps(c, w)) return rc;
     c->last_kernel = "diff_umma";
     ProfScope prof(c, st, c->last_kernel);
-    e = esp::launch_diff_umma(d, c->upool_map, c->kb_map, c->vb_map, st, &c->launches);
+    e = esp::launch_diff_umma(d, widen, c->upool_map, c->kb_map, c->vb_map, st, &c->launches);
   } else {
     c->last_kernel = "diff_general";
     ProfScope prof(c, st, c->last_kernel);

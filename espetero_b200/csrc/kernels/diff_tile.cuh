@@ -13,6 +13,7 @@ namespace difft {
 constexpr int BM = 128;          // (row, head) pairs of a tile: the lanes of tensor memory
 constexpr int BN = 128;          // keys per block
 constexpr int kPages = BN / 16;  // TMA pages per K or V tile
+constexpr int kScaleSlots = 8;   // blocks whose page scales are kept (E4M3 pools)
 
 __device__ __forceinline__ uint64_t low_bits64(int n) { return n <= 0 ? 0ull : (n >= 64 ? ~0ull : ((1ull << n) - 1ull)); }
 
@@ -40,6 +41,56 @@ __device__ __forceinline__ void tmem_wait_ld_of(uint32_t (&r)[32]) {
                : "memory");
 }
 
+// MMA issue by a whole converged warp, of which one lane (`one` = 1) issues. The warp's loop counters and descriptors then stay in
+// uniform registers; a loop that only one lane runs spends about 100 clocks per instruction group on moving them there, more than
+// the tensor pipe takes (3794 against 3411 clocks per 128 keys in diff_umma).
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "}\n"
+      : "=r"(one));
+  return one;
+}
+// Descriptors as their low words (the high word of this file's tiles never changes).
+__device__ __forceinline__ void mma_ss(uint32_t one, uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p, q;\n\t"
+      ".reg .b64 a, b;\n\t"
+      "mov.b64 a, {%1, %2};\n\t"
+      "mov.b64 b, {%3, %4};\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "setp.ne.b32 q, %7, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n\t"
+      "}\n" ::"r"(d), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate), "r"(one)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t one, uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p, q;\n\t"
+      ".reg .b64 b;\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "setp.ne.b32 q, %6, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t"
+      "}\n" ::"r"(d), "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate), "r"(one)
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t one, uint64_t* bar) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t"
+      "}\n" ::"r"(smem_u32(bar)), "r"(one)
+      : "memory");
+}
+
 // The key blocks of a tile: its cached range in blocks of 128, then the batch blocks some row of the tile can see - those below
 // the rows' ancestor ranges (desc.z) and those of their own segments (desc.x .. row) -, as bounds over the tile's rows.
 struct BlockList {
@@ -49,6 +100,8 @@ struct BlockList {
   int a_hi, b_lo;       // batch blocks [0, a_hi) and from b_lo on
   int anc_min, seg_max; // keys below anc_min are seen by every row; segments start at seg_max at the latest
   int r_first;          // the tile's first row, relative to its tree
+  int full_c, full_a, seg_0, seg_n;  // blocks every row sees whole: [0, full_c), nbc + [0, full_a), seg_0 + [0, seg_n)
+  __device__ __forceinline__ bool whole(int b) const { return b < full_c || uint32_t(b - nbc) < uint32_t(full_a) || uint32_t(b - seg_0) < uint32_t(seg_n); }
   __device__ __forceinline__ int n() const { return nbc + nbb; }
   __device__ __forceinline__ int j0(int b) const {
     if (b < nbc) return k0 + BN * b;
@@ -63,6 +116,7 @@ __device__ __forceinline__ BlockList block_list(const KernelArgs& a, const esp_a
   BlockList L;
   L.k0 = tile.k0, L.k1 = tile.k1, L.nbc = (tile.k1 - tile.k0 + BN - 1) / BN;
   L.nbb = 0, L.k_last = -1, L.a_hi = L.b_lo = 0, L.anc_min = 0, L.seg_max = 0, L.r_first = tile.r0 - tree.base;
+  L.full_c = (tile.k1 - tile.k0) / BN, L.full_a = L.seg_n = 0, L.seg_0 = 0;
   if (!tile.last) return L;
   if (a.anc_mask) {
     L.k_last = min(tree.M, 64) - 1;
@@ -86,34 +140,36 @@ __device__ __forceinline__ BlockList block_list(const KernelArgs& a, const esp_a
   L.a_hi = min((max(anc_max, 0) + BN - 1) / BN, n_all);
   L.b_lo = max(L.a_hi, max(seg_min, 0) / BN);
   L.nbb = L.a_hi + max(0, min(r_last / BN, n_all - 1) - L.b_lo + 1);
+  // whole blocks: those that end below every row's ancestors, and - batch blocks [lo, hi) of the rows' segments - those that start
+  // at or after every segment's start and end at or before the first row
+  L.full_a = min(L.a_hi, min(anc_min, tree.M) / BN);
+  const int lo = max(L.b_lo, (seg_max + BN - 1) / BN), hi = (L.r_first + 1) / BN;
+  L.seg_0 = L.nbc + L.a_hi + (lo - L.b_lo), L.seg_n = max(0, hi - lo);
   return L;
 }
 
-// What one row sees of block b: 128 bits. Returns false when every column is visible (the words are then not set).
-__device__ __forceinline__ bool row_visibility(const BlockList& L, int b, const int4& d, uint64_t am, bool use_anc, int rr, uint32_t (&vw)[4]) {
-  const bool cached = b < L.nbc;
-  const int j0 = L.j0(b), n_valid = L.n_valid(b);
-  bool need = n_valid < BN;
-  if (!cached) need = need || use_anc || !((j0 + BN - 1 < L.anc_min) || (j0 >= L.seg_max && j0 + BN - 1 <= L.r_first));
-  if (!need) return false;
-#pragma unroll
-  for (int hf = 0; hf < 2; ++hf) {
-    const int jb = j0 + 64 * hf;
-    uint64_t vm = low_bits64(n_valid - 64 * hf);
-    if (!cached) {
-      if (use_anc) vm &= hf == 0 ? am : 0ull;  // one block, j0 = 0
-      else vm &= low_bits64(d.z - jb) | (low_bits64(rr + 1 - jb) & ~low_bits64(d.x - jb));  // j < d.z || d.x <= j <= rr
-    }
-    vw[2 * hf] = uint32_t(vm), vw[2 * hf + 1] = uint32_t(vm >> 32);
+// Takes the scores that a row does not see out of 64 columns of block b from column c0 on (two registers of 32).
+__device__ __forceinline__ void hide_columns(const BlockList& L, int b, int c0, const int4& d, uint64_t am, bool use_anc, int rr, uint32_t (&s0)[32], uint32_t (&s1)[32]) {
+  const int jb = L.j0(b) + c0;
+  uint64_t vm = low_bits64(L.n_valid(b) - c0);
+  if (b >= L.nbc) {
+    if (use_anc) vm &= jb == 0 ? am : 0ull;  // an ancestor mask covers the tree's first 64 rows, which are all it may have
+    else vm &= low_bits64(d.z - jb) | (low_bits64(rr + 1 - jb) & ~low_bits64(d.x - jb));  // j < d.z || d.x <= j <= rr
   }
-  return true;
+  const uint32_t w0 = uint32_t(vm), w1 = uint32_t(vm >> 32);
+#pragma unroll
+  for (int c = 0; c < 32; ++c) {
+    if (!((w0 >> c) & 1u)) s0[c] = 0xFF800000u;  // -inf
+    if (!((w1 >> c) & 1u)) s1[c] = 0xFF800000u;
+  }
 }
 
 // A TMA producer warp's walk over the pages of its tile's blocks: lane w < 8 handles the w-th 16-key page of every block. `load(kind, y)`
-// is called by those lanes, block after block: kind -1 nothing to load (past the range), 0 row y of the pool, 1 row y of Kb / Vb.
-// `which`: 0 keys, 1 values. Table entries are fetched four blocks per load, two groups ahead of their use; an entry outside the
-// region is recorded and block 0 is read in its place.
-template <class Load>
+// is called by those lanes, block after block: kind -1 nothing to load (past the range), 0 row y of the pool (its page is `blk` of the
+// region), 1 row y of Kb / Vb. `which`: 0 keys, 1 values. F8: the pool map covers the widened pages, which lie in the order of the
+// block list. Table entries are fetched four blocks per load, two groups ahead of their use; an entry outside the region is
+// recorded and block 0 stands in for it.
+template <bool F8, class Load>
 __device__ __forceinline__ void walk_pages(const KernelArgs& a, const esp_attn_tree& tree, const BlockList& L, int which, int lane, Load&& load) {
   const int bt = a.p.bt;
   auto group = [&](int g) {
@@ -133,42 +189,27 @@ __device__ __forceinline__ void walk_pages(const KernelArgs& a, const esp_attn_t
       nxt = group((b >> 2) + 1);
     }
     const int blk = __shfl_sync(0xffffffffu, cur, ((b & 3) << 3) | (lane & 7));
-    if (lane < kPages) load(blk >= 0 ? 0 : -1, (blk * 2 + which) * bt + (L.k0 + BN * b + 16 * lane) % bt);
+    const int j = L.k0 + BN * b + 16 * lane;
+    const int page = F8 ? tree.table + j / bt : blk;
+    if (lane < kPages) load(b, blk >= 0 ? 0 : -1, (page * 2 + which) * bt + j % bt, blk);
   }
   for (int b = L.nbc; b < L.n(); ++b) {
     const int j = L.j0(b) + 16 * lane;
-    if (lane < kPages) load(j <= L.k_last ? 1 : -1, tree.base + j);
+    if (lane < kPages) load(b, j <= L.k_last ? 1 : -1, tree.base + j, 0);
   }
 }
 
-// One row's 128 scores s (raw products) -> 128 weights as 16-bit pairs, in the exp2 domain against m_ref, lazily rescaled: the reference
-// maximum only moves when a block exceeds it by 2^8. The caller moves O when `grow` says so.
-struct RowState {
-  float m_ref = -INFINITY, l = 0.0f;
-};
-
-__device__ __forceinline__ float chunk_max(uint32_t (&s)[32], bool mask, uint32_t w) {
-  float m0 = -INFINITY, m1 = -INFINITY;
-  if (mask) {
+__device__ __forceinline__ float chunk_max(const uint32_t (&s)[32]) {
+  float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-    for (int c = 0; c < 32; ++c) {
-      const float x = ((w >> c) & 1u) ? __uint_as_float(s[c]) : -INFINITY;
-      s[c] = __float_as_uint(x);
-      m0 = fmaxf(m0, x);
-    }
-  } else {
-#pragma unroll
-    for (int c = 0; c < 32; c += 4) {
-      m0 = fmax3(m0, __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
-      m1 = fmax3(m1, __uint_as_float(s[c + 2]), __uint_as_float(s[c + 3]));
-    }
-  }
-  return fmaxf(m0, m1);
+  for (int c = 0; c < 32; c += 2) m[(c >> 1) & 3] = fmax3(m[(c >> 1) & 3], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+  return fmax3(fmaxf(m[0], m[1]), m[2], m[3]);
 }
 
-// 32 scores -> 16 packed pairs of weights; `sum` (two partial sums) gains the unrounded weights.
-template <int QDT>
-__device__ __forceinline__ void chunk_weights(const uint32_t (&s)[32], uint32_t (&pk)[16], uint64_t sl2x2, uint64_t neg_m2, uint64_t (&sum)[2]) {
+// 32 scores -> 16 packed pairs of weights exp2(sl2 s - m); `sum` (two partial sums) gains the unrounded weights. F8: v0, v1 = the V scales
+// of the chunk's two pages, in units of the tile's reference, on the weights that are handed on.
+template <int QDT, bool F8>
+__device__ __forceinline__ void chunk_weights(const uint32_t (&s)[32], uint32_t* pk, uint64_t sl2x2, uint64_t neg_m2, uint64_t (&sum)[2], float v0, float v1) {
 #pragma unroll
   for (int c = 0; c < 16; ++c) {
     const uint64_t x2 = f32x2_fma(f32x2_pack(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1])), sl2x2, neg_m2);
@@ -176,8 +217,24 @@ __device__ __forceinline__ void chunk_weights(const uint32_t (&s)[32], uint32_t 
     f32x2_unpack(x2, x0, x1);
     const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
     sum[c & 1] = f32x2_add(sum[c & 1], f32x2_pack(p0, p1));
-    pk[c] = Elem16<QDT>::pack2(p0, p1);
+    const float v = c < 8 ? v0 : v1;
+    pk[c] = F8 ? Elem16<QDT>::pack2(p0 * v, p1 * v) : Elem16<QDT>::pack2(p0, p1);
   }
+}
+
+// 2^floor(log2 x), and its reciprocal, for a positive normal x.
+__device__ __forceinline__ float pow2_floor(float x) { return __uint_as_float(__float_as_uint(x) & 0x7F800000u); }
+__device__ __forceinline__ float pow2_inverse(float p) { return __uint_as_float(0x7F000000u - __float_as_uint(p)); }
+
+// The reference of a tile's V scales over an E4M3 pool. The weights of a page are multiplied by its scale before they are rounded to 16
+// bits, relative to a power of two that follows the largest scale seen so far (within a factor of 16): neither tiny nor huge scales
+// leave fp16's range. Returns the factor for what has been summed in the old unit.
+__device__ __forceinline__ float follow_scale(float& ref, float largest) {
+  if (ref > 0.0f && !(largest > 16.0f * ref)) return 1.0f;
+  const float now = pow2_floor(fminf(fmaxf(largest, 1.17549435e-38f), 1.0e38f));
+  const float f = ref > 0.0f ? ref * pow2_inverse(now) : 1.0f;
+  ref = now;
+  return f;
 }
 
 }  // namespace difft

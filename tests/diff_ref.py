@@ -28,11 +28,11 @@ def rotate64(x, pos, inv_freq, maps, adjacent):
 
 
 def keys_values(w, i, kvh):
-    """Cached and own K, V [P + M, HD] (float64) of tree i for one kv head."""
+    """Cached and own K, V [P + M, HD] (float64) of tree i for one kv head, and the largest scale of its V pages (1 for 16-bit pools)."""
     t = w.trees[i]
     P, M, base, HD = int(t["P"]), int(t["M"]), int(t["base"]), w.HD
     cols = slice(kvh * HD, (kvh + 1) * HD)
-    out = []
+    out, unit = [], 1.0
     pool = w.kv[w.kv_base:].reshape(-1)[:w.n_blocks * 2 * w.bt * w.kv_ld].reshape(w.n_blocks, 2, w.bt, w.kv_ld)
     for which, fresh in ((0, w.Kb), (1, w.Vb)):
         j = np.arange(P)
@@ -40,10 +40,12 @@ def keys_values(w, i, kvh):
         raw = pool[b, which, j % w.bt][:, cols]
         if w.kv_dtype == wl.E4M3:
             kept = wl.e4m3_decode(raw).astype(np.float64) * w.kv_scales[b, which, kvh].astype(np.float64)[:, None]
+            if which == 1 and P:
+                unit = max(float(w.kv_scales[b, 1, kvh].max()), 1.0 if M else 0.0)
         else:
             kept = wl.from_bits16(raw, w.kv_dtype).astype(np.float64)
         out.append(np.concatenate([kept, wl.from_bits16(fresh[base:base + M, cols], w.q_dtype).astype(np.float64)]))
-    return out
+    return out[0], out[1], unit
 
 
 def visible(w, i):
@@ -82,7 +84,7 @@ def diff64(w, lam, norm_w, eps, out_scale, p_unit, rows_of=None):
         vis = visible(w, i)
         n = vis.shape[1]
         for kvh in range(w.Hkv):
-            K, V = keys_values(w, i, kvh)
+            K, V, unit = keys_values(w, i, kvh)
             with np.errstate(invalid="ignore"):
                 Vz = np.where(np.isfinite(V), V, 0.0)  # a key nobody sees may hold anything
                 Kz = np.where(np.isfinite(K), K, 0.0)
@@ -101,7 +103,8 @@ def diff64(w, lam, norm_w, eps, out_scale, p_unit, rows_of=None):
                     D += sign * f * (p @ Vz)
                     A += np.abs(f) * (p @ np.abs(Vz))
                     if p_unit:
-                        raw = np.where(vis, 1.0, 0.0) @ np.abs(Vz)
+                        # over E4M3 pools the weight carries its page's scale, in units of the largest: a code is at most 448
+                        raw = np.where(vis, 1.0, 0.0) @ (np.abs(Vz) if w.kv_dtype != wl.E4M3 else np.full_like(Vz, 448.0 * unit))
                         sub += np.abs(f) * (2.0 ** -25 if p_unit < 2.0 ** -9 else 0.0) * np.divide(raw, tot, out=np.zeros_like(raw), where=tot > 0)
                     e1 = np.maximum(e1, 2 * es + 2.0 ** -21 + (n + 8) * 2.0 ** -24 + p_unit)
                 e = e1 * A + sub

@@ -133,15 +133,7 @@ ROWS_CASES = [
 def test_rows_on_tensor_cores(case, dt, HD):
     name, trees, H, Hkv, bt, pool, mask, tile_rows, split = case
     w = wl.make_pass(name, len(name) + HD, trees, H, Hkv, HD, bt, dt, pool, scale=(HD // 2) ** -0.5, mask=mask)
-    if pool == wl.E4M3 and w.kv.size:
-        _widened(w)
     _check(w, TC[HD], tile_rows=tile_rows, plan_opts=dict(split=split, groups=4096 if split else 1))
-
-
-def _widened(w):
-    """The widening pass rounds code * scale to 16 bits: scales that make it exact (powers of two) keep that out of the bound."""
-    scales = np.exp2(np.round(np.log2(w.kv_scales))).astype(np.float32)
-    w.kv_scales = scales
 
 
 @gpu
@@ -149,6 +141,23 @@ def _widened(w):
 def test_rows_over_e4m3_without_scratch(HD):
     w = wl.make_pass("no scratch", 4, [(64, 9)], 8, 2, HD, 16, wl.BF16, wl.E4M3, scale=0.125)
     _check(w, "diff_general", tile_rows=128, plan_opts=dict(split=0), scratch=False)
+
+
+@gpu
+@pytest.mark.parametrize("HD", [128, 256])
+@pytest.mark.parametrize("shape", ["decode", "rows", "rows split"])
+@pytest.mark.parametrize("order", ["rising", "falling", "wild"])
+def test_page_scales_of_every_size(shape, order, HD):
+    """V scales from 2^-24 to 2^6 within a sequence: the weights carry them, and neither end may leave fp16's range. Values
+    small enough that products with the scales stay in the output's range."""
+    trees = [(700, 1), (64, 1)] if shape == "decode" else [(700, 40), (64, 3)]
+    w = wl.make_pass("scales", 4, trees, 8, 2, HD, 16, wl.F16, wl.E4M3, scale=(HD // 2) ** -0.5)
+    n = 44
+    e = np.linspace(-24, 6, n)
+    e = {"rising": e, "falling": e[::-1], "wild": np.random.default_rng(3).permutation(e)}[order]
+    for i, b in enumerate(w.blocks[:n]):
+        w.kv_scales[b, 1] = 2.0 ** e[i]
+    _check(w, None if shape == "decode" else TC.get(HD), tile_rows=8 if shape == "decode" else 128, plan_opts=dict(split=256 if shape == "rows split" else 0))
 
 
 @gpu

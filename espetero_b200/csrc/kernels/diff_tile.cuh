@@ -13,7 +13,6 @@ namespace difft {
 constexpr int BM = 128;          // (row, head) pairs of a tile: the lanes of tensor memory
 constexpr int BN = 128;          // keys per block
 constexpr int kPages = BN / 16;  // TMA pages per K or V tile
-constexpr int kScaleSlots = 8;   // blocks whose page scales are kept (E4M3 pools)
 
 __device__ __forceinline__ uint64_t low_bits64(int n) { return n <= 0 ? 0ull : (n >= 64 ? ~0ull : ((1ull << n) - 1ull)); }
 
@@ -148,20 +147,20 @@ __device__ __forceinline__ BlockList block_list(const KernelArgs& a, const esp_a
   return L;
 }
 
-// Takes the scores that a row does not see out of 64 columns of block b from column c0 on (two registers of 32).
-__device__ __forceinline__ void hide_columns(const BlockList& L, int b, int c0, const int4& d, uint64_t am, bool use_anc, int rr, uint32_t (&s0)[32], uint32_t (&s1)[32]) {
-  const int jb = L.j0(b) + c0;
-  uint64_t vm = low_bits64(L.n_valid(b) - c0);
+// What a row sees of 32 columns of block b from column c on (a multiple of 32): one bit per column.
+__device__ __forceinline__ uint32_t visible32(const BlockList& L, int b, int c, const int4& d, uint64_t am, bool use_anc, int rr) {
+  const int jb = L.j0(b) + c;
+  uint64_t vm = low_bits64(L.n_valid(b) - c);
   if (b >= L.nbc) {
-    if (use_anc) vm &= jb == 0 ? am : 0ull;  // an ancestor mask covers the tree's first 64 rows, which are all it may have
+    if (use_anc) vm &= jb < 64 ? am >> jb : 0ull;  // an ancestor mask covers the tree's first 64 rows, which are all it may have
     else vm &= low_bits64(d.z - jb) | (low_bits64(rr + 1 - jb) & ~low_bits64(d.x - jb));  // j < d.z || d.x <= j <= rr
   }
-  const uint32_t w0 = uint32_t(vm), w1 = uint32_t(vm >> 32);
+  return uint32_t(vm);
+}
+__device__ __forceinline__ void hide(uint32_t (&s)[32], uint32_t visible) {
 #pragma unroll
-  for (int c = 0; c < 32; ++c) {
-    if (!((w0 >> c) & 1u)) s0[c] = 0xFF800000u;  // -inf
-    if (!((w1 >> c) & 1u)) s1[c] = 0xFF800000u;
-  }
+  for (int c = 0; c < 32; ++c)
+    if (!((visible >> c) & 1u)) s[c] = 0xFF800000u;  // -inf
 }
 
 // A TMA producer warp's walk over the pages of its tile's blocks: lane w < 8 handles the w-th 16-key page of every block. `load(kind, y)`

@@ -1,25 +1,27 @@
-// Differential attention on the 5th-generation tensor cores (sm_100a), 128-dim heads: prefill, chunks behind a prefix, draft trees.
+// Differential attention on the 5th-generation tensor cores (sm_100a), 128- and 256-dim heads: prefill, chunks behind a prefix, draft
+// trees.
 //
-// A CTA owns 128 (row, head) pairs - tile_rows rows x 128 / tile_rows heads of one kv head - and both softmax maps of each:
-//   S_c[128 x 64] = Q_c . K_c^T    c = 1, 2: 4 tcgen05.mma each over map c's 64 dims, which are one 64-dim chunk of the Q and K tiles
-//   P_c = exp2(scale (S_c - m_c))  one softmax warpgroup per map, thread i = row i
-//   O_c[128 x 128] += P_c . V      4 tcgen05.mma, A = P_c from tensor memory, B = V from shared memory: one V tile for both maps
-// P_c is written over S_c as 16-bit pairs (the MMA takes A and B in one 16-bit type; the row sums stay fp32 and unrounded).
+// A tile is 128 (row, head) pairs - tile_rows rows x 128 / tile_rows heads of one kv head. Two CTAs, a cluster, work on it, one per
+// softmax map c:
+//   S_c[128 x BU] = Q_c . K_c^T   tcgen05.mma over the map's HD / 2 dims: its own half of the Q and K tiles, so nothing is computed twice
+//   P_c = exp2(scale (S_c - m_c)) thread = row
+//   O_c[128 x HD] += P_c . V      A = P_c from tensor memory (16-bit pairs over S_c: the MMA takes A and B in one 16-bit type; the row
+//                                 sums stay fp32 and unrounded), B = V from shared memory
+// and the maps meet at the end: each CTA sends half of the columns of its O_c / l_c (map 2's times -lam) into the other's shared memory,
+// both add, exchange the rows' sums of squares and write HD / 2 columns of the normalised difference.
 //
-// Tensor memory: O_1, O_2 (128 fp32 columns each) and two buffers of 64 columns for each S_c: all 512. Tiles of 128 keys are worked on
-// in halves of 64: while a warpgroup is on one half of its map, the other's scores are being made or wait, so it never sits through
-// P . V and the next Q . K^T. With one buffer of 128 columns per map it did: 2 x 8192 causal rows (H16) took 1068 us instead of
-// 932. (An instruction of 64 columns takes about as long as one of 128, so Q . K^T costs twice its share; the pipe has room.)
-// (P . V has a barrier per buffer too: a warpgroup that hands over its last unit may still have two of them in flight.)
-// O is rescaled only when a row's maximum grows by more than 2^8; its owner then waits for the P . V in flight.
-// After the last unit the maps meet: each warpgroup hands half of its normalised O to the other through shared memory, and both
-// finish 64 columns of D = O_1 / l_1 - lam O_2 / l_2 and its norm.
+// Tensor memory holds O_c and two buffers of S_c: with 256-dim heads 256 + 2 x 128 columns, one CTA per SM; with 128-dim heads 128 +
+// 2 x 64 (tiles of 128 keys in two units), two CTAs per SM. Two softmax warpgroups take the units in turn, so that one's loads, maxima
+// and hand-overs run under the other's exponentials. They share O, hence the rows' reference maxima: a warp reads them from its
+// partner (the warp of the other group with the same rows) after its own maximum, and passes them on before its exponentials.
+// The reference only moves when a maximum exceeds it by 2^8; the warp that moves it rescales its rows of O, after the P . V of the unit
+// before.
 //
-// Bound: per 128 keys the exponentials of two maps (2 * 128 * 128 at 16 a clock: 2048 clocks of the special-function unit), 1800
-// clocks of MMA, 1800 clocks of the shared-memory port (224 KB of operands and tiles).
-// One CTA per SM. Warps 0-3 softmax of map 1, 4-7 of map 2, 8 MMA issue (owns tensor memory), 9 / 10 K / V producers (TMA, one load
-// per 16-key page and 64-dim chunk). Hand-offs by mbarrier; every wait is bounded: after a timeout the CTA records a code, stops
-// waiting, finishes its loop, frees its tensor memory and returns.
+// Bound per 128 keys of a tile: 256-dim heads 1536 clocks of MMA per map (8 instructions of N = 128 and 8 of N = 256, 64 and 128
+// clocks each) on an SM, 1024 of exponentials; 128-dim heads 1024 of exponentials per map, two maps per SM, against 1600 of MMA.
+// Warps 0-7 softmax, 8 MMA issue (owns tensor memory), 9 / 10 K / V producers (TMA, one load per 16-key page and 64-dim chunk), 11 idle (it
+// completes the warpgroup that hands registers over). Hand-offs by mbarrier; every wait is bounded: after a timeout the CTA records a
+// code, stops waiting, finishes its loop, frees its tensor memory and returns.
 // E4M3 pools (F8): the pages are 16-bit codes (diff_widen.cu); the K producer leaves each block's page scales in shared memory, the
 // K scale goes on the score and the V scale on the weight.
 #include "diff_tile.cuh"
@@ -29,49 +31,78 @@ namespace {
 
 using namespace difft;
 
-constexpr int HD = 128;
-constexpr int CHUNK = 128 * 128;                 // bytes of a 64-dim chunk of a tile: [128 rows][128 B]
-constexpr int TILE = 2 * CHUNK;                  // Q, K or V tile
-constexpr int KS = 3, VS = 3;                    // ring depths: 192 KB in flight for prefixes streamed from HBM
-constexpr int TILES_BYTES = (1 + KS + VS) * TILE;
-constexpr int BU = 64;                           // keys per half block
-constexpr uint32_t COL_S = 0, COL_O = 256;       // S_c, buffer i at COL_S + 128 c + 64 i (P_c over its first 32 columns), O_c at COL_O + 128 c
-constexpr float kGrow = 8.0f;                    // log2 units a row's maximum may grow before O is rescaled
-constexpr int kSoftmax = 256, kMmaWarp = 8, kWarpK = 9, kWarpV = 10, kThreads = 352;
+constexpr float kGrow = 8.0f;  // log2 units a row's maximum may grow before O is rescaled
+constexpr int kSoftmax = 256, kMmaWarp = 8, kWarpK = 9, kWarpV = 10, kThreads = 384;
+constexpr int KS = 2, VS = 2;  // ring depths, in tiles of 128 keys
 
+template <int HD_>
+struct Geo {
+  static constexpr int HD = HD_, MAP = HD / 2;
+  static constexpr int CHUNK = 128 * 128;          // bytes of a 64-dim chunk of a tile: [128 rows][128 B]
+  static constexpr int QC = MAP / 64, VC = HD / 64;  // chunks of a Q or K tile (one map), of a V tile
+  static constexpr int K_TILE = QC * CHUNK, V_TILE = VC * CHUNK;
+  static constexpr int TILES = (1 + KS) * K_TILE + VS * V_TILE;
+  static constexpr int SMEM = TILES + 1024;
+  static constexpr int BU = HD == 256 ? 128 : 64;  // keys per unit
+  static constexpr int UPB = BN / BU;              // units per block
+  static constexpr uint32_t COL_O = 0, COL_S = HD; // S buffer i at COL_S + BU i (P over its first BU / 2 columns)
+  static constexpr uint32_t COLS = HD + 2 * BU;    // 512 or 256
+  static constexpr int CTAS = HD == 256 ? 1 : 2;   // per SM
+  // 256-dim heads: a softmax thread holds its 128 scores; the last warpgroup hands registers over (128 x 96 + 256 x 200 <= 384 x 168).
+  // 128-dim heads: two CTAs leave 80 registers a thread, so a unit's 64 scores are read twice, 32 at a time: for the maximum, then for
+  // the weights. (Held at once, with 96 registers for the softmax threads, they spilled: 2 x 8192 rows, H16, took 2255 us instead of 944.)
+  static constexpr bool HOLD = HD == 256;
+};
+
+constexpr int kRegsAux = 96, kRegsSoftmax = 200;  // 256-dim heads
+constexpr int kSlots = 4;  // blocks whose page scales are kept
 struct Shared {
-  uint64_t k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], s_full[2][2], p_full[2][2], o_done[2][2], sc_full[kScaleSlots];
+  uint64_t k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], s_full[2], p_full[2], o_done[2], sc_full[kSlots], m_ready[2][4];
   uint32_t tmem;
   volatile int dead;
-  float k_scale[kScaleSlots][kPages], v_scale[kScaleSlots][kPages];
+  float k_scale[kSlots][kPages], v_scale[kSlots][kPages];
+  float m_ref[BM], v_ref[4];
 };
-constexpr int SMEM = TILES_BYTES + 1024;
 static_assert(sizeof(Shared) <= 1024, "bookkeeping behind the tiles");
-static_assert(kScaleSlots > KS + 2, "page scales must outlive their readers");
+// K tile b is released once its Q . K^T is through, which is issued behind P . V of two units before its last: the softmax is at most one
+// block behind then, and the producer KS blocks ahead.
+static_assert(kSlots >= KS + 2, "page scales must outlive their readers");
 
-template <int QDT, bool F8>
-__global__ void __launch_bounds__(kThreads, 1)
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t peer_addr(const void* p, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void peer_store(uint32_t addr, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory"); }
+
+template <int HD, int QDT, bool F8>
+__global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
     diff_umma_kernel(const __grid_constant__ CUtensorMap pool_map, const __grid_constant__ CUtensorMap kb_map, const __grid_constant__ CUtensorMap vb_map,
                      const DiffArgs args) {
+  using C = Geo<HD>;
   using QE = Elem16<QDT>;
   extern __shared__ __align__(1024) uint8_t smem[];
-  Shared& sh = *reinterpret_cast<Shared*>(smem + TILES_BYTES);
+  Shared& sh = *reinterpret_cast<Shared*>(smem + C::TILES);
   const KernelArgs& a = args.k;
   const esp_attn_params& p = a.p;
   uint8_t* q_sm = smem;
-  uint8_t* k_sm = smem + TILE;
-  uint8_t* v_sm = smem + (1 + KS) * TILE;
-  if ((smem_u32(smem) & 1023u) != 0) {  // never expected; the swizzle would be wrong
-    if (threadIdx.x == 0) atomicExch(a.status, kStatusBadBlock);
-    return;
-  }
+  uint8_t* k_sm = smem + C::K_TILE;
+  uint8_t* v_sm = smem + (1 + KS) * C::K_TILE;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int map = int(blockIdx.z);  // = rank in the cluster
   if (tid == 0) {
+    if ((smem_u32(smem) & 1023u) != 0) atomicExch(a.status, kStatusBadBlock);  // never expected; the swizzle would be wrong
     for (int s = 0; s < KS; ++s) mbar_init(&sh.k_full[s], kPages), mbar_init(&sh.k_empty[s], 1);
     for (int s = 0; s < VS; ++s) mbar_init(&sh.v_full[s], kPages), mbar_init(&sh.v_empty[s], 1);
-    for (int c = 0; c < 2; ++c)
-      for (int i = 0; i < 2; ++i) mbar_init(&sh.s_full[c][i], 1), mbar_init(&sh.p_full[c][i], BM), mbar_init(&sh.o_done[c][i], 1);
-    for (int s = 0; s < kScaleSlots; ++s) mbar_init(&sh.sc_full[s], 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh.s_full[i], 1), mbar_init(&sh.p_full[i], BM), mbar_init(&sh.o_done[i], 1);
+      for (int w = 0; w < 4; ++w) mbar_init(&sh.m_ready[i][w], 1);
+    }
+    for (int s = 0; s < kSlots; ++s) mbar_init(&sh.sc_full[s], 1);
     mbar_fence_init();
     sh.dead = 0;
   }
@@ -84,7 +115,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int kvh = (int(blockIdx.y) * HPC) / G;
   const int end = tree.base + tree.M, rows_live = min(TR, end - tile.r0);
   const BlockList L = block_list(a, tile, tree, rows_live, lane);
-  const int nb = L.n();
+  const int nb = L.n(), N = nb * C::UPB;
+  const bool whole_rows = tile.part < 0;
 
   auto wait_bar = [&](uint64_t* bar, uint32_t parity, int code) {
     if (mbar_try_wait(bar, parity) || sh.dead) return;
@@ -94,109 +126,124 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   };
 
-  if (warp == kWarpK || warp == kWarpV) {
-    const bool is_v = warp == kWarpV;
-    if (lane == 0) tma_prefetch_desc(is_v ? &vb_map : &kb_map), tma_prefetch_desc(&pool_map);
-    const int depth = is_v ? VS : KS;
-    uint64_t* full = is_v ? sh.v_full : sh.k_full;
-    uint64_t* empty = is_v ? sh.v_empty : sh.k_empty;
-    uint8_t* ring = is_v ? v_sm : k_sm;
-    int stage = 0;
-    uint32_t par = 1;  // the first use of a slot finds it empty
-    walk_pages<F8>(a, tree, L, is_v ? 1 : 0, lane, [&](int b, int kind, int y, int blk) {
-      uint8_t* dst = ring + stage * TILE + lane * 2048;
-      float ks = 1.0f, vs = kind < 0 ? 0.0f : 1.0f;
-      if (F8 && !is_v && kind == 0) {
-        ks = a.kv_scales[size_t(blk) * 2 * p.Hkv + kvh];
-        vs = a.kv_scales[(size_t(blk) * 2 + 1) * p.Hkv + kvh];
-      }
-      wait_bar(&empty[stage], par, kStatusMmaTimeout);
-      if (kind < 0) {
-        mbar_arrive(&full[stage]);
-      } else {
-        const CUtensorMap* m = kind ? (is_v ? &vb_map : &kb_map) : &pool_map;
-        mbar_arrive_expect_tx(&full[stage], 4096);
-        tma_load_3d(dst, m, &full[stage], 0, y, kvh * 2);
-        tma_load_3d(dst + CHUNK, m, &full[stage], 0, y, kvh * 2 + 1);
-      }
-      if (F8 && !is_v) {
-        // The slot's last readers are done: a K slot is released once Q . K^T of its block is, two units ahead of the softmax at
-        // most, so the producer is at most KS + 2 blocks ahead of it, and there are more slots than that.
-        const int slot = b % kScaleSlots;
-        sh.k_scale[slot][lane] = ks, sh.v_scale[slot][lane] = vs;
-        __syncwarp(0xFFu);
-        if (lane == 0) mbar_arrive(&sh.sc_full[slot]);
-      }
-      if (++stage == depth) stage = 0, par ^= 1;
-    });
-  } else if (warp == kMmaWarp) {
-    tmem_alloc(&sh.tmem, 512);
-    tmem_relinquish();
-    tc_fence_before_sync();
-    named_barrier(1, kSoftmax + 32);  // Q is staged, tensor memory allocated
-    tc_fence_after_sync();
-    const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
-    if (nb > 0) {
-      const uint32_t one = elect_one();
-      constexpr uint32_t idesc_qk = umma_idesc<QDT>(BM, BU, 0, 0), idesc_pv = umma_idesc<QDT>(BM, HD, 0, 1);
-      const uint64_t q_desc = umma_smem_desc(smem_u32(q_sm), 16, 1024), k_desc = umma_smem_desc(smem_u32(k_sm), 16, 1024);
-      const uint64_t v_desc = umma_smem_desc(smem_u32(v_sm), CHUNK, 1024);
-      const uint32_t q_lo = uint32_t(q_desc), k_lo0 = uint32_t(k_desc), v_lo0 = uint32_t(v_desc);
-      const uint32_t hi_qk = uint32_t(q_desc >> 32), hi_v = uint32_t(v_desc >> 32);
-      int kst = 0, vst = 0;
-      uint32_t kpar = 0, vpar = 0;
-      // S_c of the half h of the block in K slot kst
-      auto issue_qk = [&](int c, int h) {
-        if (c == 0 && h == 0) {
-          wait_bar(&sh.k_full[kst], kpar, kStatusTmaTimeout);
-          tc_fence_after_sync();
+  if (warp >= kMmaWarp) {
+    if constexpr (C::HOLD) regs_dec<kRegsAux>();
+    if (warp == kWarpK || warp == kWarpV) {
+      const bool is_v = warp == kWarpV;
+      if (lane == 0) tma_prefetch_desc(is_v ? &vb_map : &kb_map), tma_prefetch_desc(&pool_map);
+      const int depth = is_v ? VS : KS;
+      uint64_t* full = is_v ? sh.v_full : sh.k_full;
+      uint64_t* empty = is_v ? sh.v_empty : sh.k_empty;
+      int stage = 0;
+      uint32_t par = 1;  // the first use of a slot finds it empty
+      walk_pages<F8>(a, tree, L, is_v ? 1 : 0, lane, [&](int b, int kind, int y, int blk) {
+        float ks = 1.0f, vs = kind < 0 ? 0.0f : 1.0f;
+        if (F8 && !is_v && kind == 0) {
+          ks = a.kv_scales[size_t(blk) * 2 * p.Hkv + kvh];
+          vs = a.kv_scales[(size_t(blk) * 2 + 1) * p.Hkv + kvh];
         }
-        const uint32_t k_lo = k_lo0 + uint32_t(kst) * (TILE >> 4);
+        wait_bar(&empty[stage], par, kStatusMmaTimeout);
+        if (kind < 0) {
+          mbar_arrive(&full[stage]);
+        } else {
+          const CUtensorMap* m = kind ? (is_v ? &vb_map : &kb_map) : &pool_map;
+          if (is_v) {
+            uint8_t* dst = v_sm + stage * C::V_TILE + lane * 2048;
+            mbar_arrive_expect_tx(&full[stage], 2048 * C::VC);
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks)
-          mma_ss(one, tmem + COL_S + c * 128 + h * BU, q_lo + ((c * CHUNK + ks * 32) >> 4), hi_qk, k_lo + ((c * CHUNK + h * (BU * 128) + ks * 32) >> 4), hi_qk, idesc_qk, ks > 0);
-        mma_commit(one, &sh.s_full[c][h]);
-        if (c == 1 && h == 1) {
-          mma_commit(one, &sh.k_empty[kst]);
-          if (++kst == KS) kst = 0, kpar ^= 1;
-        }
-      };
+            for (int i = 0; i < C::VC; ++i) tma_load_3d(dst + i * C::CHUNK, m, &full[stage], 0, y, kvh * C::VC + i);
+          } else {
+            uint8_t* dst = k_sm + stage * C::K_TILE + lane * 2048;
+            mbar_arrive_expect_tx(&full[stage], 2048 * C::QC);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) issue_qk(0, h), issue_qk(1, h);
-#pragma unroll 1
-      for (int b = 0; b < nb; ++b) {
-        const uint32_t v_lo = v_lo0 + uint32_t(vst) * (TILE >> 4), more = b > 0;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            wait_bar(&sh.p_full[c][h], b & 1, kStatusMmaTimeout);
-            if (c == 0 && h == 0) wait_bar(&sh.v_full[vst], vpar, kStatusTmaTimeout);
-            tc_fence_after_sync();
-#pragma unroll
-            for (int ks = 0; ks < BU / 16; ++ks)
-              mma_ts(one, tmem + COL_O + c * HD, tmem + COL_S + c * 128 + h * BU + ks * 8, v_lo + ((h * (BU * 128) + ks * 16 * 128) >> 4), hi_v, idesc_pv, (h > 0 || ks > 0) ? 1u : more);
-            mma_commit(one, &sh.o_done[c][h]);
-            if (c == 1 && h == 1) mma_commit(one, &sh.v_empty[vst]);
-            if (b + 1 < nb) issue_qk(c, h);  // the next block's half, over P_c: behind the P_c . V that reads it
+            for (int i = 0; i < C::QC; ++i) tma_load_3d(dst + i * C::CHUNK, m, &full[stage], 0, y, kvh * C::VC + map * C::QC + i);
           }
         }
-        if (++vst == VS) vst = 0, vpar ^= 1;
+        if (F8 && !is_v) {
+          const int slot = b % kSlots;
+          sh.k_scale[slot][lane] = ks, sh.v_scale[slot][lane] = vs;
+          __syncwarp(0xFFu);
+          if (lane == 0) mbar_arrive(&sh.sc_full[slot]);
+        }
+        if (++stage == depth) stage = 0, par ^= 1;
+      });
+      __syncwarp();
+    } else if (warp == kMmaWarp) {
+      tmem_alloc(&sh.tmem, C::COLS);
+      tmem_relinquish();
+      tc_fence_before_sync();
+      named_barrier(1, kSoftmax + 32);  // Q is staged, tensor memory allocated
+      tc_fence_after_sync();
+      const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
+      if (N > 0) {
+        const uint32_t one = elect_one();
+        constexpr uint32_t idesc_qk = umma_idesc<QDT>(BM, C::BU, 0, 0), idesc_pv = umma_idesc<QDT>(BM, HD, 0, 1);
+        const uint64_t q_desc = umma_smem_desc(smem_u32(q_sm), 16, 1024), k_desc = umma_smem_desc(smem_u32(k_sm), 16, 1024);
+        const uint64_t v_desc = umma_smem_desc(smem_u32(v_sm), C::CHUNK, 1024);
+        const uint32_t q_lo = uint32_t(q_desc), k_lo0 = uint32_t(k_desc), v_lo0 = uint32_t(v_desc);
+        const uint32_t hi_qk = uint32_t(q_desc >> 32), hi_v = uint32_t(v_desc >> 32);
+        int kst = 0, vst = 0;
+        uint32_t kpar = 0, vpar = 0;
+        // S of unit n = (block of K slot kst, half h), into buffer i = n & 1
+        auto issue_qk = [&](int h, int i) {
+          if (h == 0) {
+            wait_bar(&sh.k_full[kst], kpar, kStatusTmaTimeout);
+            tc_fence_after_sync();
+          }
+          const uint32_t k_lo = k_lo0 + uint32_t(kst) * (C::K_TILE >> 4) + uint32_t((h * C::BU * 128) >> 4);
+#pragma unroll
+          for (int ks = 0; ks < C::MAP / 16; ++ks)
+            mma_ss(one, tmem + C::COL_S + i * C::BU, q_lo + (((ks >> 2) * C::CHUNK + (ks & 3) * 32) >> 4), hi_qk, k_lo + (((ks >> 2) * C::CHUNK + (ks & 3) * 32) >> 4), hi_qk,
+                   idesc_qk, ks > 0);
+          mma_commit(one, &sh.s_full[i]);
+          if (h == C::UPB - 1) {
+            mma_commit(one, &sh.k_empty[kst]);
+            if (++kst == KS) kst = 0, kpar ^= 1;
+          }
+        };
+        issue_qk(0, 0);
+        if (N > 1) issue_qk(1 % C::UPB, 1);
+#pragma unroll 1
+        for (int n0 = 0; n0 < N; n0 += 2) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int n = n0 + i, h = i % C::UPB;
+            if (n >= N) break;
+            wait_bar(&sh.p_full[i], uint32_t(n >> 1) & 1u, kStatusMmaTimeout);
+            if (h == 0) wait_bar(&sh.v_full[vst], vpar, kStatusTmaTimeout);
+            tc_fence_after_sync();
+            const uint32_t v_lo = v_lo0 + uint32_t(vst) * (C::V_TILE >> 4) + uint32_t((h * C::BU * 128) >> 4);
+#pragma unroll
+            for (int ks = 0; ks < C::BU / 16; ++ks)
+              mma_ts(one, tmem + C::COL_O, tmem + C::COL_S + i * C::BU + ks * 8, v_lo + ((ks * 16 * 128) >> 4), hi_v, idesc_pv, ks > 0 ? 1u : uint32_t(n > 0));
+            mma_commit(one, &sh.o_done[i]);
+            if (h == C::UPB - 1) {
+              mma_commit(one, &sh.v_empty[vst]);
+              if (++vst == VS) vst = 0, vpar ^= 1;
+            }
+            if (n + 2 < N) issue_qk(h, i);  // over P of unit n: behind the P . V that reads it
+          }
+        }
       }
     }
-  } else if (warp < kMmaWarp) {
-    const int map = tid >> 7, srow = tid & (BM - 1), fm = srow / HPC, head = int(blockIdx.y) * HPC + srow % HPC;
+    if (whole_rows) cluster_sync(), cluster_sync(), cluster_sync();  // the softmax warps' epilogue
+  } else {
+    if constexpr (C::HOLD) regs_inc<kRegsSoftmax>();
+    const int wg = tid >> 7, srow = tid & (BM - 1), fm = srow / HPC, head = int(blockIdx.y) * HPC + srow % HPC, wq = warp & 3;
     const bool row_ok = fm < rows_live;
     const int row = row_ok ? tile.r0 + fm : end - 1, rr = row - tree.base;
     int4 dsc = make_int4(0, 0, 0, 0);
     uint64_t am = 0;
     const bool use_anc = a.anc_mask != nullptr;
     {
-      // this thread's half of its Q row - its map's 64 dims - into the map's chunk (K-major, 128-byte swizzle)
-      const uint4* src = reinterpret_cast<const uint4*>(static_cast<const typename QE::T*>(a.Q) + size_t(row) * p.q_ld + size_t(head) * HD + map * 64);
-      uint8_t* qd = q_sm + map * CHUNK + srow * 128;
+      // the map's dims of this Q row, half of them per warpgroup (K-major, 128-byte swizzle)
+      constexpr int LINES = C::MAP / 16;  // 16-byte pieces per thread
+      const uint4* src = reinterpret_cast<const uint4*>(static_cast<const typename QE::T*>(a.Q) + size_t(row) * p.q_ld + size_t(head) * HD + map * C::MAP);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(qd + ((i ^ (srow & 7)) << 4)) = src[i];
+      for (int k = 0; k < LINES; ++k) {
+        const int i = wg * LINES + k;
+        *reinterpret_cast<uint4*>(q_sm + (i >> 3) * C::CHUNK + srow * 128 + (((i & 7) ^ (srow & 7)) << 4)) = src[i];
+      }
       fence_proxy_async_smem();
       if (tile.last) {
         if (use_anc) am = a.anc_mask[row];
@@ -206,105 +253,145 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_before_sync();
     named_barrier(1, kSoftmax + 32);
     tc_fence_after_sync();
-    const uint32_t t_lane = sh.tmem + (uint32_t((warp & 3) * 32) << 16);  // this warp's quarter of the lanes
-    const uint32_t t_s = t_lane + COL_S + map * 128, t_o = t_lane + COL_O + map * HD;
+    const uint32_t t_lane = sh.tmem + (uint32_t(wq * 32) << 16);  // this warp's quarter of the lanes
+    const uint32_t t_o = t_lane + C::COL_O, buf = t_lane + C::COL_S + wg * C::BU;
     const float sl2 = a.scale * kLog2e;
-    float m_ref = -INFINITY, l_run = 0.0f, v_ref = F8 ? 0.0f : 1.0f;
-    int vst = 0;
-    uint32_t vpar = 0;
     const uint64_t sl2x2 = f32x2_pack(sl2, sl2);
-    for (int b = 0; b < nb; ++b) {
+    float m_seen = -INFINITY, l_run = 0.0f;  // this group's sum, against the reference it last saw
+    constexpr int NS = C::BU / 32;
+    for (int n = wg; n < N; n += 2) {
+      const int b = n / C::UPB, c0 = (n % C::UPB) * C::BU;
+      const uint32_t par = uint32_t(n >> 1) & 1u;
       const bool whole = L.whole(b);
-      const uint32_t par = b & 1;
-      if constexpr (F8) wait_bar(&sh.sc_full[b % kScaleSlots], uint32_t(b / kScaleSlots) & 1u, kStatusTmaTimeout);
+      if constexpr (F8) wait_bar(&sh.sc_full[b % kSlots], uint32_t(b / kSlots) & 1u, kStatusTmaTimeout);
+      wait_bar(&sh.s_full[wg], par, kStatusMmaTimeout);
+      tc_fence_after_sync();
+      float ks[2 * NS], vs[2 * NS], largest = 0.0f;
+      if constexpr (F8) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t buf = t_s + h * BU;
-        wait_bar(&sh.s_full[map][h], par, kStatusMmaTimeout);
-        tc_fence_after_sync();
-        uint32_t s0[32], s1[32];
-        tmem_ld32(buf, s0);
-        tmem_ld32(buf + 32, s1);
-        tmem_wait_ld_of(s0);
-        tmem_wait_ld_of(s1);
-        float vfac = 1.0f, vs[4] = {1.0f, 1.0f, 1.0f, 1.0f};
-        if constexpr (F8) {
-          float ks[4], largest = 0.0f;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            ks[i] = sh.k_scale[b % kScaleSlots][4 * h + i], vs[i] = sh.v_scale[b % kScaleSlots][4 * h + i];
-            largest = fmaxf(largest, vs[i]);
-          }
-          vfac = follow_scale(v_ref, largest);
-          const float inv = pow2_inverse(v_ref);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) vs[i] *= inv;
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            s0[i] = __float_as_uint(__uint_as_float(s0[i]) * ks[i >> 4]);
-            s1[i] = __float_as_uint(__uint_as_float(s1[i]) * ks[2 + (i >> 4)]);
-          }
+        for (int i = 0; i < 2 * NS; ++i) {
+          ks[i] = sh.k_scale[b % kSlots][c0 / 16 + i], vs[i] = sh.v_scale[b % kSlots][c0 / 16 + i];
+          largest = fmaxf(largest, vs[i]);
         }
-        if (!whole) {
-          hide_columns(L, b, h * BU, dsc, am, use_anc, rr, s0, s1);
-          const int first = max(L.n_valid(b), h * BU), n = (h + 1) * BU - first;
-          if (map == 0 && n > 0) {
-            // V rows past the range are stale or foreign: 0 * NaN must not happen. Map 1's warpgroup clears the half's before it hands
-            // over P_1; P_2 . V is issued after P_1 . V.
-            wait_bar(&sh.v_full[vst], vpar, kStatusTmaTimeout);
-            for (int i = srow; i < n * 16; i += BM) {
-              const int r = first + i / 16, c = i % 16;
-              *reinterpret_cast<uint4*>(v_sm + vst * TILE + (c >> 3) * CHUNK + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
-            }
-            fence_proxy_async_smem();
-          }
-        }
-        const float mx = sl2 * fmaxf(chunk_max(s0), chunk_max(s1));  // scale > 0
-        float factor = vfac;
-        const bool grow = mx > m_ref + kGrow;  // also the first finite maximum
-        if (grow) {
-          const float f = fast_exp2(m_ref - mx);
-          factor *= f, l_run *= f;
-          m_ref = mx;
-        }
-        if ((b > 0 || h > 0) && __any_sync(0xffffffffu, grow || vfac != 1.0f)) {
-          wait_bar(&sh.o_done[map][h ^ 1], h ? par : par ^ 1, kStatusMmaTimeout);  // every half before this one is in O_c
-          tc_fence_after_sync();
-#pragma unroll 1
-          for (int c = 0; c < HD / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld32(t_o + 32 * c, o);
-            tmem_wait_ld_of(o);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
-            tmem_st32(t_o + 32 * c, o);
-          }
-        }
-        const float neg_m = m_ref == -INFINITY ? 0.0f : -m_ref;
-        const uint64_t neg_m2 = f32x2_pack(neg_m, neg_m);
-        uint64_t sum[2] = {f32x2_pack(0.0f, 0.0f), f32x2_pack(0.0f, 0.0f)};
-        uint32_t pk[32];
-        chunk_weights<QDT, F8>(s0, pk, sl2x2, neg_m2, sum, vs[0], vs[1]);
-        chunk_weights<QDT, F8>(s1, pk + 16, sl2x2, neg_m2, sum, vs[2], vs[3]);
-        tmem_st32(buf, pk);
-        float a0, a1;
-        f32x2_unpack(f32x2_add(sum[0], sum[1]), a0, a1);
-        l_run += a0 + a1;
-        tmem_wait_st();
-        tc_fence_before_sync();
-        mbar_arrive(&sh.p_full[map][h]);
       }
-      if (++vst == VS) vst = 0, vpar ^= 1;
+      // 32 scores as they count: times their pages' K scales, hidden where the row does not see the key
+      auto shape = [&](uint32_t (&x)[32], int i) {
+        if constexpr (F8) {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) x[k] = __float_as_uint(__uint_as_float(x[k]) * ks[2 * i + (k >> 4)]);
+        }
+        if (!whole) hide(x, visible32(L, b, c0 + 32 * i, dsc, am, use_anc, rr));
+      };
+      constexpr int HELD = C::HOLD ? NS : 1;
+      uint32_t s[HELD][32];
+      float mx = -INFINITY;
+      if constexpr (C::HOLD) {
+#pragma unroll
+        for (int i = 0; i < NS; ++i) tmem_ld32(buf + 32 * i, s[i]);
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+          tmem_wait_ld_of(s[i]);
+          shape(s[i], i);
+          mx = fmaxf(mx, chunk_max(s[i]));
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+          tmem_ld32(buf + 32 * i, s[0]);
+          tmem_wait_ld_of(s[0]);
+          shape(s[0], i);
+          mx = fmaxf(mx, chunk_max(s[0]));
+        }
+      }
+      mx *= sl2;  // scale > 0
+      if (!whole) {
+        const int first = max(L.n_valid(b), c0), lost = c0 + C::BU - first;
+        if (lost > 0) {
+          // V rows past the range are stale or foreign: 0 * NaN must not happen. Cleared before P is handed over.
+          const int vst = b % VS;
+          wait_bar(&sh.v_full[vst], uint32_t(b / VS) & 1u, kStatusTmaTimeout);
+          for (int i = srow; i < lost * 8 * C::VC; i += BM) {
+            const int r = first + i / (8 * C::VC), c = i % (8 * C::VC);
+            *reinterpret_cast<uint4*>(v_sm + vst * C::V_TILE + (c >> 3) * C::CHUNK + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+        }
+      }
+      // the reference, from the partner warp that had the unit before
+      float m_old = -INFINITY, v_ref = 0.0f;
+      if (n > 0) {
+        wait_bar(&sh.m_ready[wg ^ 1][wq], uint32_t((n - 1) >> 1) & 1u, kStatusMmaTimeout);
+        m_old = *const_cast<volatile float*>(&sh.m_ref[srow]);
+        if constexpr (F8) v_ref = *const_cast<volatile float*>(&sh.v_ref[wq]);
+      }
+      const bool grow = mx > m_old + kGrow;  // also the first finite maximum
+      const float m_new = grow ? mx : m_old;
+      float vfac = 1.0f;
+      if constexpr (F8) {
+        vfac = follow_scale(v_ref, largest);
+        if (lane == 0) *const_cast<volatile float*>(&sh.v_ref[wq]) = v_ref;
+      }
+      *const_cast<volatile float*>(&sh.m_ref[srow]) = m_new;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.m_ready[wg][wq]);
+      if (m_new > m_seen) {
+        l_run *= fast_exp2(m_seen - m_new);
+        m_seen = m_new;
+      }
+      if (n > 0 && __any_sync(0xffffffffu, grow || vfac != 1.0f)) {
+        wait_bar(&sh.o_done[wg ^ 1], uint32_t((n - 1) >> 1) & 1u, kStatusMmaTimeout);  // every unit before this one is in O
+        tc_fence_after_sync();
+        const float factor = (grow ? fast_exp2(m_old - m_new) : 1.0f) * vfac;
+#pragma unroll 1
+        for (int c = 0; c < HD / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld32(t_o + 32 * c, o);
+          tmem_wait_ld_of(o);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
+          tmem_st32(t_o + 32 * c, o);
+        }
+      }
+      const float neg_m = m_new == -INFINITY ? 0.0f : -m_new;
+      const uint64_t neg_m2 = f32x2_pack(neg_m, neg_m);
+      uint64_t sum[2] = {f32x2_pack(0.0f, 0.0f), f32x2_pack(0.0f, 0.0f)};
+      const float vinv = F8 ? pow2_inverse(v_ref) : 1.0f;
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        if constexpr (!C::HOLD) {  // P of chunk i lies in columns the chunks to come do not use
+          tmem_ld32(buf + 32 * i, s[0]);
+          tmem_wait_ld_of(s[0]);
+          shape(s[0], i);
+        }
+        uint32_t pk[16];
+        chunk_weights<QDT, F8>(s[C::HOLD ? i : 0], pk, sl2x2, neg_m2, sum, F8 ? vs[2 * i] * vinv : 1.0f, F8 ? vs[2 * i + 1] * vinv : 1.0f);
+        tmem_st16(buf + 16 * i, pk);
+      }
+      float a0, a1;
+      f32x2_unpack(f32x2_add(sum[0], sum[1]), a0, a1);
+      l_run += a0 + a1;
+      tmem_wait_st();
+      tc_fence_before_sync();
+      mbar_arrive(&sh.p_full[wg]);
     }
 
     // ---- epilogue
     pdl_launch_dependents();
-    if (nb > 0) {
-      wait_bar(&sh.o_done[map][1], (nb - 1) & 1, kStatusMmaTimeout);
+    named_barrier(2, kSoftmax);  // both groups are through: the reference is final, and all but the last two P . V are known to be done
+    float m_fin = -INFINITY, v_ref = 1.0f;
+    if (N > 0) {
+      wait_bar(&sh.o_done[(N - 1) & 1], uint32_t((N - 1) >> 1) & 1u, kStatusMmaTimeout);
       tc_fence_after_sync();
+      m_fin = *const_cast<volatile float*>(&sh.m_ref[srow]);
+      if constexpr (F8) v_ref = *const_cast<volatile float*>(&sh.v_ref[wq]);
     }
+    // the groups' sums (the rings are idle: every load has been waited for and every MMA that reads them is done)
+    float* lsum = reinterpret_cast<float*>(k_sm);
+    lsum[tid] = m_seen == -INFINITY ? 0.0f : l_run * fast_exp2(m_seen - m_fin);
+    named_barrier(2, kSoftmax);
+    const float l = lsum[srow] + lsum[BM + srow];
     auto load_o = [&](int col, float (&v)[32]) {
-      if (nb > 0) {
+      if (N > 0) {
         uint32_t o[32];
         tmem_ld32(t_o + col, o);
         tmem_wait_ld_of(o);
@@ -315,56 +402,58 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; i < 32; ++i) v[i] = 0.0f;
       }
     };
-    if (tile.part >= 0) {
+    if (!whole_rows) {
       float* rec = a.parts + diff_record(a, tile.part, kvh, fm, head % G, map);
-      const float unit = F8 && nb > 0 ? v_ref : 1.0f;
 #pragma unroll 1
-      for (int col = 0; col < HD; col += 32) {
+      for (int col = wg * C::MAP; col < (wg + 1) * C::MAP; col += 32) {
         float v[32];
         load_o(col, v);
         if (row_ok) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) *reinterpret_cast<float2*>(rec + col + i) = make_float2(v[i] * unit, v[i + 1] * unit);
+          for (int i = 0; i < 32; i += 2) *reinterpret_cast<float2*>(rec + col + i) = make_float2(v[i] * v_ref, v[i + 1] * v_ref);
         }
       }
-      if (row_ok) *reinterpret_cast<float2*>(rec + HD) = make_float2(m_ref * kLn2, l_run);
+      if (row_ok && wg == 0) *reinterpret_cast<float2*>(rec + HD) = make_float2(m_fin * kLn2, l);
     } else {
-      // map 1 takes columns [0, 64), map 2 [64, 128): each hands the other's half over in shared memory ([column][row]: lanes side
-      // by side), already divided by its sum (and times lam). The K tiles are spent: every Q . K^T came before the last P . V.
-      float* give = reinterpret_cast<float*>(k_sm) + (map ^ 1) * 64 * BM;
-      const float* take = reinterpret_cast<const float*>(k_sm) + map * 64 * BM;
-      float* sq = reinterpret_cast<float*>(v_sm);  // both warpgroups have seen their last P . V at the barrier below
-      const float inv = l_run > 0.0f ? (map ? -diff_lam(args, row, head) : 1.0f) * (F8 ? v_ref : 1.0f) / l_run : 0.0f;
+      constexpr int MINE = HD / 4;  // columns a thread finishes: CTA `map` has [map HD / 2, ..), group wg half of those
+      float* take = reinterpret_cast<float*>(v_sm);         // [HD / 2 columns][128 rows], lanes side by side; written by the peer
+      float* sq = reinterpret_cast<float*>(q_sm);           // [CTA * 2 + group][128 rows]: the rows' sums of squares; written by both
+      const float inv = l > 0.0f ? (map ? -diff_lam(args, row, head) : 1.0f) * v_ref / l : 0.0f;
+      cluster_sync();  // neither CTA uses its tiles any more
+      const uint32_t peer_take = peer_addr(take, uint32_t(map ^ 1)) + uint32_t((wg * MINE * BM + srow) * 4);
 #pragma unroll 1
-      for (int q = 0; q < 2; ++q) {
+      for (int q = 0; q < MINE / 32; ++q) {
         float v[32];
-        load_o(64 * (map ^ 1) + 32 * q, v);
+        load_o((map ^ 1) * C::MAP + wg * MINE + 32 * q, v);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) give[(32 * q + i) * BM + srow] = v[i] * inv;
+        for (int i = 0; i < 32; ++i) peer_store(peer_take + uint32_t((32 * q + i) * BM * 4), v[i] * inv);
       }
-      float dv[64];
+      float dv[MINE];
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
+      for (int q = 0; q < MINE / 32; ++q) {
         float v[32];
-        load_o(64 * map + 32 * q, v);
+        load_o(map * C::MAP + wg * MINE + 32 * q, v);
 #pragma unroll
         for (int i = 0; i < 32; ++i) dv[32 * q + i] = v[i] * inv;
       }
-      named_barrier(2, kSoftmax);
+      cluster_sync();  // the peer's half has arrived
       float ss = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 64; ++i) {
-        dv[i] += take[i * BM + srow];
+      for (int i = 0; i < MINE; ++i) {
+        dv[i] += take[(wg * MINE + i) * BM + srow];
         ss = fmaf(dv[i], dv[i], ss);
       }
-      sq[map * BM + srow] = ss;
-      named_barrier(2, kSoftmax);
-      const float f = diff_row_factor(args, ss + sq[(map ^ 1) * BM + srow], HD);
+      sq[(map * 2 + wg) * BM + srow] = ss;
+      peer_store(peer_addr(sq, uint32_t(map ^ 1)) + uint32_t(((map * 2 + wg) * BM + srow) * 4), ss);
+      cluster_sync();
+      ss = sq[srow] + sq[BM + srow] + sq[2 * BM + srow] + sq[3 * BM + srow];  // the same order in both CTAs
+      const float f = diff_row_factor(args, ss, HD);
       if (row_ok) {
-        typename QE::T* op = static_cast<typename QE::T*>(a.O) + size_t(row) * p.q_ld + size_t(head) * HD + map * 64;
-        const float* w = args.norm_w ? args.norm_w + map * 64 : nullptr;
+        const int col = map * C::MAP + wg * MINE;
+        typename QE::T* op = static_cast<typename QE::T*>(a.O) + size_t(row) * p.q_ld + size_t(head) * HD + col;
+        const float* w = args.norm_w ? args.norm_w + col : nullptr;
 #pragma unroll
-        for (int i = 0; i < 64; i += 8) {
+        for (int i = 0; i < MINE; i += 8) {
           float x[8];
 #pragma unroll
           for (int k = 0; k < 8; ++k) x[k] = dv[i + k] * f * (w ? w[i + k] : 1.0f);
@@ -375,34 +464,58 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   tc_fence_before_sync();
   __syncthreads();
-  if (warp == kMmaWarp) tmem_dealloc(sh.tmem, 512);
+  if (warp == kMmaWarp) tmem_dealloc(sh.tmem, C::COLS);
+}
+
+template <int HD, int QDT, bool F8>
+cudaError_t setup_one() {
+  return cudaFuncSetAttribute(diff_umma_kernel<HD, QDT, F8>, cudaFuncAttributeMaxDynamicSharedMemorySize, Geo<HD>::SMEM);
+}
+template <int HD>
+cudaError_t setup_hd() {
+  cudaError_t e = setup_one<HD, ESP_F16, false>();
+  if (e == cudaSuccess) e = setup_one<HD, ESP_BF16, false>();
+  if (e == cudaSuccess) e = setup_one<HD, ESP_F16, true>();
+  if (e == cudaSuccess) e = setup_one<HD, ESP_BF16, true>();
+  return e;
+}
+template <int HD>
+cudaError_t launch_hd(const DiffArgs& a, bool f8, const CUtensorMap& pool_map, const CUtensorMap& kb_map, const CUtensorMap& vb_map, cudaStream_t stream) {
+  const bool f16 = a.k.q_dtype == ESP_F16;
+  auto kernel = f8 ? (f16 ? diff_umma_kernel<HD, ESP_F16, true> : diff_umma_kernel<HD, ESP_BF16, true>)
+                   : (f16 ? diff_umma_kernel<HD, ESP_F16, false> : diff_umma_kernel<HD, ESP_BF16, false>);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(a.k.n_tiles), unsigned(a.k.p.H / (BM / a.k.tile_rows)), 2), cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = Geo<HD>::SMEM, cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 1, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 2;
+  cfg.attrs = attr, cfg.numAttrs = 2;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, pool_map, kb_map, vb_map, a);
+  return e == cudaSuccess ? cudaGetLastError() : e;
 }
 
 }  // namespace
 
 // 128 / tile_rows heads of a tile must belong to one kv head.
-bool diff_umma_supports(int32_t HDim, int32_t G, int32_t tile_rows, int32_t bt) {
-  if (HDim != HD || bt <= 0 || bt % 16 != 0) return false;
+bool diff_umma_supports(int32_t HD, int32_t G, int32_t tile_rows, int32_t bt) {
+  if ((HD != 128 && HD != 256) || bt <= 0 || bt % 16 != 0) return false;
   if (tile_rows != 16 && tile_rows != 32 && tile_rows != 64 && tile_rows != 128) return false;
   const int hpc = BM / tile_rows;
   return hpc <= G && G % hpc == 0;
 }
 
 cudaError_t diff_umma_setup() {
-  cudaError_t e = cudaFuncSetAttribute(diff_umma_kernel<ESP_F16, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(diff_umma_kernel<ESP_BF16, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(diff_umma_kernel<ESP_F16, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(diff_umma_kernel<ESP_BF16, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
-  return e;
+  const cudaError_t e = setup_hd<128>();
+  return e == cudaSuccess ? setup_hd<256>() : e;
 }
 
 cudaError_t launch_diff_umma(const DiffArgs& a, bool f8, const CUtensorMap& pool_map, const CUtensorMap& kb_map, const CUtensorMap& vb_map, cudaStream_t stream,
                              uint64_t* launches) {
   if (a.k.n_tiles <= 0) return cudaSuccess;
-  const dim3 grid(unsigned(a.k.n_tiles), unsigned(a.k.p.H / (BM / a.k.tile_rows)));
-  const bool f16 = a.k.q_dtype == ESP_F16;
-  auto kernel = f8 ? (f16 ? diff_umma_kernel<ESP_F16, true> : diff_umma_kernel<ESP_BF16, true>) : (f16 ? diff_umma_kernel<ESP_F16, false> : diff_umma_kernel<ESP_BF16, false>);
-  const cudaError_t e = launch_pdl(kernel, grid, dim3(kThreads), SMEM, stream, pool_map, kb_map, vb_map, a);
+  const cudaError_t e = a.k.HD == 128 ? launch_hd<128>(a, f8, pool_map, kb_map, vb_map, stream) : launch_hd<256>(a, f8, pool_map, kb_map, vb_map, stream);
   if (e == cudaSuccess) ++*launches;
   return e;
 }

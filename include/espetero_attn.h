@@ -507,11 +507,11 @@ int esp_kv_append(esp_attn_ctx* ctx, void* stream, const esp_kv_append_args* arg
  *    suit a pass; every plan of esp_attn_plan is right, some are slow (see below).
  * A row that sees no key gets zeros. Rows that no tile covers are left as they were. Keys behind a tree's last row and pool
  * rows past P are never mixed in, whatever they hold; keys that another row of the same tree sees must be finite.
- * Kernels: "diff_decode" (all trees have one row, G <= 8, HD 128 or 256, pages of 16 n keys), "diff_umma" (HD 128) and
- * "diff_umma_pair" (HD 256) for tiles of 128 / c rows, c heads, c <= G (16-bit pools; E4M3 pools through dequant_scratch as in
- * esp_attn_forward, and passes without cached keys), "diff_general" for everything else, plus "diff_combine" for split plans.
+ * Kernels: "diff_decode" (all trees have one row, G <= 8, HD 128 or 256, pages of 16 n keys), "diff_umma"
+ * (HD 128 or 256, pages of 16 n keys, tile ranges that start at a multiple of 16) for tiles of 16, 32, 64 or 128 rows, 128 / tile_rows heads of
+ * one kv head each (16-bit pools; E4M3 pools through dequant_scratch, sized as for esp_attn_forward; passes without cached keys), "diff_general" for everything else, plus "diff_combine" for split plans.
  * esp_attn_last_kernel names the first of these. Sums, maxima and the difference are fp32; softmax weights are rounded to the
- * pass's 16-bit type (fp16 over E4M3 pools in diff_decode) before they meet V. */
+ * pass's 16-bit type (fp16 over E4M3 pools in diff_decode, not at all in diff_general) before they meet V. */
 typedef struct esp_diff_args {
   const float* lam;    /* lam[row * lam_ld + h]: per head, lam_ld = 0, or per row and head, lam_ld >= H */
   const float* norm_w; /* [HD], or NULL: no norm */

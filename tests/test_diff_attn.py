@@ -108,7 +108,7 @@ def test_decode_long_and_hidden_from_itself():
     assert O[0].any() and not O[1].any() and O[2].any()
 
 
-TC = {128: "diff_umma"}
+TC = {128: "diff_umma", 256: "diff_umma"}
 # name, trees (P, M), H, Hkv, bt, pool, mask, tile_rows, split
 ROWS_CASES = [
     ("prefill", [(0, 1), (0, 15), (0, 128), (0, 129), (0, 300)], 4, 2, 16, None, "causal", 128, 0),

@@ -49,6 +49,11 @@ struct esp_attn_ctx {
   const void* umap_kb = nullptr;
   const void* umap_vb = nullptr;
   uint64_t umap_base = 0;
+  // differential attention reads Kb / Vb 128 rows at a time
+  CUtensorMap dkb_map{}, dvb_map{};
+  const void* dmap_kb = nullptr;
+  const void* dmap_vb = nullptr;
+  int32_t dmap_rows = 0, dmap_ld = 0;
   int32_t umap_blocks = 0, umap_rows = 0, umap_ld = 0;
   // Re-planning of reference-shaped multi-row passes (8-row tiles) for the tensor-core kernels: the new
   // tiles and jobs are built on the host and travel through a small ring of pinned staging slots into
@@ -248,11 +253,11 @@ int pool_tensor_map(esp_attn_ctx* c, const esp_attn_args& a) {
   return ESP_OK;
 }
 
-// One 3-D map [64 elements][rows][kv_ld / 64] over 16-bit rows of width kv_ld, box = 64 x 16 x 1.
-int rows_tensor_map(esp_attn_ctx* c, CUtensorMap* out, const void* base, uint64_t rows, int32_t kv_ld) {
+// One 3-D map [64 elements][rows][kv_ld / 64] over 16-bit rows of width kv_ld, box = 64 x box_rows x 1.
+int rows_tensor_map(esp_attn_ctx* c, CUtensorMap* out, const void* base, uint64_t rows, int32_t kv_ld, uint32_t box_rows = 16) {
   const cuuint64_t gdim[3] = {64, rows, cuuint64_t(kv_ld) / 64};
   const cuuint64_t gstride[2] = {cuuint64_t(kv_ld) * 2, 128};
-  const cuuint32_t box[3] = {64, 16, 1};
+  const cuuint32_t box[3] = {64, box_rows, 1};
   const cuuint32_t estr[3] = {1, 1, 1};
   const CUresult r = reinterpret_cast<EncodeTiledFn>(c->encode_tiled)(
       out, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(base), gdim, gstride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -1283,9 +1288,15 @@ int esp_diff_forward(esp_attn_ctx* c, void* stream, const esp_attn_args* ap, con
       w.kv = nullptr;
     }
     if (int rc = umma_tensor_maps(c, w)) return rc;
+    if (c->dmap_kb != a.Kb || c->dmap_vb != a.Vb || c->dmap_rows != a.n_rows || c->dmap_ld != a.p.kv_ld) {
+      c->dmap_kb = c->dmap_vb = nullptr;
+      if (int rc = rows_tensor_map(c, &c->dkb_map, a.Kb, uint64_t(a.n_rows), a.p.kv_ld, 128)) return rc;
+      if (int rc = rows_tensor_map(c, &c->dvb_map, a.Vb, uint64_t(a.n_rows), a.p.kv_ld, 128)) return rc;
+      c->dmap_kb = a.Kb, c->dmap_vb = a.Vb, c->dmap_rows = a.n_rows, c->dmap_ld = a.p.kv_ld;
+    }
     c->last_kernel = "diff_umma";
     ProfScope prof(c, st, c->last_kernel);
-    e = esp::launch_diff_umma(d, widen, c->upool_map, c->kb_map, c->vb_map, st, &c->launches);
+    e = esp::launch_diff_umma(d, widen, c->upool_map, c->dkb_map, c->dvb_map, st, &c->launches);
   } else {
     c->last_kernel = "diff_general";
     ProfScope prof(c, st, c->last_kernel);

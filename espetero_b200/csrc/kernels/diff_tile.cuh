@@ -163,13 +163,13 @@ __device__ __forceinline__ void hide(uint32_t (&s)[32], uint32_t visible) {
     if (!((visible >> c) & 1u)) s[c] = 0xFF800000u;  // -inf
 }
 
-// A TMA producer warp's walk over the pages of its tile's blocks: lane w < 8 handles the w-th 16-key page of every block. `load(kind, y)`
-// is called by those lanes, block after block: kind -1 nothing to load (past the range), 0 row y of the pool (its page is `blk` of the
-// region), 1 row y of Kb / Vb. `which`: 0 keys, 1 values. F8: the pool map covers the widened pages, which lie in the order of the
-// block list. Table entries are fetched four blocks per load, two groups ahead of their use; an entry outside the region is
-// recorded and block 0 stands in for it.
-template <bool F8, class Load>
-__device__ __forceinline__ void walk_pages(const KernelArgs& a, const esp_attn_tree& tree, const BlockList& L, int which, int lane, Load&& load) {
+// A TMA producer warp's walk over its tile's blocks. `page(b, kind, y, blk)` is called by lanes 0 .. 7 for the lane's 16-key page of cached
+// block b: kind -1 nothing to load (past the range), 0 row y of the pool (its page is `blk` of the region). `rows(b, y)` is called by
+// the same lanes for batch block b, which begins at row y of Kb / Vb. `which`: 0 keys, 1 values. F8: the pool map covers the widened
+// pages, which lie in the order of the block list. Table entries are fetched four blocks per load, two groups ahead of their use; an
+// entry outside the region is recorded and block 0 stands in for it.
+template <bool F8, class Page, class Rows>
+__device__ __forceinline__ void walk_pages(const KernelArgs& a, const esp_attn_tree& tree, const BlockList& L, int which, int lane, Page&& page, Rows&& rows) {
   const int bt = a.p.bt;
   auto group = [&](int g) {
     const int b = 4 * g + (lane >> 3), j = L.k0 + BN * b + 16 * (lane & 7);
@@ -189,13 +189,11 @@ __device__ __forceinline__ void walk_pages(const KernelArgs& a, const esp_attn_t
     }
     const int blk = __shfl_sync(0xffffffffu, cur, ((b & 3) << 3) | (lane & 7));
     const int j = L.k0 + BN * b + 16 * lane;
-    const int page = F8 ? tree.table + j / bt : blk;
-    if (lane < kPages) load(b, blk >= 0 ? 0 : -1, (page * 2 + which) * bt + j % bt, blk);
+    const int at = F8 ? tree.table + j / bt : blk;
+    if (lane < kPages) page(b, blk >= 0 ? 0 : -1, (at * 2 + which) * bt + j % bt, blk);
   }
-  for (int b = L.nbc; b < L.n(); ++b) {
-    const int j = L.j0(b) + 16 * lane;
-    if (lane < kPages) load(b, j <= L.k_last ? 1 : -1, tree.base + j, 0);
-  }
+  for (int b = L.nbc; b < L.n(); ++b)
+    if (lane < kPages) rows(b, tree.base + L.j0(b));
 }
 
 __device__ __forceinline__ float chunk_max(const uint32_t (&s)[32]) {

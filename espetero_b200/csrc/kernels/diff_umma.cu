@@ -19,7 +19,8 @@
 //
 // Bound per 128 keys of a tile: 256-dim heads 1536 clocks of MMA per map (8 instructions of N = 128 and 8 of N = 256, 64 and 128
 // clocks each) on an SM, 1024 of exponentials; 128-dim heads 1024 of exponentials per map, two maps per SM, against 1600 of MMA.
-// Warps 0-7 softmax, 8 MMA issue (owns tensor memory), 9 / 10 K / V producers (TMA, one load per 16-key page and 64-dim chunk), 11 idle (it
+// Warps 0-7 softmax, 8 MMA issue (owns tensor memory), 9 / 10 K / V producers (TMA, one load per 16-key page and 64-dim chunk of the pool,
+// one per 128 rows of the batch), 11 idle (it
 // completes the warpgroup that hands registers over). Hand-offs by mbarrier; every wait is bounded: after a timeout the CTA records a
 // code, stops waiting, finishes its loop, frees its tensor memory and returns.
 // E4M3 pools (F8): the pages are 16-bit codes (diff_widen.cu); the K producer leaves each block's page scales in shared memory, the
@@ -57,7 +58,7 @@ struct Geo {
 constexpr int kRegsAux = 96, kRegsSoftmax = 200;  // 256-dim heads
 constexpr int kSlots = 4;  // blocks whose page scales are kept
 struct Shared {
-  uint64_t k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], s_full[2], p_full[2], o_done[2], sc_full[kSlots], m_ready[2][4];
+  uint64_t k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], s_full[2], p_full[2][2], o_done[2], sc_full[kSlots], m_ready[2][4];
   uint32_t tmem;
   volatile int dead;
   float k_scale[kSlots][kPages], v_scale[kSlots][kPages];
@@ -99,7 +100,7 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
     for (int s = 0; s < KS; ++s) mbar_init(&sh.k_full[s], kPages), mbar_init(&sh.k_empty[s], 1);
     for (int s = 0; s < VS; ++s) mbar_init(&sh.v_full[s], kPages), mbar_init(&sh.v_empty[s], 1);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&sh.s_full[i], 1), mbar_init(&sh.p_full[i], BM), mbar_init(&sh.o_done[i], 1);
+      mbar_init(&sh.s_full[i], 1), mbar_init(&sh.p_full[i][0], BM), mbar_init(&sh.p_full[i][1], BM), mbar_init(&sh.o_done[i], 1);
       for (int w = 0; w < 4; ++w) mbar_init(&sh.m_ready[i][w], 1);
     }
     for (int s = 0; s < kSlots; ++s) mbar_init(&sh.sc_full[s], 1);
@@ -136,37 +137,55 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
       uint64_t* empty = is_v ? sh.v_empty : sh.k_empty;
       int stage = 0;
       uint32_t par = 1;  // the first use of a slot finds it empty
-      walk_pages<F8>(a, tree, L, is_v ? 1 : 0, lane, [&](int b, int kind, int y, int blk) {
-        float ks = 1.0f, vs = kind < 0 ? 0.0f : 1.0f;
-        if (F8 && !is_v && kind == 0) {
-          ks = a.kv_scales[size_t(blk) * 2 * p.Hkv + kvh];
-          vs = a.kv_scales[(size_t(blk) * 2 + 1) * p.Hkv + kvh];
-        }
-        wait_bar(&empty[stage], par, kStatusMmaTimeout);
-        if (kind < 0) {
-          mbar_arrive(&full[stage]);
-        } else {
-          const CUtensorMap* m = kind ? (is_v ? &vb_map : &kb_map) : &pool_map;
-          if (is_v) {
-            uint8_t* dst = v_sm + stage * C::V_TILE + lane * 2048;
-            mbar_arrive_expect_tx(&full[stage], 2048 * C::VC);
-#pragma unroll
-            for (int i = 0; i < C::VC; ++i) tma_load_3d(dst + i * C::CHUNK, m, &full[stage], 0, y, kvh * C::VC + i);
-          } else {
-            uint8_t* dst = k_sm + stage * C::K_TILE + lane * 2048;
-            mbar_arrive_expect_tx(&full[stage], 2048 * C::QC);
-#pragma unroll
-            for (int i = 0; i < C::QC; ++i) tma_load_3d(dst + i * C::CHUNK, m, &full[stage], 0, y, kvh * C::VC + map * C::QC + i);
-          }
-        }
-        if (F8 && !is_v) {
-          const int slot = b % kSlots;
-          sh.k_scale[slot][lane] = ks, sh.v_scale[slot][lane] = vs;
-          __syncwarp(0xFFu);
-          if (lane == 0) mbar_arrive(&sh.sc_full[slot]);
-        }
+      auto advance = [&]() {
         if (++stage == depth) stage = 0, par ^= 1;
-      });
+      };
+      auto scales = [&](int b, float ks, float vs) {  // this lane's page of block b
+        if (!F8 || is_v) return;
+        const int slot = b % kSlots;
+        sh.k_scale[slot][lane] = ks, sh.v_scale[slot][lane] = vs;
+        __syncwarp(0xFFu);
+        if (lane == 0) mbar_arrive(&sh.sc_full[slot]);
+      };
+      walk_pages<F8>(
+          a, tree, L, is_v ? 1 : 0, lane,
+          [&](int b, int kind, int y, int blk) {
+            float ks = 1.0f, vs = kind < 0 ? 0.0f : 1.0f;
+            if (F8 && !is_v && kind == 0) {
+              ks = a.kv_scales[size_t(blk) * 2 * p.Hkv + kvh];
+              vs = a.kv_scales[(size_t(blk) * 2 + 1) * p.Hkv + kvh];
+            }
+            wait_bar(&empty[stage], par, kStatusMmaTimeout);
+            if (kind < 0) {
+              mbar_arrive(&full[stage]);
+            } else if (is_v) {
+              uint8_t* dst = v_sm + stage * C::V_TILE + lane * 2048;
+              mbar_arrive_expect_tx(&full[stage], 2048 * C::VC);
+#pragma unroll
+              for (int i = 0; i < C::VC; ++i) tma_load_3d(dst + i * C::CHUNK, &pool_map, &full[stage], 0, y, kvh * C::VC + i);
+            } else {
+              uint8_t* dst = k_sm + stage * C::K_TILE + lane * 2048;
+              mbar_arrive_expect_tx(&full[stage], 2048 * C::QC);
+#pragma unroll
+              for (int i = 0; i < C::QC; ++i) tma_load_3d(dst + i * C::CHUNK, &pool_map, &full[stage], 0, y, kvh * C::VC + map * C::QC + i);
+            }
+            scales(b, ks, vs);
+            advance();
+          },
+          // Batch rows are contiguous: one load of 128 rows per chunk, by as many lanes. (Rows behind the tree's last one come along:
+          // other trees' or none, zero past the tensor. Their scores are hidden and their V rows cleared.)
+          [&](int b, int y) {
+            wait_bar(&empty[stage], par, kStatusMmaTimeout);
+            if (lane < (is_v ? C::VC : C::QC)) {
+              mbar_arrive_expect_tx(&full[stage], C::CHUNK);
+              if (is_v) tma_load_3d(v_sm + stage * C::V_TILE + lane * C::CHUNK, &vb_map, &full[stage], 0, y, kvh * C::VC + lane);
+              else tma_load_3d(k_sm + stage * C::K_TILE + lane * C::CHUNK, &kb_map, &full[stage], 0, y, kvh * C::VC + map * C::QC + lane);
+            } else {
+              mbar_arrive(&full[stage]);
+            }
+            scales(b, 1.0f, 1.0f);
+            advance();
+          });
       __syncwarp();
     } else if (warp == kMmaWarp) {
       tmem_alloc(&sh.tmem, C::COLS);
@@ -209,13 +228,16 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
           for (int i = 0; i < 2; ++i) {
             const int n = n0 + i, h = i % C::UPB;
             if (n >= N) break;
-            wait_bar(&sh.p_full[i], uint32_t(n >> 1) & 1u, kStatusMmaTimeout);
-            if (h == 0) wait_bar(&sh.v_full[vst], vpar, kStatusTmaTimeout);
-            tc_fence_after_sync();
             const uint32_t v_lo = v_lo0 + uint32_t(vst) * (C::V_TILE >> 4) + uint32_t((h * C::BU * 128) >> 4);
 #pragma unroll
-            for (int ks = 0; ks < C::BU / 16; ++ks)
-              mma_ts(one, tmem + C::COL_O, tmem + C::COL_S + i * C::BU + ks * 8, v_lo + ((ks * 16 * 128) >> 4), hi_v, idesc_pv, ks > 0 ? 1u : uint32_t(n > 0));
+            for (int part = 0; part < C::BU / 64; ++part) {  // P comes in parts of 64 keys
+              wait_bar(&sh.p_full[i][part], uint32_t(n >> 1) & 1u, kStatusMmaTimeout);
+              if (part == 0 && h == 0) wait_bar(&sh.v_full[vst], vpar, kStatusTmaTimeout);
+              tc_fence_after_sync();
+#pragma unroll
+              for (int ks = 4 * part; ks < 4 * part + 4; ++ks)
+                mma_ts(one, tmem + C::COL_O, tmem + C::COL_S + i * C::BU + ks * 8, v_lo + ((ks * 16 * 128) >> 4), hi_v, idesc_pv, ks > 0 ? 1u : uint32_t(n > 0));
+            }
             mma_commit(one, &sh.o_done[i]);
             if (h == C::UPB - 1) {
               mma_commit(one, &sh.v_empty[vst]);
@@ -366,13 +388,15 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
         uint32_t pk[16];
         chunk_weights<QDT, F8>(s[C::HOLD ? i : 0], pk, sl2x2, neg_m2, sum, F8 ? vs[2 * i] * vinv : 1.0f, F8 ? vs[2 * i + 1] * vinv : 1.0f);
         tmem_st16(buf + 16 * i, pk);
+        if (i & 1) {  // 64 keys are ready: their P . V starts under the rest
+          tmem_wait_st();
+          tc_fence_before_sync();
+          mbar_arrive(&sh.p_full[wg][i >> 1]);
+        }
       }
       float a0, a1;
       f32x2_unpack(f32x2_add(sum[0], sum[1]), a0, a1);
       l_run += a0 + a1;
-      tmem_wait_st();
-      tc_fence_before_sync();
-      mbar_arrive(&sh.p_full[wg]);
     }
 
     // ---- epilogue
@@ -419,6 +443,9 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
       float* take = reinterpret_cast<float*>(v_sm);         // [HD / 2 columns][128 rows], lanes side by side; written by the peer
       float* sq = reinterpret_cast<float*>(q_sm);           // [CTA * 2 + group][128 rows]: the rows' sums of squares; written by both
       const float inv = l > 0.0f ? (map ? -diff_lam(args, row, head) : 1.0f) * v_ref / l : 0.0f;
+      // the norm's weights into shared memory while the peer gets here (16-byte aligned, HD floats)
+      float* w_sm = reinterpret_cast<float*>(k_sm) + 2 * BM;
+      if (args.norm_w && tid < HD / 4) reinterpret_cast<float4*>(w_sm)[tid] = reinterpret_cast<const float4*>(args.norm_w)[tid];
       cluster_sync();  // neither CTA uses its tiles any more
       const uint32_t peer_take = peer_addr(take, uint32_t(map ^ 1)) + uint32_t((wg * MINE * BM + srow) * 4);
 #pragma unroll 1
@@ -451,12 +478,16 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
       if (row_ok) {
         const int col = map * C::MAP + wg * MINE;
         typename QE::T* op = static_cast<typename QE::T*>(a.O) + size_t(row) * p.q_ld + size_t(head) * HD + col;
-        const float* w = args.norm_w ? args.norm_w + col : nullptr;
+        const float* w = w_sm + col;  // every lane reads the same word
 #pragma unroll
         for (int i = 0; i < MINE; i += 8) {
           float x[8];
 #pragma unroll
-          for (int k = 0; k < 8; ++k) x[k] = dv[i + k] * f * (w ? w[i + k] : 1.0f);
+          for (int k = 0; k < 8; ++k) x[k] = dv[i + k] * f;
+          if (args.norm_w) {
+            const float4 w0 = *reinterpret_cast<const float4*>(w + i), w1 = *reinterpret_cast<const float4*>(w + i + 4);
+            x[0] *= w0.x, x[1] *= w0.y, x[2] *= w0.z, x[3] *= w0.w, x[4] *= w1.x, x[5] *= w1.y, x[6] *= w1.z, x[7] *= w1.w;
+          }
           *reinterpret_cast<uint4*>(op + i) = make_uint4(QE::pack2(x[0], x[1]), QE::pack2(x[2], x[3]), QE::pack2(x[4], x[5]), QE::pack2(x[6], x[7]));
         }
       }

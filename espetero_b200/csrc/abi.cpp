@@ -1202,7 +1202,7 @@ size_t esp_diff_parts_floats(const esp_attn_shape* s, int32_t n_parts) { return 
 
 int esp_diff_plan_opts(const esp_attn_shape* s, const esp_attn_tree* trees, int32_t n_trees, esp_plan_opts* o) {
   if (!s || !o || n_trees < 0 || (!trees && n_trees > 0)) return fail(ESP_ERR_INVALID, "esp_diff_plan_opts: null or negative argument");
-  if (s->H <= 0 || s->Hkv <= 0 || s->H % s->Hkv) return fail(ESP_ERR_INVALID, "esp_diff_plan_opts: H=%d Hkv=%d", s->H, s->Hkv);
+  if (s->H <= 0 || s->Hkv <= 0 || s->H % s->Hkv || s->HD <= 0) return fail(ESP_ERR_INVALID, "esp_diff_plan_opts: H=%d Hkv=%d HD=%d", s->H, s->Hkv, s->HD);
   int64_t cached = 0, fresh = 0;
   bool single = true;
   for (int i = 0; i < n_trees; ++i) {
@@ -1214,8 +1214,8 @@ int esp_diff_plan_opts(const esp_attn_shape* s, const esp_attn_tree* trees, int3
   *o = esp_plan_opts{};
   o->mode = ESP_PLAN_B200, o->min_chunk = 32, o->max_parts = 64;
   const int G = s->H / s->Hkv;
-  if (single) {
-    o->tile_rows = 8, o->groups = 148 * 4, o->split = 1 << 20;
+  if (single) {  // diff_decode: one wave of its CTAs (two per SM, four where a key block is 4 KB)
+    o->tile_rows = 8, o->groups = 148 * (s->kv_dtype == ESP_E4M3 && s->HD == 128 ? 4 : 2), o->split = 1 << 20;
     return ESP_OK;
   }
   if (cached <= 2 * fresh) {  // mostly its own rows: 128-row tiles, one head each, nothing split
@@ -1224,7 +1224,36 @@ int esp_diff_plan_opts(const esp_attn_shape* s, const esp_attn_tree* trees, int3
   }
   int c = 8;  // heads per tile
   while (c > 1 && (c > G || G % c)) c >>= 1;
-  o->tile_rows = 128 / c, o->groups = std::max(1, 148 * c / G), o->split = 1 << 20;
+  o->tile_rows = 128 / c;
+  // How far to split the cached keys, by the time each choice would take: CTAs (two per tile and head group) on the SMs' slots, a
+  // fixed cost per CTA and one per 128 keys, and the join of the records. Microseconds, measured on diff_umma; with 128-dim heads two
+  // CTAs share an SM and each runs slower than alone.
+  const bool wide = s->HD >= 256;
+  const int per_tile = s->Hkv * (G / c) * 2;
+  const double t_block = 1.05, t_shared = 1.45, t_fixed = 9.0;  // per 128 keys alone / sharing an SM; start and end of a CTA
+  double best = 0;
+  for (int parts = 1; parts <= 32; ++parts) {
+    int64_t tiles = 0, rows_split = 0;
+    int longest = 0;
+    for (int i = 0; i < n_trees; ++i) {
+      const int64_t groups = (trees[i].M + o->tile_rows - 1) / o->tile_rows;
+      const int ns = trees[i].P >= 64 ? std::min(parts, std::max(1, trees[i].P / 128)) : 1;
+      tiles += groups * ns;
+      if (ns > 1) rows_split += int64_t(trees[i].M) * ns;
+      longest = std::max(longest, (trees[i].P / ns + 127) / 128 + (ns == 1 ? (std::min(trees[i].M, 1 << 20) + 127) / 128 : 1));
+    }
+    const int64_t ctas = tiles * per_tile, slots = wide ? 148 : (ctas <= 148 ? 148 : 296);
+    const double waves = double((ctas + slots - 1) / slots);
+    const double per_block = wide ? t_block : (slots == 148 ? 0.9 * t_block : t_shared);
+    const double join = rows_split ? 6.0 + double(rows_split) * s->H * 2 * (s->HD + 2) * 4 * 2 / 4.0e6 : 0.0;  // written and read at about 4 TB/s
+    const double t = waves * (longest * per_block + t_fixed) + join;
+    if (parts == 1 || t < 0.97 * best) {
+      best = t;
+      // the planner sizes its chunks so that the tiles fit `groups / Hkv`
+      o->split = parts == 1 ? 0 : 1 << 20;
+      o->groups = int(std::min<int64_t>(tiles, 1 << 24)) * s->Hkv;
+    }
+  }
   return ESP_OK;
 }
 
@@ -1304,10 +1333,10 @@ int esp_diff_forward(esp_attn_ctx* c, void* stream, const esp_attn_args* ap, con
   }
   if (e != cudaSuccess) return cuda_fail(e, c->last_kernel);
   if (a.n_jobs > 0) {
-    esp::DiffCombineArgs m{d, a.n_jobs, c->tile_rows};
+    esp::DiffCombineArgs m{d, a.n_jobs, c->tile_rows, 64};
     if (a.jobs_host) {
-      m.rows_max = 1;
-      for (int i = 0; i < a.n_jobs; ++i) m.rows_max = std::max(m.rows_max, a.jobs_host[i].rows);
+      m.rows_max = m.parts_max = 1;
+      for (int i = 0; i < a.n_jobs; ++i) m.rows_max = std::max(m.rows_max, a.jobs_host[i].rows), m.parts_max = std::max(m.parts_max, a.jobs_host[i].nparts);
     }
     ProfScope prof(c, st, "diff_combine");
     e = esp::launch_diff_combine(m, st, &c->launches);

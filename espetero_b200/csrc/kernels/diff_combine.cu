@@ -2,32 +2,37 @@
 //
 // A job's records of one (row, head) - two maps, `nparts` records each - become the row: per map
 //   M = max m_s,  L = sum e^(m_s - M) l_s,  A = sum e^(m_s - M) O_s   (records in order, no atomics: the result does not
-// depend on scheduling), then D = A_1 / L_1 - lam A_2 / L_2 and the norm. One CTA per (job row, head): 128 threads per map, HD / 4
-// of them per slice of records (4 dims each), the slices joined in order through shared memory. Latency-bound: a slice asks for
-// up to eight records before it folds the first.
+// depend on scheduling), then D = A_1 / L_1 - lam A_2 / L_2 and the norm. HD / 4 threads (4 dims each) per slice of records, NSL slices
+// per map, two maps per (row, head), as many (row, head) pairs as fit a CTA; the slices are joined in order through shared memory.
+// A slice asks for up to eight records before it folds the first. Few long jobs (decode) are latency-bound and take many slices;
+// many short ones (trees: two records per row) are bound by the records' bytes and take one: 16 x (4096 + 16) trees, split in two,
+// 43.6 us with four slices and one pair per CTA.
 #include "diff.cuh"
 
 namespace esp {
 namespace {
 
-constexpr int kThreads = 256, kPerMap = 128;
+constexpr int kThreads = 256;
 
-template <int HD, int QDT>
+template <int HD, int QDT, int NSL>
 __global__ void __launch_bounds__(kThreads) diff_combine_kernel(const DiffCombineArgs c) {
   using QE = Elem16<QDT>;
-  constexpr int TPD = HD / 4, NSL = kPerMap / TPD;  // threads per slice, slices per map
+  constexpr int TPD = HD / 4, PER_MAP = TPD * NSL, PER_PAIR = 2 * PER_MAP, PAIRS = kThreads / PER_PAIR;
   const DiffArgs& a = c.d;
   const KernelArgs& k = a.k;
   __shared__ float part[kThreads][6];  // 4 dims, L, M of a thread's slice
-  __shared__ float sq[kPerMap / 32];
+  __shared__ float sq[kThreads / 32];
   pdl_wait();
   pdl_launch_dependents();
-  const int job_i = blockIdx.x / c.rows_max, r = blockIdx.x % c.rows_max, h = blockIdx.y, kvh = h / k.G, hg = h % k.G;
-  const esp_attn_combine job = k.jobs[job_i];
-  if (r >= job.rows) return;  // the whole CTA
-  const int tid = threadIdx.x, map = tid / kPerMap, sl = (tid % kPerMap) / TPD, d4 = tid % TPD;
+  const int tid = threadIdx.x, t = tid % PER_PAIR, map = t / PER_MAP, sl = (t % PER_MAP) / TPD, d4 = t % TPD;
+  const int64_t pair = int64_t(blockIdx.x) * PAIRS + tid / PER_PAIR;  // (job, row of the job, head), heads fastest
+  const int h = int(pair % k.p.H), r = int((pair / k.p.H) % c.rows_max), job_i = int(pair / (int64_t(k.p.H) * c.rows_max));
+  esp_attn_combine job{0, 0, 0, 0};
+  if (job_i < c.n_jobs) job = k.jobs[job_i];
+  const bool live = r < job.rows;
+  const int n = live ? job.nparts : 0;
   const size_t stride = diff_record(k, 1, 0, 0, 0, 0);
-  const float* rec0 = k.parts + diff_record(k, job.part0, kvh, r, hg, map);
+  const float* rec0 = k.parts + diff_record(k, job.part0, h / k.G, live ? r : 0, h % k.G, map);
   float M = -INFINITY, L = 0.0f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   auto fold = [&](float m, float l, const float4& o) {
@@ -38,12 +43,12 @@ __global__ void __launch_bounds__(kThreads) diff_combine_kernel(const DiffCombin
     acc.x = acc.x * f + w * o.x, acc.y = acc.y * f + w * o.y, acc.z = acc.z * f + w * o.z, acc.w = acc.w * f + w * o.w;
     M = mn;
   };
-  for (int s = sl; s < job.nparts; s += 8 * NSL) {
+  for (int s = sl; s < n; s += 8 * NSL) {
     float2 ml[8], lo[8], hi[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       ml[i] = make_float2(-INFINITY, 0.0f), lo[i] = hi[i] = make_float2(0.f, 0.f);
-      if (s + i * NSL < job.nparts) {
+      if (s + i * NSL < n) {
         const float* rec = rec0 + size_t(s + i * NSL) * stride;  // records are 8-byte aligned (HD + 2 floats)
         ml[i] = *reinterpret_cast<const float2*>(rec + HD);
         lo[i] = *reinterpret_cast<const float2*>(rec + 4 * d4), hi[i] = *reinterpret_cast<const float2*>(rec + 4 * d4 + 2);
@@ -53,34 +58,38 @@ __global__ void __launch_bounds__(kThreads) diff_combine_kernel(const DiffCombin
     for (int i = 0; i < 8; ++i) fold(ml[i].x, ml[i].y, make_float4(lo[i].x, lo[i].y, hi[i].x, hi[i].y));
   }
   float* mine = part[tid];
-  mine[0] = acc.x, mine[1] = acc.y, mine[2] = acc.z, mine[3] = acc.w, mine[4] = L, mine[5] = M;
-  __syncthreads();
-  // the threads of slice 0 join the slices of their map, map 2's hand their result over, map 1's finish
-  if (sl == 0) {
-    for (int s = 1; s < NSL; ++s) {
-      const float* o = part[tid + s * TPD];
-      fold(o[5], o[4], make_float4(o[0], o[1], o[2], o[3]));
-    }
-    if (map == 1) mine[0] = acc.x, mine[1] = acc.y, mine[2] = acc.z, mine[3] = acc.w, mine[4] = L;
+  if (NSL > 1) {
+    mine[0] = acc.x, mine[1] = acc.y, mine[2] = acc.z, mine[3] = acc.w, mine[4] = L, mine[5] = M;
+    __syncthreads();
+    if (sl == 0)
+      for (int s = 1; s < NSL; ++s) {
+        const float* o = part[tid + s * TPD];
+        fold(o[5], o[4], make_float4(o[0], o[1], o[2], o[3]));
+      }
   }
+  // map 2's first slice hands its result over, map 1's finishes
+  if (sl == 0 && map == 1) mine[0] = acc.x, mine[1] = acc.y, mine[2] = acc.z, mine[3] = acc.w, mine[4] = L;
   __syncthreads();
-  const bool owner = sl == 0 && map == 0;
+  const bool owner = sl == 0 && map == 0 && live;
   float d[4] = {0.f, 0.f, 0.f, 0.f};
   const int row = job.r0 + r;
   if (owner) {
-    const float* o = part[kPerMap + d4];
+    const float* o = part[tid + PER_MAP];
     const float inv1 = L > 0.0f ? 1.0f / L : 0.0f, inv2 = o[4] > 0.0f ? diff_lam(a, row, h) / o[4] : 0.0f;
     d[0] = acc.x * inv1 - o[0] * inv2, d[1] = acc.y * inv1 - o[1] * inv2, d[2] = acc.z * inv1 - o[2] * inv2, d[3] = acc.w * inv1 - o[3] * inv2;
   }
+  // the row's sum of squares: over the TPD owners, which are whole warps or an aligned part of one
   float ss = d[0] * d[0] + d[1] * d[1] + d[2] * d[2] + d[3] * d[3];
 #pragma unroll
-  for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  if (tid < kPerMap && (tid & 31) == 0) sq[tid >> 5] = ss;
-  __syncthreads();
-  if (!owner) return;
-  ss = 0.0f;
+  for (int o = (TPD < 32 ? TPD : 32) / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  if constexpr (TPD > 32) {
+    if ((tid & 31) == 0) sq[tid >> 5] = ss;
+    __syncthreads();
+    ss = 0.0f;
 #pragma unroll
-  for (int i = 0; i < kPerMap / 32; ++i) ss += sq[i];  // threads that are no owners added zeros
+    for (int i = 0; i < TPD / 32; ++i) ss += sq[(tid - t) / 32 + i];
+  }
+  if (!owner) return;
   const float f = diff_row_factor(a, ss, HD);
   const float4 w = a.norm_w ? *reinterpret_cast<const float4*>(a.norm_w + 4 * d4) : make_float4(1.f, 1.f, 1.f, 1.f);
   *reinterpret_cast<uint2*>(static_cast<typename QE::T*>(k.O) + size_t(row) * k.p.q_ld + size_t(h) * HD + 4 * d4) =
@@ -100,14 +109,22 @@ __global__ void diff_lambda_kernel(const float* q1, const float* k1, const float
   if (lane == 0) lam[h] = expf(a) - expf(b) + init;
 }
 
+template <int HD, int QDT>
+cudaError_t launch_hd(const DiffCombineArgs& c, cudaStream_t stream) {
+  constexpr int MOST = 128 / (HD / 4);  // slices that fill a CTA with one pair
+  const bool slices = MOST > 1 && c.parts_max > 8;
+  const int64_t pairs = int64_t(c.n_jobs) * c.rows_max * c.d.k.p.H, per_cta = slices ? 1 : kThreads / (HD / 2);
+  const dim3 grid(unsigned((pairs + per_cta - 1) / per_cta));
+  if (slices) return launch_pdl(diff_combine_kernel<HD, QDT, MOST>, grid, dim3(kThreads), 0, stream, c);
+  return launch_pdl(diff_combine_kernel<HD, QDT, 1>, grid, dim3(kThreads), 0, stream, c);
+}
 template <int QDT>
 cudaError_t launch_typed(const DiffCombineArgs& c, cudaStream_t stream) {
-  const dim3 grid(unsigned(c.n_jobs) * unsigned(c.rows_max), unsigned(c.d.k.p.H));
   switch (c.d.k.HD) {
-    case 64: return launch_pdl(diff_combine_kernel<64, QDT>, grid, dim3(kThreads), 0, stream, c);
-    case 128: return launch_pdl(diff_combine_kernel<128, QDT>, grid, dim3(kThreads), 0, stream, c);
-    case 256: return launch_pdl(diff_combine_kernel<256, QDT>, grid, dim3(kThreads), 0, stream, c);
-    case 512: return launch_pdl(diff_combine_kernel<512, QDT>, grid, dim3(kThreads), 0, stream, c);
+    case 64: return launch_hd<64, QDT>(c, stream);
+    case 128: return launch_hd<128, QDT>(c, stream);
+    case 256: return launch_hd<256, QDT>(c, stream);
+    case 512: return launch_hd<512, QDT>(c, stream);
   }
   return cudaErrorInvalidValue;
 }

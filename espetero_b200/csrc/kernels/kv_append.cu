@@ -8,196 +8,215 @@
 //
 // The angle: an fp32 product loses 2^-25 of up to 10^5 radians at far positions, more than a bf16 step. pos * inv_freq / 2 pi is
 // formed in double (the product of an int32 and an fp32 number is exact there), whole turns are taken off, and the rest, at most
-// half a turn, is good to fp32: rot_half values per row, formed once per CTA in shared memory.
+// half a turn, is good to fp32.
 //
-// HBM-bound for prompts (every byte is read and written once), latency-bound for single tokens. A thread's item is one rotating
-// pair of 8-dim chunks, (d, d + rot_half), or one chunk that needs no partner: 16-byte loads and stores, and since an item's
-// reads precede its own writes and no other item touches them, outputs may lie over the sources. Rows whose addresses or sizes do
-// not allow 16-byte accesses take the same kernel with one-dim items.
+// HBM-bound for prompts (every byte is read and written once), latency-bound for single tokens. A warp owns one row, or a part of it when
+// rows are few. A lane's item is a rotating pair of 8-dim chunks, (d, d + rot_half), or one chunk that needs no partner; 32 lanes
+// cover 32 / P2 maps, P2 = the items of a map rounded up to a power of two, so a lane's place within a map is the same in every step:
+// it forms its 4 or 8 sines and cosines once, in registers, addresses advance by a constant, and nothing is shared between warps.
+// 8192 rows of H32 / Hkv4 / HD128, fp16: 34.4 us = 5.37 TB/s = 0.82 of the copy peak (71.7 us with a table of sines per CTA and items
+// dealt out by division, which left the instruction issue and the CTAs' trips to memory in charge); 5001 fp32 rows of H16 / Hkv2 / HD256:
+// 36.8 us = 4.45 TB/s. kBatch items are asked for before the first is turned: 2 at three CTAs per SM; 4 and 8 measured 36.6 and 41.2 us, 1
+// 43.0.
+// An item's reads precede its own writes and no other item touches its bytes, so outputs may lie over the sources.
+#include <type_traits>
+
 #include "common.cuh"
 #include "../launch.h"
 
 namespace esp {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kWarps = 8, kThreads = 32 * kWarps;
+constexpr int kBatch = 2;  // items a lane asks for at once
 
-template <int QDT, bool SRC32, bool FP8_POOL, int VEC>
-__global__ void __launch_bounds__(kThreads) kv_append_kernel(const AppendArgs args, const int HD, const int rows_per_cta) {
-  using QE = Elem16<QDT>;
-  using T = typename QE::T;
-  const esp_kv_append_args& a = args.a;
-  const esp_attn_params& p = a.p;
-  extern __shared__ float2 turn[];  // [row of the CTA][rot_half]: cos, sin
-  const int D = HD / a.maps, half = a.rot_half;
-  const int row0 = blockIdx.x * rows_per_cta;
-  const int n_rows = min(rows_per_cta, a.rows - row0);
-  pdl_wait();  // the projection, and what a pass before this one may still read of the pool
-
-  for (int i = threadIdx.x; i < n_rows * half; i += kThreads) {
-    const int r = i / half, f = i - r * half;
-    const double turns = double(a.pos[row0 + r]) * double(a.inv_freq[f]) * 0.15915494309189533577;
-    float s, c;
-    sincospif(2.0f * float(turns - rint(turns)), &s, &c);
-    turn[i] = make_float2(c, s);
-  }
-  __syncthreads();
-  pdl_launch_dependents();
-
-  // items of one map: rotating chunk pairs first, then the chunks that pass through; adjacent pairs lie within a chunk
-  const int n_pair = a.adjacent ? 0 : half / VEC;
-  const int per_map = a.adjacent ? D / VEC : n_pair + (D - 2 * half) / VEC;
-  const int per_head = per_map * a.maps, v_head = HD / VEC;
-  const int n_q = a.Q ? p.H * per_head : 0, n_k = p.Hkv * per_head, n_v = p.Hkv * v_head;
-  const int per_row = n_q + n_k + n_v;
-
-  auto load = [&](const void* base, int64_t at, float (&x)[VEC]) {
-    if constexpr (SRC32) {
-      const float* src = static_cast<const float*>(base) + at;
-      if constexpr (VEC == 8) {
-        const float4 u = reinterpret_cast<const float4*>(src)[0], w = reinterpret_cast<const float4*>(src)[1];
-        x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w, x[4] = w.x, x[5] = w.y, x[6] = w.z, x[7] = w.w;
-      } else {
-        x[0] = src[0];
-      }
-    } else {
-      const T* src = static_cast<const T*>(base) + at;
-      if constexpr (VEC == 8) {
-        const uint4 u = *reinterpret_cast<const uint4*>(src);
-        const float2 f0 = QE::unpack2(u.x), f1 = QE::unpack2(u.y), f2 = QE::unpack2(u.z), f3 = QE::unpack2(u.w);
-        x[0] = f0.x, x[1] = f0.y, x[2] = f1.x, x[3] = f1.y, x[4] = f2.x, x[5] = f2.y, x[6] = f3.x, x[7] = f3.y;
-      } else {
-        x[0] = QE::to_f32(src[0]);
-      }
-    }
-  };
-  // 16-bit values of x at `dst`; x becomes those values again (what an E4M3 pool encodes)
-  auto round16 = [&](float (&x)[VEC], uint32_t (&w)[VEC == 8 ? 4 : 1]) {
-    if constexpr (VEC == 8) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = QE::pack2(x[2 * i], x[2 * i + 1]);
-    } else {
-      w[0] = QE::pack2(x[0], 0.0f);
-    }
-  };
-  auto store16 = [&](void* base, size_t at, const uint32_t (&w)[VEC == 8 ? 4 : 1]) {
-    T* dst = static_cast<T*>(base) + at;
-    if constexpr (VEC == 8) *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-    else *reinterpret_cast<uint16_t*>(dst) = uint16_t(w[0]);
-  };
-  auto store_pool = [&](size_t at, const uint32_t (&w)[VEC == 8 ? 4 : 1], float scale) {
-    if constexpr (!FP8_POOL) {
-      store16(a.kv, at, w);
-    } else {
-      // division, as esp_kv_save does, so that both give the same codes
-      uint8_t* dst = static_cast<uint8_t*>(a.kv) + at;
-      if constexpr (VEC == 8) {
-        uint32_t o[2] = {0, 0};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 f = QE::unpack2(w[i]);
-          const uint32_t two = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(f.x, scale), __fdiv_rn(f.y, scale)), __NV_SATFINITE, __NV_E4M3);
-          o[i >> 1] |= two << (16 * (i & 1));
-        }
-        *reinterpret_cast<uint2*>(dst) = make_uint2(o[0], o[1]);
-      } else {
-        *dst = f32_to_e4m3(__fdiv_rn(QE::unpack2(w[0]).x, scale));
-      }
-    }
-  };
-
-  const int total = n_rows * per_row;
-  for (int idx = blockIdx.y * kThreads + threadIdx.x; idx < total; idx += kThreads * gridDim.y) {
-    const int r = idx / per_row, item = idx - r * per_row;
-    const int row = row0 + r;
-    const float2* tr = turn + r * half;
-    const bool is_v = item >= n_q + n_k, is_q = item < n_q;
-    const int rel = is_q ? item : (is_v ? item - n_q - n_k : item - n_q);
-    const int head = rel / (is_v ? v_head : per_head);
-    int in_head = rel - head * (is_v ? v_head : per_head);
-    int d0 = in_head * VEC, d1 = -1, f0 = -1;  // first dim of the item, of its partner chunk, and the frequency of its first pair
-    if (!is_v) {
-      const int map = in_head / per_map, in_map = in_head - map * per_map;
-      if (a.adjacent) {
-        d0 = in_map * VEC;
-        f0 = d0 < 2 * half ? d0 / 2 : -1;
-      } else if (in_map < n_pair) {
-        d0 = f0 = in_map * VEC, d1 = d0 + half;
-      } else {
-        d0 = 2 * half + (in_map - n_pair) * VEC;
-      }
-      d0 += map * D;
-      if (d1 >= 0) d1 += map * D;
-    }
-    const void* src = is_q ? a.Q : (is_v ? a.V : a.K);
-    const int64_t at = int64_t(row) * (is_q ? a.q_src_ld : (is_v ? a.v_src_ld : a.k_src_ld)) + int64_t(head) * HD;
-
-    float x[VEC], y[VEC];
-    load(src, at + d0, x);
-    if (d1 >= 0) load(src, at + d1, y);
-    if (d1 >= 0) {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const float2 cs = tr[f0 + i];
-        const float u = x[i];
-        x[i] = u * cs.x - y[i] * cs.y;
-        y[i] = y[i] * cs.x + u * cs.y;
-      }
-    } else if (f0 >= 0) {
-      if constexpr (VEC == 8) {
-#pragma unroll
-        for (int i = 0; i < VEC; i += 2) {
-          const float2 cs = tr[f0 + i / 2];
-          const float u = x[i];
-          x[i] = u * cs.x - x[i + 1] * cs.y;
-          x[i + 1] = x[i + 1] * cs.x + u * cs.y;
-        }
-      }
-    }
-    uint32_t wx[VEC == 8 ? 4 : 1], wy[VEC == 8 ? 4 : 1];
-    if (is_q) {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) x[i] *= a.qscale;
-      round16(x, wx);
-      const size_t to = size_t(row) * p.q_ld + size_t(head) * HD;
-      store16(a.Qo, to + d0, wx);
-      if (d1 >= 0) {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) y[i] *= a.qscale;
-        round16(y, wy);
-        store16(a.Qo, to + d1, wy);
-      }
-      continue;
-    }
-    round16(x, wx);
-    if (d1 >= 0) round16(y, wy);
-    void* batch = is_v ? a.Vb : a.Kb;
-    if (batch) {
-      const size_t to = size_t(row) * p.kv_ld + size_t(head) * HD;
-      store16(batch, to + d0, wx);
-      if (d1 >= 0) store16(batch, to + d1, wy);
-    }
-    if (a.kv) {
-      const int2 slot = reinterpret_cast<const int2*>(a.slots)[row];
-      if (slot.x < 0) continue;
-      if (slot.x >= a.n_blocks || slot.y < 0 || slot.y >= p.bt) {  // the table lives on the device: no host check sees it
-        atomicExch(args.status, kStatusBadBlock);
-        continue;
-      }
-      const size_t blk = size_t(p.bt) * p.kv_ld;
-      const size_t to = p.kv_base + (size_t(slot.x) * 2 + (is_v ? 1 : 0)) * blk + size_t(slot.y) * p.kv_ld + size_t(head) * HD;
-      float scale = 1.0f;
-      if constexpr (FP8_POOL) scale = a.kv_scales[(size_t(slot.x) * 2 + (is_v ? 1 : 0)) * p.Hkv + head];
-      store_pool(to + d0, wx, scale);
-      if (d1 >= 0) store_pool(to + d1, wy, scale);
-    }
-  }
+__device__ __forceinline__ float2 turn_of(int pos, float inv_freq) {
+  const double turns = double(pos) * double(inv_freq) * 0.15915494309189533577;
+  float s, c;
+  sincospif(2.0f * float(turns - rint(turns)), &s, &c);
+  return make_float2(c, s);
 }
 
-// Adjacent pairs without 16-byte accesses: one item = one pair (or, past the rotating dims, two dims that pass through). The same
-// arithmetic; kept apart because its item holds two neighbouring dims.
+// Where a row's keys (which = 0) or values go in the pool; false: nowhere. The table lives on the device, no host check sees it.
+__device__ __forceinline__ bool pool_row(const AppendArgs& args, int row, int2& slot) {
+  const esp_kv_append_args& a = args.a;
+  slot = reinterpret_cast<const int2*>(a.slots)[row];
+  if (slot.x < 0) return false;
+  if (slot.x >= a.n_blocks || slot.y < 0 || slot.y >= a.p.bt) {
+    atomicExch(args.status, kStatusBadBlock);
+    return false;
+  }
+  return true;
+}
+__device__ __forceinline__ size_t pool_at(const esp_attn_params& p, const int2& slot, int which) {
+  return p.kv_base + (size_t(slot.x) * 2 + which) * (size_t(p.bt) * p.kv_ld) + size_t(slot.y) * p.kv_ld;
+}
+
+// How a row falls into steps of 32 lanes.
+struct Steps {
+  int32_t q, k, v;      // steps of the queries, keys and values
+  int32_t log_p2;       // lanes per map: 1 << log_p2
+  int32_t n_pair;       // chunk pairs of a map (0 for adjacent pairs, which lie within a chunk)
+  int32_t per_map;      // items of a map
+  int32_t per_part;     // steps a warp takes
+  int32_t parts;        // warps per row
+};
+
+template <bool SRC32>
+struct Raw {  // 8 dims as they were loaded
+  uint4 a;
+  uint4 b;
+};
+template <>
+struct Raw<false> {
+  uint4 a;
+};
+
+template <int QDT, bool SRC32, bool FP8_POOL, bool ADJ>
+__global__ void __launch_bounds__(kThreads, 3) kv_append_kernel(const AppendArgs args, const Steps st, const int HD) {
+  using QE = Elem16<QDT>;
+  using T = typename QE::T;
+  using S = std::conditional_t<SRC32, float, T>;
+  const esp_kv_append_args& a = args.a;
+  const esp_attn_params& p = a.p;
+  const int lane = threadIdx.x & 31;
+  const int64_t task = int64_t(blockIdx.x) * kWarps + (threadIdx.x >> 5);
+  const int row = int(task / st.parts), part = int(task - int64_t(row) * st.parts);
+  pdl_wait();  // the projection, and what a pass before this one may still read of the pool
+  pdl_launch_dependents();
+  if (row >= a.rows) return;
+  const int D = HD / a.maps, half = a.rot_half;
+  const int s0 = part * st.per_part, s1 = min(s0 + st.per_part, st.q + st.k + st.v);
+
+  // this lane's place within a map: its chunk, the distance to the chunk's partner (0: none), the frequency of its first pair
+  const int in_map = lane & ((1 << st.log_p2) - 1), maps_per_step = 32 >> st.log_p2, map_in_step = lane >> st.log_p2;
+  const bool in_use = in_map < st.per_map, paired = !ADJ && in_map < st.n_pair;
+  const int c0 = (paired || ADJ) ? in_map * 8 : 2 * half + (in_map - st.n_pair) * 8;
+  const bool turns = ADJ ? c0 < 2 * half : paired;
+  float2 cs[ADJ ? 4 : 8];
+  if (turns && s0 < st.q + st.k) {
+    const int pos = a.pos[row], f0 = ADJ ? c0 / 2 : c0;
+    float fr[ADJ ? 4 : 8];
+#pragma unroll
+    for (int i = 0; i < (ADJ ? 4 : 8); ++i) fr[i] = a.inv_freq[f0 + i];
+#pragma unroll
+    for (int i = 0; i < (ADJ ? 4 : 8); ++i) cs[i] = turn_of(pos, fr[i]);
+  }
+  int2 slot = make_int2(-1, 0);
+  const bool kept = a.kv && s1 > st.q && pool_row(args, row, slot);
+
+  auto load = [](const S* src) {
+    Raw<SRC32> w;
+    w.a = reinterpret_cast<const uint4*>(src)[0];
+    if constexpr (SRC32) w.b = reinterpret_cast<const uint4*>(src)[1];
+    return w;
+  };
+  auto values = [](const Raw<SRC32>& w, float (&x)[8]) {
+    const uint32_t u[4] = {w.a.x, w.a.y, w.a.z, w.a.w};
+    if constexpr (SRC32) {
+      const uint32_t v[4] = {w.b.x, w.b.y, w.b.z, w.b.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(u[i]), x[4 + i] = __uint_as_float(v[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = QE::unpack2(u[i]);
+        x[2 * i] = f.x, x[2 * i + 1] = f.y;
+      }
+    }
+  };
+  auto round16 = [](const float (&x)[8]) { return make_uint4(QE::pack2(x[0], x[1]), QE::pack2(x[2], x[3]), QE::pack2(x[4], x[5]), QE::pack2(x[6], x[7])); };
+  auto store_pool = [&](size_t at, const uint4& w, float scale) {
+    if constexpr (!FP8_POOL) {
+      *reinterpret_cast<uint4*>(static_cast<T*>(a.kv) + at) = w;
+    } else {
+      // division, as esp_kv_save does, so that both give the same codes
+      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+      uint32_t o[2] = {0, 0};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = QE::unpack2(u[i]);
+        const uint32_t two = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(f.x, scale), __fdiv_rn(f.y, scale)), __NV_SATFINITE, __NV_E4M3);
+        o[i >> 1] |= two << (16 * (i & 1));
+      }
+      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.kv) + at) = make_uint2(o[0], o[1]);
+    }
+  };
+
+  // One kind (0 queries, 1 keys, 2 values): steps [t0, t1) of its own; consecutive steps lie `stride` dims apart in source and outputs.
+  auto walk = [&](auto kind_c, int t0, int t1) {
+    constexpr int kind = decltype(kind_c)::value;
+    if (t0 >= t1) return;
+    const int stride = kind == 2 ? 256 : maps_per_step * D;                    // dims of a step
+    const int first = kind == 2 ? lane * 8 : map_in_step * D + c0;              // this lane's dims in step 0
+    const int width = (kind == 0 ? p.H : p.Hkv) * HD;                           // dims of the row
+    const bool mine = kind == 2 || in_use;
+    const S* src = static_cast<const S*>(kind == 0 ? a.Q : (kind == 1 ? a.K : a.V)) + int64_t(row) * (kind == 0 ? a.q_src_ld : (kind == 1 ? a.k_src_ld : a.v_src_ld));
+    T* out = kind == 0 ? static_cast<T*>(a.Qo) + size_t(row) * p.q_ld : static_cast<T*>(kind == 1 ? a.Kb : a.Vb);
+    if (kind != 0 && out) out += size_t(row) * p.kv_ld;
+    const size_t pool = kind != 0 && kept ? pool_at(p, slot, kind == 2) : 0;
+#pragma unroll 1
+    for (int t = t0; t < t1; t += kBatch) {
+      Raw<SRC32> rx[kBatch], ry[kBatch];
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const int at = first + (t + u) * stride;
+        if (mine && t + u < t1 && at < width) {
+          rx[u] = load(src + at);
+          if (!ADJ && kind != 2 && paired) ry[u] = load(src + at + half);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const int at = first + (t + u) * stride;
+        if (!(mine && t + u < t1 && at < width)) continue;
+        float v0[8], v1[8] = {};
+        values(rx[u], v0);
+        if (!ADJ && kind != 2 && paired) {
+          values(ry[u], v1);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float2 c = cs[ADJ ? 0 : i];
+            const float e = v0[i];
+            v0[i] = e * c.x - v1[i] * c.y;
+            v1[i] = v1[i] * c.x + e * c.y;
+          }
+        } else if (ADJ && kind != 2 && turns) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float e = v0[2 * i];
+            v0[2 * i] = e * cs[i].x - v0[2 * i + 1] * cs[i].y;
+            v0[2 * i + 1] = v0[2 * i + 1] * cs[i].x + e * cs[i].y;
+          }
+        }
+        if (kind == 0) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v0[i] *= a.qscale, v1[i] *= a.qscale;
+        }
+        const uint4 w0 = round16(v0), w1 = round16(v1);
+        const bool two = !ADJ && kind != 2 && paired;
+        if (kind == 0 || out) {
+          *reinterpret_cast<uint4*>(out + at) = w0;
+          if (two) *reinterpret_cast<uint4*>(out + at + half) = w1;
+        }
+        if (kind != 0 && kept) {
+          float scale = 1.0f;
+          if constexpr (FP8_POOL) scale = a.kv_scales[(size_t(slot.x) * 2 + size_t(kind == 2)) * p.Hkv + at / HD];
+          store_pool(pool + at, w0, scale);
+          if (two) store_pool(pool + at + half, w1, scale);
+        }
+      }
+    }
+  };
+  walk(std::integral_constant<int, 0>{}, min(s0, st.q), min(s1, st.q));
+  walk(std::integral_constant<int, 1>{}, max(s0 - st.q, 0), min(s1 - st.q, st.k));
+  walk(std::integral_constant<int, 2>{}, max(s0 - st.q - st.k, 0), s1 - st.q - st.k);
+}
+
+// Rows whose addresses, strides or rotary widths do not allow 16-byte accesses, and maps of more than 256 dims: the same arithmetic, an item is
+// two dims - a rotating pair, or past the rotating dims two neighbours.
 template <int QDT, bool SRC32, bool FP8_POOL>
-__global__ void __launch_bounds__(kThreads) kv_append_adjacent_kernel(const AppendArgs args, const int HD) {
+__global__ void __launch_bounds__(kThreads) kv_append_narrow_kernel(const AppendArgs args, const int HD) {
   using QE = Elem16<QDT>;
   using T = typename QE::T;
   const esp_kv_append_args& a = args.a;
@@ -205,57 +224,48 @@ __global__ void __launch_bounds__(kThreads) kv_append_adjacent_kernel(const Appe
   extern __shared__ float2 turn[];
   const int D = HD / a.maps, half = a.rot_half, row = blockIdx.x;
   pdl_wait();
-  for (int f = threadIdx.x; f < half; f += kThreads) {
-    const double turns = double(a.pos[row]) * double(a.inv_freq[f]) * 0.15915494309189533577;
-    float s, c;
-    sincospif(2.0f * float(turns - rint(turns)), &s, &c);
-    turn[f] = make_float2(c, s);
-  }
+  for (int f = threadIdx.x; f < half; f += kThreads) turn[f] = turn_of(a.pos[row], a.inv_freq[f]);
   __syncthreads();
   pdl_launch_dependents();
+  int2 slot = make_int2(-1, 0);
+  const bool kept = a.kv && pool_row(args, row, slot);
   const int n_q = a.Q ? p.H * HD / 2 : 0, n_k = p.Hkv * HD / 2;
   for (int item = blockIdx.y * kThreads + threadIdx.x; item < n_q + 2 * n_k; item += kThreads * gridDim.y) {
     const bool is_q = item < n_q, is_v = item >= n_q + n_k;
     const int rel = is_q ? item : (is_v ? item - n_q - n_k : item - n_q);
-    const int head = rel / (HD / 2), d = 2 * (rel - head * (HD / 2));
+    const int head = rel / (HD / 2), in_head = rel - head * (HD / 2), map = in_head / (D / 2), i = in_head - map * (D / 2);
+    const bool turns = !is_v && i < half;
+    const int d0 = map * D + (turns && !a.adjacent ? i : 2 * i), d1 = d0 + (turns && !a.adjacent ? half : 1);
     const void* src = is_q ? a.Q : (is_v ? a.V : a.K);
-    const int64_t at = int64_t(row) * (is_q ? a.q_src_ld : (is_v ? a.v_src_ld : a.k_src_ld)) + int64_t(head) * HD + d;
+    const int64_t at = int64_t(row) * (is_q ? a.q_src_ld : (is_v ? a.v_src_ld : a.k_src_ld)) + int64_t(head) * HD;
     float x, y;
-    if constexpr (SRC32) x = static_cast<const float*>(src)[at], y = static_cast<const float*>(src)[at + 1];
-    else x = QE::to_f32(static_cast<const T*>(src)[at]), y = QE::to_f32(static_cast<const T*>(src)[at + 1]);
-    const int f = (d % D) / 2;
-    if (!is_v && f < half) {
-      const float2 cs = turn[f];
-      const float u = x;
-      x = u * cs.x - y * cs.y;
-      y = y * cs.x + u * cs.y;
+    if constexpr (SRC32) x = static_cast<const float*>(src)[at + d0], y = static_cast<const float*>(src)[at + d1];
+    else x = QE::to_f32(static_cast<const T*>(src)[at + d0]), y = QE::to_f32(static_cast<const T*>(src)[at + d1]);
+    if (turns) {
+      const float2 cs = turn[i];
+      const float e = x;
+      x = e * cs.x - y * cs.y;
+      y = y * cs.x + e * cs.y;
     }
     if (is_q) {
-      T* dst = static_cast<T*>(a.Qo) + size_t(row) * p.q_ld + size_t(head) * HD + d;
-      dst[0] = QE::from_f32(x * a.qscale), dst[1] = QE::from_f32(y * a.qscale);
+      T* dst = static_cast<T*>(a.Qo) + size_t(row) * p.q_ld + size_t(head) * HD;
+      dst[d0] = QE::from_f32(x * a.qscale), dst[d1] = QE::from_f32(y * a.qscale);
       continue;
     }
     const T rx = QE::from_f32(x), ry = QE::from_f32(y);
     if (void* batch = is_v ? a.Vb : a.Kb) {
-      T* dst = static_cast<T*>(batch) + size_t(row) * p.kv_ld + size_t(head) * HD + d;
-      dst[0] = rx, dst[1] = ry;
+      T* dst = static_cast<T*>(batch) + size_t(row) * p.kv_ld + size_t(head) * HD;
+      dst[d0] = rx, dst[d1] = ry;
     }
-    if (!a.kv) continue;
-    const int2 slot = reinterpret_cast<const int2*>(a.slots)[row];
-    if (slot.x < 0) continue;
-    if (slot.x >= a.n_blocks || slot.y < 0 || slot.y >= p.bt) {
-      atomicExch(args.status, kStatusBadBlock);
-      continue;
-    }
-    const size_t blk = size_t(p.bt) * p.kv_ld;
-    const size_t to = p.kv_base + (size_t(slot.x) * 2 + (is_v ? 1 : 0)) * blk + size_t(slot.y) * p.kv_ld + size_t(head) * HD + d;
+    if (!kept) continue;
+    const size_t to = pool_at(p, slot, is_v) + size_t(head) * HD;
     if constexpr (FP8_POOL) {
-      const float scale = a.kv_scales[(size_t(slot.x) * 2 + (is_v ? 1 : 0)) * p.Hkv + head];
+      const float scale = a.kv_scales[(size_t(slot.x) * 2 + is_v) * p.Hkv + head];
       uint8_t* dst = static_cast<uint8_t*>(a.kv) + to;
-      dst[0] = f32_to_e4m3(__fdiv_rn(QE::to_f32(rx), scale)), dst[1] = f32_to_e4m3(__fdiv_rn(QE::to_f32(ry), scale));
+      dst[d0] = f32_to_e4m3(__fdiv_rn(QE::to_f32(rx), scale)), dst[d1] = f32_to_e4m3(__fdiv_rn(QE::to_f32(ry), scale));
     } else {
       T* dst = static_cast<T*>(a.kv) + to;
-      dst[0] = rx, dst[1] = ry;
+      dst[d0] = rx, dst[d1] = ry;
     }
   }
 }
@@ -265,21 +275,30 @@ cudaError_t launch_typed(const AppendArgs& args, int32_t HD, cudaStream_t stream
   const esp_kv_append_args& a = args.a;
   const size_t ssz = SRC32 ? 4 : 2;
   auto ok16 = [](const void* q, int64_t row_bytes) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0 && row_bytes % 16 == 0; };
-  const bool wide = (a.adjacent ? a.rot_half % 4 : a.rot_half % 8) == 0 && ok16(a.Q, a.q_src_ld * int64_t(ssz)) && ok16(a.K, a.k_src_ld * int64_t(ssz)) &&
-                    ok16(a.V, a.v_src_ld * int64_t(ssz)) && ok16(a.Qo, 0) && ok16(a.Kb, 0) && ok16(a.Vb, 0) && ok16(a.kv, 0);
-  const int vec = wide ? 8 : 1;
-  const int heads = (a.Q ? a.p.H : 0) + 2 * a.p.Hkv;
-  const int per_row = heads * HD / vec;  // items of a row, at most
-  // A row with fewer chunks than a CTA has threads shares its CTA with others; a batch with fewer rows than SMs spreads each row
-  // over several CTAs.
-  const int rpc = wide ? int(std::max<int64_t>(1, std::min<int64_t>(2 * kThreads / per_row, a.rows / 148))) : 1;
-  const unsigned gx = unsigned((a.rows + rpc - 1) / rpc);
-  const int most_y = (rpc * per_row + kThreads - 1) / kThreads;
-  const unsigned gy = unsigned(std::max(1, std::min(most_y, int(4 * 148 / gx))));
-  const size_t smem = size_t(rpc) * a.rot_half * sizeof(float2);
-  if (wide) return launch_pdl(kv_append_kernel<QDT, SRC32, FP8_POOL, 8>, dim3(gx, gy), dim3(kThreads), smem, stream, args, HD, rpc);
-  if (a.adjacent) return launch_pdl(kv_append_adjacent_kernel<QDT, SRC32, FP8_POOL>, dim3(gx, gy), dim3(kThreads), smem, stream, args, HD);
-  return launch_pdl(kv_append_kernel<QDT, SRC32, FP8_POOL, 1>, dim3(gx, gy), dim3(kThreads), smem, stream, args, HD, rpc);
+  const int D = HD / a.maps, n_pair = a.adjacent ? 0 : a.rot_half / 8, per_map = a.adjacent ? D / 8 : n_pair + (D - 2 * a.rot_half) / 8;
+  const bool wide = (a.adjacent ? a.rot_half % 4 : a.rot_half % 8) == 0 && per_map <= 32 && ok16(a.Q, a.q_src_ld * int64_t(ssz)) &&
+                    ok16(a.K, a.k_src_ld * int64_t(ssz)) && ok16(a.V, a.v_src_ld * int64_t(ssz)) && ok16(a.Qo, 0) && ok16(a.Kb, 0) && ok16(a.Vb, 0) && ok16(a.kv, 0);
+  if (!wide) {
+    const int items = ((a.Q ? a.p.H : 0) + 2 * a.p.Hkv) * HD / 2;
+    const unsigned gy = unsigned(std::clamp(4 * 148 / a.rows, 1, (items + kThreads - 1) / kThreads));
+    return launch_pdl(kv_append_narrow_kernel<QDT, SRC32, FP8_POOL>, dim3(unsigned(a.rows), gy), dim3(kThreads), size_t(a.rot_half) * sizeof(float2), stream, args, HD);
+  }
+  Steps st{};
+  while ((1 << st.log_p2) < per_map) ++st.log_p2;
+  const int maps_per_step = 32 >> st.log_p2;
+  st.q = a.Q ? (a.p.H * a.maps + maps_per_step - 1) / maps_per_step : 0;
+  st.k = (a.p.Hkv * a.maps + maps_per_step - 1) / maps_per_step;
+  st.v = (a.p.Hkv * HD / 8 + 31) / 32;
+  st.n_pair = n_pair, st.per_map = per_map;
+  // Rows that do not fill the SMs' warps (about 16 an SM) are cut into parts of at least one batch, single tokens down to one step.
+  const int steps = st.q + st.k + st.v;
+  const int64_t want = 148 * 16;
+  const int least = a.rows * int64_t(steps) <= want ? 1 : kBatch;
+  st.parts = int(std::clamp<int64_t>((want + a.rows - 1) / a.rows, 1, (steps + least - 1) / least));
+  st.per_part = (steps + st.parts - 1) / st.parts;
+  st.parts = (steps + st.per_part - 1) / st.per_part;
+  const int64_t tasks = int64_t(a.rows) * st.parts;
+  return launch_pdl(a.adjacent ? kv_append_kernel<QDT, SRC32, FP8_POOL, true> : kv_append_kernel<QDT, SRC32, FP8_POOL, false>, dim3(unsigned((tasks + kWarps - 1) / kWarps)), dim3(kThreads), 0, stream, args, st, HD);
 }
 
 }  // namespace

@@ -216,7 +216,7 @@ struct DiffArgs {
 };
 struct DiffCombineArgs {
   DiffArgs d;
-  int32_t n_jobs, rows_max;
+  int32_t n_jobs, rows_max, parts_max;  // most rows, most records of any job
 };
 cudaError_t launch_diff_general(const DiffArgs& a, cudaStream_t stream, uint64_t* launches);
 // Single-row trees; pool_map is the map of the plain decode kernel.

@@ -15,7 +15,7 @@ import numpy as np
 import torch
 
 from . import capi
-from .workloads import COMBINE_DT, E4M3, KVSAVE_DT, TILE_DT, TREE_DT, Workload
+from .workloads import COMBINE_DT, E4M3, F16, KVSAVE_DT, TILE_DT, TREE_DT, Workload
 
 
 @dataclass
@@ -68,10 +68,10 @@ def make_trees(rows, cached, tables) -> np.ndarray:
     return trees
 
 
-def diff_plan_options(trees: np.ndarray, H: int, Hkv: int, HD: int):
+def diff_plan_options(trees: np.ndarray, H: int, Hkv: int, HD: int, kv_dtype: int = F16):
     """esp_diff_plan_opts: (tile_rows for the context, keyword arguments for plan_tiles)."""
     o = capi.PlanOpts()
-    shape = capi.Shape(H, Hkv, HD)
+    shape = capi.Shape(H, Hkv, HD, kv_dtype=kv_dtype)
     trees = np.ascontiguousarray(trees, dtype=TREE_DT)
     capi.check(capi.load().esp_diff_plan_opts(C.byref(shape), trees.ctypes.data_as(C.POINTER(capi.Tree)), len(trees), C.byref(o)))
     return o.tile_rows, dict(mode=o.mode, split=o.split, min_chunk=o.min_chunk, groups=o.groups, tile_rows=o.tile_rows, max_parts=o.max_parts)
@@ -310,10 +310,15 @@ class AttnOp:
         a.p = capi.Params(s.H, s.Hkv, s.H * s.HD if Qo is None else Qo.stride(0), s.Hkv * s.HD, 2 * s.H * s.HD, s.bt, kv_base)
         return Call(a, None, (Q, K, V, Qo, Kb, Vb, kv, kv_scales, slots, pos, inv_freq))
 
+    def _stream(self, stream: int | None) -> int:
+        """The given cudaStream_t, or torch's current one (without the Stream object, which costs as much as the call)."""
+        return torch._C._cuda_getCurrentRawStream(self.device.index) if stream is None else stream
+
     def kv_append(self, call: Call, stream: int | None = None):
         """esp_kv_append on torch's current stream (or the given cudaStream_t)."""
-        s = torch.cuda.current_stream(self.device).cuda_stream if stream is None else stream
-        capi.check(self.lib.esp_kv_append(self.ctx, C.c_void_p(s), C.byref(call.args)))
+        rc = self.lib.esp_kv_append(self.ctx, self._stream(stream), call.args)
+        if rc:
+            capi.check(rc)
 
     def diff_call(self, plan: Plan, trees: np.ndarray, Q, Kb, Vb, O, kv=None, kv_scales=None, blocks=None, n_blocks=0, desc=None,
                   anc_mask=None, lam=None, lam_ld=0, norm_w=None, eps=0.0, out_scale=1.0, kv_base=0, parts=None, scratch=None) -> Call:
@@ -342,8 +347,9 @@ class AttnOp:
 
     def diff_forward(self, call: Call, stream: int | None = None):
         """esp_diff_forward on torch's current stream (or the given cudaStream_t)."""
-        s = torch.cuda.current_stream(self.device).cuda_stream if stream is None else stream
-        capi.check(self.lib.esp_diff_forward(self.ctx, C.c_void_p(s), C.byref(call.args), C.byref(call.more)))
+        rc = self.lib.esp_diff_forward(self.ctx, self._stream(stream), call.args, call.more)
+        if rc:
+            capi.check(rc)
 
     def diff_lambda(self, q1, k1, q2, k2, lambda_init: float, H: int | None = None, stream: int | None = None):
         """esp_diff_lambda: [H, dim] vectors, or one [dim] vector for every head."""

@@ -523,8 +523,8 @@ typedef struct esp_diff_args {
 int esp_diff_forward(esp_attn_ctx* ctx, void* stream, const esp_attn_args* args, const esp_diff_args* diff);
 /* Floats of `parts` for n_parts records. */
 size_t esp_diff_parts_floats(const esp_attn_shape* shape, int32_t n_parts);
-/* Planner options for a pass (pure host): opts->tile_rows is also the tile_rows its context wants. Reads H, Hkv and HD of the
- * shape. */
+/* Planner options for a pass (pure host): opts->tile_rows is also the tile_rows its context wants. Reads H, Hkv, HD and
+ * kv_dtype of the shape. */
 int esp_diff_plan_opts(const esp_attn_shape* shape, const esp_attn_tree* trees_host, int32_t n_trees, esp_plan_opts* opts);
 /* lam[h] = exp(q1_h . k1_h) - exp(q2_h . k2_h) + lambda_init for h < H, from the layer's learned vectors ([H][dim] fp32, rows
  * ld elements apart; ld = 0: one vector for every head). Once per model load. One launch. */

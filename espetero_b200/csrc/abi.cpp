@@ -1304,6 +1304,12 @@ int esp_diff_forward(esp_attn_ctx* c, void* stream, const esp_attn_args* ap, con
   if (decode) {
     if (int rc = pool_tensor_map(c, a)) return rc;
     c->last_kernel = "diff_decode";
+    // Jobs of few records are joined by the CTA that finishes last (option "fuse_combine": 0 never, 2 always); long ones take the
+    // join kernel's parallelism.
+    int most = 0;
+    for (int i = 0; a.jobs_host && i < a.n_jobs; ++i) most = std::max(most, a.jobs_host[i].nparts);
+    k.fuse = c->opt_fuse_combine && a.n_jobs > 0 && a.jobs && (c->opt_fuse_combine == 2 || most <= 16) &&
+             esp::plan_fusable(a.tiles_host, a.n_tiles, a.jobs_host, a.n_jobs, s.Hkv);
     ProfScope prof(c, st, c->last_kernel);
     e = esp::launch_diff_decode(d, c->pool_map, st, &c->launches);
   } else if (umma) {
@@ -1332,7 +1338,7 @@ int esp_diff_forward(esp_attn_ctx* c, void* stream, const esp_attn_args* ap, con
     e = esp::launch_diff_general(d, st, &c->launches);
   }
   if (e != cudaSuccess) return cuda_fail(e, c->last_kernel);
-  if (a.n_jobs > 0) {
+  if (a.n_jobs > 0 && !k.fuse) {
     esp::DiffCombineArgs m{d, a.n_jobs, c->tile_rows, 64};
     if (a.jobs_host) {
       m.rows_max = m.parts_max = 1;

@@ -95,7 +95,10 @@ LENGTHS = [0, 1, 15, 16, 17, 31, 64, 65, 333, 1024]
 @pytest.mark.parametrize("split", [0, 32], ids=["whole", "split"])
 def test_decode(HD, heads, types, split):
     w = wl.make_pass("decode", HD + heads[0], [(n, 1) for n in LENGTHS], heads[0], heads[1], HD, 48 if split else 16, types[0], types[1], scale=(HD // 2) ** -0.5)
-    _check(w, "diff_decode", plan_opts=dict(split=split, groups=4096 if split else 1))
+    O, _ = _check(w, "diff_decode", plan_opts=dict(split=split, groups=4096 if split else 1))
+    if split:  # joined in the kernel (jobs of 32 records, too), or by the join kernel
+        for fuse in (0, 2):
+            _check(w, "diff_decode", plan_opts=dict(split=split, groups=4096), options=dict(fuse_combine=fuse))
 
 
 @gpu
@@ -331,6 +334,41 @@ def test_a_serving_loop(pool):
     assert (np.abs(last.cpu().numpy().astype(np.float64) - O64[-1:]) <= tol[-1:]).all()
     for k in keep:
         k[0].close()
+
+
+@gpu
+@pytest.mark.parametrize("HD", [128, 256])
+def test_counters_are_ready_for_the_next_pass(HD):
+    """Passes joined in the kernel, one after another on one context and in a replayed graph, all give the first one's bits."""
+    w = wl.make_pass("again", 9, [(1000, 1), (130, 1), (700, 1)], 8, 2, HD, 16, wl.BF16, scale=0.125)
+    lam, nw = _weights(w, 4)
+    op = host.AttnOp.for_workload(w, 8)
+    dp = op.upload(w)
+    plan = host.plan_tiles(w.trees, w.Hkv, **dict(host.diff_plan_options(w.trees, w.H, w.Hkv, HD)[1], groups=40))
+    assert 1 < max(plan.jobs["nparts"]) <= 16
+    O = torch.zeros((w.n_rows, w.q_ld), dtype=torch.int16, device=op.device)
+    call = op.diff_call(plan, w.trees, dp.Q, dp.Kb, dp.Vb, O, kv=dp.kv, blocks=dp.blocks, n_blocks=w.n_blocks, desc=dp.desc, lam=torch.from_numpy(lam).cuda(),
+                        norm_w=torch.from_numpy(nw).cuda(), eps=EPS, out_scale=SCALE)
+    before = op.launch_count
+    op.diff_forward(call)
+    torch.cuda.synchronize()
+    assert op.launch_count == before + 1
+    want = O.clone()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        op.diff_forward(call)
+    for _ in range(5):
+        O.zero_()
+        call.keep[5].fill_(float("nan"))
+        op.diff_forward(call)
+        torch.cuda.synchronize()
+        assert torch.equal(O, want)
+        O.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(O, want)
+    op.check_status()
+    op.close()
 
 
 @gpu

@@ -46,6 +46,7 @@ struct Geo {
   static constexpr int SMEM = TILES + 1024;
   static constexpr int BU = HD == 256 ? 128 : 64;  // keys per unit
   static constexpr int UPB = BN / BU;              // units per block
+  static constexpr int PART = BU / 2;              // keys whose weights are handed over together
   static constexpr uint32_t COL_O = 0, COL_S = HD; // S buffer i at COL_S + BU i (P over its first BU / 2 columns)
   static constexpr uint32_t COLS = HD + 2 * BU;    // 512 or 256
   static constexpr int CTAS = HD == 256 ? 1 : 2;   // per SM
@@ -230,12 +231,12 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
             if (n >= N) break;
             const uint32_t v_lo = v_lo0 + uint32_t(vst) * (C::V_TILE >> 4) + uint32_t((h * C::BU * 128) >> 4);
 #pragma unroll
-            for (int part = 0; part < C::BU / 64; ++part) {  // P comes in parts of 64 keys
+            for (int part = 0; part < 2; ++part) {
               wait_bar(&sh.p_full[i][part], uint32_t(n >> 1) & 1u, kStatusMmaTimeout);
               if (part == 0 && h == 0) wait_bar(&sh.v_full[vst], vpar, kStatusTmaTimeout);
               tc_fence_after_sync();
 #pragma unroll
-              for (int ks = 4 * part; ks < 4 * part + 4; ++ks)
+              for (int ks = part * (C::PART / 16); ks < (part + 1) * (C::PART / 16); ++ks)
                 mma_ts(one, tmem + C::COL_O, tmem + C::COL_S + i * C::BU + ks * 8, v_lo + ((ks * 16 * 128) >> 4), hi_v, idesc_pv, ks > 0 ? 1u : uint32_t(n > 0));
             }
             mma_commit(one, &sh.o_done[i]);
@@ -285,17 +286,24 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
       const int b = n / C::UPB, c0 = (n % C::UPB) * C::BU;
       const uint32_t par = uint32_t(n >> 1) & 1u;
       const bool whole = L.whole(b);
-      if constexpr (F8) wait_bar(&sh.sc_full[b % kSlots], uint32_t(b / kSlots) & 1u, kStatusTmaTimeout);
-      wait_bar(&sh.s_full[wg], par, kStatusMmaTimeout);
-      tc_fence_after_sync();
+      // the reference, from the partner warp that had the unit before: its maximum has long been known when these scores arrive
+      float m_old = -INFINITY, v_ref = 0.0f;
+      if (n > 0) {
+        wait_bar(&sh.m_ready[wg ^ 1][wq], uint32_t((n - 1) >> 1) & 1u, kStatusMmaTimeout);
+        m_old = *const_cast<volatile float*>(&sh.m_ref[srow]);
+        if constexpr (F8) v_ref = *const_cast<volatile float*>(&sh.v_ref[wq]);
+      }
       float ks[2 * NS], vs[2 * NS], largest = 0.0f;
       if constexpr (F8) {
+        wait_bar(&sh.sc_full[b % kSlots], uint32_t(b / kSlots) & 1u, kStatusTmaTimeout);
 #pragma unroll
         for (int i = 0; i < 2 * NS; ++i) {
           ks[i] = sh.k_scale[b % kSlots][c0 / 16 + i], vs[i] = sh.v_scale[b % kSlots][c0 / 16 + i];
           largest = fmaxf(largest, vs[i]);
         }
       }
+      wait_bar(&sh.s_full[wg], par, kStatusMmaTimeout);
+      tc_fence_after_sync();
       // 32 scores as they count: times their pages' K scales, hidden where the row does not see the key
       auto shape = [&](uint32_t (&x)[32], int i) {
         if constexpr (F8) {
@@ -339,13 +347,6 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
           fence_proxy_async_smem();
         }
       }
-      // the reference, from the partner warp that had the unit before
-      float m_old = -INFINITY, v_ref = 0.0f;
-      if (n > 0) {
-        wait_bar(&sh.m_ready[wg ^ 1][wq], uint32_t((n - 1) >> 1) & 1u, kStatusMmaTimeout);
-        m_old = *const_cast<volatile float*>(&sh.m_ref[srow]);
-        if constexpr (F8) v_ref = *const_cast<volatile float*>(&sh.v_ref[wq]);
-      }
       const bool grow = mx > m_old + kGrow;  // also the first finite maximum
       const float m_new = grow ? mx : m_old;
       float vfac = 1.0f;
@@ -388,10 +389,10 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
         uint32_t pk[16];
         chunk_weights<QDT, F8>(s[C::HOLD ? i : 0], pk, sl2x2, neg_m2, sum, F8 ? vs[2 * i] * vinv : 1.0f, F8 ? vs[2 * i + 1] * vinv : 1.0f);
         tmem_st16(buf + 16 * i, pk);
-        if (i & 1) {  // 64 keys are ready: their P . V starts under the rest
+        if ((i + 1) % (C::PART / 32) == 0) {  // a part is ready: its P . V starts under the rest
           tmem_wait_st();
           tc_fence_before_sync();
-          mbar_arrive(&sh.p_full[wg][i >> 1]);
+          mbar_arrive(&sh.p_full[wg][i / (C::PART / 32)]);
         }
       }
       float a0, a1;

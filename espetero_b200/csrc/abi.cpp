@@ -49,11 +49,12 @@ struct esp_attn_ctx {
   const void* umap_kb = nullptr;
   const void* umap_vb = nullptr;
   uint64_t umap_base = 0;
-  // differential attention reads Kb / Vb 128 rows at a time
-  CUtensorMap dkb_map{}, dvb_map{};
+  // differential attention reads Q, Kb and Vb 128 or 64 rows at a time
+  CUtensorMap dq_map{}, dkb_map{}, dvb_map{};
+  const void* dmap_q = nullptr;
   const void* dmap_kb = nullptr;
   const void* dmap_vb = nullptr;
-  int32_t dmap_rows = 0, dmap_ld = 0;
+  int32_t dmap_rows = 0, dmap_ld = 0, dmap_qld = 0;
   int32_t umap_blocks = 0, umap_rows = 0, umap_ld = 0;
   // Re-planning of reference-shaped multi-row passes (8-row tiles) for the tensor-core kernels: the new
   // tiles and jobs are built on the host and travel through a small ring of pinned staging slots into
@@ -1323,15 +1324,16 @@ int esp_diff_forward(esp_attn_ctx* c, void* stream, const esp_attn_args* ap, con
       w.kv = nullptr;
     }
     if (int rc = umma_tensor_maps(c, w)) return rc;
-    if (c->dmap_kb != a.Kb || c->dmap_vb != a.Vb || c->dmap_rows != a.n_rows || c->dmap_ld != a.p.kv_ld) {
-      c->dmap_kb = c->dmap_vb = nullptr;
+    if (c->dmap_q != a.Q || c->dmap_kb != a.Kb || c->dmap_vb != a.Vb || c->dmap_rows != a.n_rows || c->dmap_ld != a.p.kv_ld || c->dmap_qld != a.p.q_ld) {
+      c->dmap_kb = nullptr;
+      if (int rc = rows_tensor_map(c, &c->dq_map, a.Q, uint64_t(a.n_rows), a.p.q_ld, 128)) return rc;
       if (int rc = rows_tensor_map(c, &c->dkb_map, a.Kb, uint64_t(a.n_rows), a.p.kv_ld, 128)) return rc;
-      if (int rc = rows_tensor_map(c, &c->dvb_map, a.Vb, uint64_t(a.n_rows), a.p.kv_ld, 128)) return rc;
-      c->dmap_kb = a.Kb, c->dmap_vb = a.Vb, c->dmap_rows = a.n_rows, c->dmap_ld = a.p.kv_ld;
+      if (int rc = rows_tensor_map(c, &c->dvb_map, a.Vb, uint64_t(a.n_rows), a.p.kv_ld, s.HD == 256 ? 64 : 128)) return rc;
+      c->dmap_q = a.Q, c->dmap_kb = a.Kb, c->dmap_vb = a.Vb, c->dmap_rows = a.n_rows, c->dmap_ld = a.p.kv_ld, c->dmap_qld = a.p.q_ld;
     }
     c->last_kernel = "diff_umma";
     ProfScope prof(c, st, c->last_kernel);
-    e = esp::launch_diff_umma(d, widen, c->upool_map, c->dkb_map, c->dvb_map, st, &c->launches);
+    e = esp::launch_diff_umma(d, widen, c->upool_map, c->dq_map, c->dkb_map, c->dvb_map, st, &c->launches);
   } else {
     c->last_kernel = "diff_general";
     ProfScope prof(c, st, c->last_kernel);

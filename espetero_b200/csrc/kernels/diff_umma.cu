@@ -20,7 +20,7 @@
 // Bound per 128 keys of a tile: 256-dim heads 1536 clocks of MMA per map (8 instructions of N = 128 and 8 of N = 256, 64 and 128
 // clocks each) on an SM, 1024 of exponentials; 128-dim heads 1024 of exponentials per map, two maps per SM, against 1600 of MMA.
 // Warps 0-7 softmax, 8 MMA issue (owns tensor memory), 9 / 10 K / V producers (TMA, one load per 16-key page and 64-dim chunk of the pool,
-// one per 128 rows of the batch), 11 idle (it
+// one per 64 or 128 rows of the batch; the Q tile, too, where it is 128 rows of one head), 11 idle (it
 // completes the warpgroup that hands registers over). Hand-offs by mbarrier; every wait is bounded: after a timeout the CTA records a
 // code, stops waiting, finishes its loop, frees its tensor memory and returns.
 // E4M3 pools (F8): the pages are 16-bit codes (diff_widen.cu); the K producer leaves each block's page scales in shared memory, the
@@ -34,18 +34,23 @@ using namespace difft;
 
 constexpr float kGrow = 8.0f;  // log2 units a row's maximum may grow before O is rescaled
 constexpr int kSoftmax = 256, kMmaWarp = 8, kWarpK = 9, kWarpV = 10, kThreads = 384;
-constexpr int KS = 2, VS = 2;  // ring depths, in tiles of 128 keys
+constexpr int KS = 2;          // K ring, in tiles of 128 keys
 
 template <int HD_>
 struct Geo {
   static constexpr int HD = HD_, MAP = HD / 2;
   static constexpr int CHUNK = 128 * 128;          // bytes of a 64-dim chunk of a tile: [128 rows][128 B]
   static constexpr int QC = MAP / 64, VC = HD / 64;  // chunks of a Q or K tile (one map), of a V tile
-  static constexpr int K_TILE = QC * CHUNK, V_TILE = VC * CHUNK;
-  static constexpr int TILES = (1 + KS) * K_TILE + VS * V_TILE;
-  static constexpr int SMEM = TILES + 1024;
+  // V ring, two blocks deep. 256-dim heads: slots of 64 keys, refilled while the other half of their block is still read (8192 causal
+  // rows, H16: 677 -> 652 us); 128-dim heads: whole blocks (halves cost the producers more than they gave: 700 rows behind 20001
+  // E4M3 keys 592 us against 647).
+  static constexpr int VK = HD == 256 ? 64 : 128, SPB = BN / VK, VS = 2 * SPB;
+  static constexpr int V_CHUNK = VK * 128;         // bytes of a 64-dim chunk of a V slot: [VK rows][128 B]
+  static constexpr int K_TILE = QC * CHUNK, V_SLOT = VC * V_CHUNK;
+  static constexpr int TILES = (1 + KS) * K_TILE + VS * V_SLOT;
   static constexpr int BU = HD == 256 ? 128 : 64;  // keys per unit
   static constexpr int UPB = BN / BU;              // units per block
+  static constexpr int SMEM = TILES + (HD == 256 ? 2048 : 1024);  // two CTAs of 113 KB (and the 1 KB each that is taken for them) fill an SM
   static constexpr int PART = BU / 2;              // keys whose weights are handed over together
   static constexpr uint32_t COL_O = 0, COL_S = HD; // S buffer i at COL_S + BU i (P over its first BU / 2 columns)
   static constexpr uint32_t COLS = HD + 2 * BU;    // 512 or 256
@@ -57,18 +62,19 @@ struct Geo {
 };
 
 constexpr int kRegsAux = 96, kRegsSoftmax = 200;  // 256-dim heads
-constexpr int kSlots = 4;  // blocks whose page scales are kept
+// Blocks whose page scales are kept. The producer writes those of block b + 4 once
+// K tile b + 2 is released, that is once its last unit's Q . K^T is through, which is issued behind the P . V of two units before: of a
+// unit of block b + 1, or with one unit per block of block b. The readers of block b are then done.
+constexpr int kSlots = 4;
+static_assert(kSlots >= KS + 2, "page scales must outlive their readers");
+template <int VS>
 struct Shared {
-  uint64_t k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], s_full[2], p_full[2][2], o_done[2], sc_full[kSlots], m_ready[2][4];
+  uint64_t q_full, k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], s_full[2], p_full[2][2], o_done[2], sc_full[kSlots], m_ready[2];
   uint32_t tmem;
   volatile int dead;
   float k_scale[kSlots][kPages], v_scale[kSlots][kPages];
   float m_ref[BM], v_ref[4];
 };
-static_assert(sizeof(Shared) <= 1024, "bookkeeping behind the tiles");
-// K tile b is released once its Q . K^T is through, which is issued behind P . V of two units before its last: the softmax is at most one
-// block behind then, and the producer KS blocks ahead.
-static_assert(kSlots >= KS + 2, "page scales must outlive their readers");
 
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release;" ::: "memory");
@@ -80,15 +86,21 @@ __device__ __forceinline__ uint32_t peer_addr(const void* p, uint32_t rank) {
   return r;
 }
 __device__ __forceinline__ void peer_store(uint32_t addr, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory"); }
+__device__ __forceinline__ void peer_store4(uint32_t addr, float x, float y, float z, float w) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(x), "f"(y), "f"(z), "f"(w) : "memory");
+}
 
 template <int HD, int QDT, bool F8>
 __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
-    diff_umma_kernel(const __grid_constant__ CUtensorMap pool_map, const __grid_constant__ CUtensorMap kb_map, const __grid_constant__ CUtensorMap vb_map,
-                     const DiffArgs args) {
+    diff_umma_kernel(const __grid_constant__ CUtensorMap pool_map, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap kb_map,
+                     const __grid_constant__ CUtensorMap vb_map, const DiffArgs args) {
   using C = Geo<HD>;
   using QE = Elem16<QDT>;
   extern __shared__ __align__(1024) uint8_t smem[];
-  Shared& sh = *reinterpret_cast<Shared*>(smem + C::TILES);
+  using Sh = Shared<C::VS>;
+  constexpr int VS = C::VS;
+  static_assert(C::TILES + int(sizeof(Sh)) <= C::SMEM, "bookkeeping behind the tiles");
+  Sh& sh = *reinterpret_cast<Sh*>(smem + C::TILES);
   const KernelArgs& a = args.k;
   const esp_attn_params& p = a.p;
   uint8_t* q_sm = smem;
@@ -98,11 +110,12 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
   const int map = int(blockIdx.z);  // = rank in the cluster
   if (tid == 0) {
     if ((smem_u32(smem) & 1023u) != 0) atomicExch(a.status, kStatusBadBlock);  // never expected; the swizzle would be wrong
+    mbar_init(&sh.q_full, 1);
     for (int s = 0; s < KS; ++s) mbar_init(&sh.k_full[s], kPages), mbar_init(&sh.k_empty[s], 1);
-    for (int s = 0; s < VS; ++s) mbar_init(&sh.v_full[s], kPages), mbar_init(&sh.v_empty[s], 1);
+    for (int s = 0; s < VS; ++s) mbar_init(&sh.v_full[s], kPages / C::SPB), mbar_init(&sh.v_empty[s], 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sh.s_full[i], 1), mbar_init(&sh.p_full[i][0], BM), mbar_init(&sh.p_full[i][1], BM), mbar_init(&sh.o_done[i], 1);
-      for (int w = 0; w < 4; ++w) mbar_init(&sh.m_ready[i][w], 1);
+      mbar_init(&sh.m_ready[i], 4);
     }
     for (int s = 0; s < kSlots; ++s) mbar_init(&sh.sc_full[s], 1);
     mbar_fence_init();
@@ -133,13 +146,15 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
     if (warp == kWarpK || warp == kWarpV) {
       const bool is_v = warp == kWarpV;
       if (lane == 0) tma_prefetch_desc(is_v ? &vb_map : &kb_map), tma_prefetch_desc(&pool_map);
-      const int depth = is_v ? VS : KS;
-      uint64_t* full = is_v ? sh.v_full : sh.k_full;
-      uint64_t* empty = is_v ? sh.v_empty : sh.k_empty;
+      // One code for both: two copies of the walk cost 4 to 5 % of a pass over cached pages.
+      const int depth = is_v ? VS : KS, step = is_v ? C::SPB : 1, lanes = is_v ? kPages / C::SPB : kPages;  // slots, slots per block, lanes per slot
+      uint64_t* full0 = is_v ? sh.v_full : sh.k_full;
+      uint64_t* empty0 = is_v ? sh.v_empty : sh.k_empty;
+      const int part = C::SPB > 1 && is_v && lane >= lanes ? 1 : 0, l = lane - part * lanes;  // this lane's slot of the block, its place there
       int stage = 0;
       uint32_t par = 1;  // the first use of a slot finds it empty
       auto advance = [&]() {
-        if (++stage == depth) stage = 0, par ^= 1;
+        if ((stage += step) == depth) stage = 0, par ^= 1;
       };
       auto scales = [&](int b, float ks, float vs) {  // this lane's page of block b
         if (!F8 || is_v) return;
@@ -148,6 +163,12 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
         __syncwarp(0xFFu);
         if (lane == 0) mbar_arrive(&sh.sc_full[slot]);
       };
+      if (!is_v && TR == BM && N > 0 && lane == 0) {  // a tile of one head: its Q rows are contiguous, too
+        mbar_arrive_expect_tx(&sh.q_full, C::K_TILE);
+#pragma unroll
+        for (int i = 0; i < C::QC; ++i) tma_load_3d(q_sm + i * C::CHUNK, &q_map, &sh.q_full, 0, tile.r0, int(blockIdx.y) * C::VC + map * C::QC + i);
+      }
+      __syncwarp();
       walk_pages<F8>(
           a, tree, L, is_v ? 1 : 0, lane,
           [&](int b, int kind, int y, int blk) {
@@ -156,33 +177,35 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
               ks = a.kv_scales[size_t(blk) * 2 * p.Hkv + kvh];
               vs = a.kv_scales[(size_t(blk) * 2 + 1) * p.Hkv + kvh];
             }
-            wait_bar(&empty[stage], par, kStatusMmaTimeout);
+            uint64_t* full = full0 + stage + part;
+            wait_bar(empty0 + stage + part, par, kStatusMmaTimeout);
             if (kind < 0) {
-              mbar_arrive(&full[stage]);
+              mbar_arrive(full);
             } else if (is_v) {
-              uint8_t* dst = v_sm + stage * C::V_TILE + lane * 2048;
-              mbar_arrive_expect_tx(&full[stage], 2048 * C::VC);
+              uint8_t* dst = v_sm + (stage + part) * C::V_SLOT + l * 2048;
+              mbar_arrive_expect_tx(full, 2048 * C::VC);
 #pragma unroll
-              for (int i = 0; i < C::VC; ++i) tma_load_3d(dst + i * C::CHUNK, &pool_map, &full[stage], 0, y, kvh * C::VC + i);
+              for (int i = 0; i < C::VC; ++i) tma_load_3d(dst + i * C::V_CHUNK, &pool_map, full, 0, y, kvh * C::VC + i);
             } else {
-              uint8_t* dst = k_sm + stage * C::K_TILE + lane * 2048;
-              mbar_arrive_expect_tx(&full[stage], 2048 * C::QC);
+              uint8_t* dst = k_sm + stage * C::K_TILE + l * 2048;
+              mbar_arrive_expect_tx(full, 2048 * C::QC);
 #pragma unroll
-              for (int i = 0; i < C::QC; ++i) tma_load_3d(dst + i * C::CHUNK, &pool_map, &full[stage], 0, y, kvh * C::VC + map * C::QC + i);
+              for (int i = 0; i < C::QC; ++i) tma_load_3d(dst + i * C::CHUNK, &pool_map, full, 0, y, kvh * C::VC + map * C::QC + i);
             }
             scales(b, ks, vs);
             advance();
           },
-          // Batch rows are contiguous: one load of 128 rows per chunk, by as many lanes. (Rows behind the tree's last one come along:
+          // Batch rows are contiguous: one load per slot and chunk, by as many lanes. (Rows behind the tree's last one come along:
           // other trees' or none, zero past the tensor. Their scores are hidden and their V rows cleared.)
           [&](int b, int y) {
-            wait_bar(&empty[stage], par, kStatusMmaTimeout);
-            if (lane < (is_v ? C::VC : C::QC)) {
-              mbar_arrive_expect_tx(&full[stage], C::CHUNK);
-              if (is_v) tma_load_3d(v_sm + stage * C::V_TILE + lane * C::CHUNK, &vb_map, &full[stage], 0, y, kvh * C::VC + lane);
-              else tma_load_3d(k_sm + stage * C::K_TILE + lane * C::CHUNK, &kb_map, &full[stage], 0, y, kvh * C::VC + map * C::QC + lane);
+            uint64_t* full = full0 + stage + part;
+            wait_bar(empty0 + stage + part, par, kStatusMmaTimeout);
+            if (l < (is_v ? C::VC : C::QC)) {
+              mbar_arrive_expect_tx(full, is_v ? C::V_CHUNK : C::CHUNK);
+              if (is_v) tma_load_3d(v_sm + (stage + part) * C::V_SLOT + l * C::V_CHUNK, &vb_map, full, 0, y + C::VK * part, kvh * C::VC + l);
+              else tma_load_3d(k_sm + stage * C::K_TILE + l * C::CHUNK, &kb_map, full, 0, y, kvh * C::VC + map * C::QC + l);
             } else {
-              mbar_arrive(&full[stage]);
+              mbar_arrive(full);
             }
             scales(b, 1.0f, 1.0f);
             advance();
@@ -199,7 +222,7 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
         const uint32_t one = elect_one();
         constexpr uint32_t idesc_qk = umma_idesc<QDT>(BM, C::BU, 0, 0), idesc_pv = umma_idesc<QDT>(BM, HD, 0, 1);
         const uint64_t q_desc = umma_smem_desc(smem_u32(q_sm), 16, 1024), k_desc = umma_smem_desc(smem_u32(k_sm), 16, 1024);
-        const uint64_t v_desc = umma_smem_desc(smem_u32(v_sm), C::CHUNK, 1024);
+        const uint64_t v_desc = umma_smem_desc(smem_u32(v_sm), C::V_CHUNK, 1024);
         const uint32_t q_lo = uint32_t(q_desc), k_lo0 = uint32_t(k_desc), v_lo0 = uint32_t(v_desc);
         const uint32_t hi_qk = uint32_t(q_desc >> 32), hi_v = uint32_t(v_desc >> 32);
         int kst = 0, vst = 0;
@@ -221,6 +244,7 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
             if (++kst == KS) kst = 0, kpar ^= 1;
           }
         };
+        if (TR == BM) wait_bar(&sh.q_full, 0, kStatusTmaTimeout);
         issue_qk(0, 0);
         if (N > 1) issue_qk(1 % C::UPB, 1);
 #pragma unroll 1
@@ -229,21 +253,25 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
           for (int i = 0; i < 2; ++i) {
             const int n = n0 + i, h = i % C::UPB;
             if (n >= N) break;
-            const uint32_t v_lo = v_lo0 + uint32_t(vst) * (C::V_TILE >> 4) + uint32_t((h * C::BU * 128) >> 4);
 #pragma unroll
             for (int part = 0; part < 2; ++part) {
+              constexpr int KSTEPS = C::PART / 16;
+              const int key0 = h * C::BU + part * C::PART;  // of the block
+              const bool opens = key0 % C::VK == 0, closes = (key0 + C::PART) % C::VK == 0;  // a V slot
               wait_bar(&sh.p_full[i][part], uint32_t(n >> 1) & 1u, kStatusMmaTimeout);
-              if (part == 0 && h == 0) wait_bar(&sh.v_full[vst], vpar, kStatusTmaTimeout);
+              if (opens) wait_bar(&sh.v_full[vst], vpar, kStatusTmaTimeout);
               tc_fence_after_sync();
+              const uint32_t v_lo = v_lo0 + uint32_t(vst) * (C::V_SLOT >> 4) + uint32_t((key0 % C::VK) * 128 >> 4);
 #pragma unroll
-              for (int ks = part * (C::PART / 16); ks < (part + 1) * (C::PART / 16); ++ks)
-                mma_ts(one, tmem + C::COL_O, tmem + C::COL_S + i * C::BU + ks * 8, v_lo + ((ks * 16 * 128) >> 4), hi_v, idesc_pv, ks > 0 ? 1u : uint32_t(n > 0));
+              for (int ks = 0; ks < KSTEPS; ++ks)
+                mma_ts(one, tmem + C::COL_O, tmem + C::COL_S + i * C::BU + (part * KSTEPS + ks) * 8, v_lo + ((ks * 16 * 128) >> 4), hi_v, idesc_pv,
+                       part > 0 || ks > 0 ? 1u : uint32_t(n > 0));
+              if (closes) {
+                mma_commit(one, &sh.v_empty[vst]);
+                if (++vst == VS) vst = 0, vpar ^= 1;
+              }
             }
             mma_commit(one, &sh.o_done[i]);
-            if (h == C::UPB - 1) {
-              mma_commit(one, &sh.v_empty[vst]);
-              if (++vst == VS) vst = 0, vpar ^= 1;
-            }
             if (n + 2 < N) issue_qk(h, i);  // over P of unit n: behind the P . V that reads it
           }
         }
@@ -258,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
     int4 dsc = make_int4(0, 0, 0, 0);
     uint64_t am = 0;
     const bool use_anc = a.anc_mask != nullptr;
-    {
+    if (TR != BM) {
       // the map's dims of this Q row, half of them per warpgroup (K-major, 128-byte swizzle)
       constexpr int LINES = C::MAP / 16;  // 16-byte pieces per thread
       const uint4* src = reinterpret_cast<const uint4*>(static_cast<const typename QE::T*>(a.Q) + size_t(row) * p.q_ld + size_t(head) * HD + map * C::MAP);
@@ -268,10 +296,10 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
         *reinterpret_cast<uint4*>(q_sm + (i >> 3) * C::CHUNK + srow * 128 + (((i & 7) ^ (srow & 7)) << 4)) = src[i];
       }
       fence_proxy_async_smem();
-      if (tile.last) {
-        if (use_anc) am = a.anc_mask[row];
-        else dsc = reinterpret_cast<const int4*>(a.desc)[row];
-      }
+    }
+    if (tile.last) {
+      if (use_anc) am = a.anc_mask[row];
+      else dsc = reinterpret_cast<const int4*>(a.desc)[row];
     }
     tc_fence_before_sync();
     named_barrier(1, kSoftmax + 32);
@@ -289,7 +317,7 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
       // the reference, from the partner warp that had the unit before: its maximum has long been known when these scores arrive
       float m_old = -INFINITY, v_ref = 0.0f;
       if (n > 0) {
-        wait_bar(&sh.m_ready[wg ^ 1][wq], uint32_t((n - 1) >> 1) & 1u, kStatusMmaTimeout);
+        wait_bar(&sh.m_ready[wg ^ 1], uint32_t((n - 1) >> 1) & 1u, kStatusMmaTimeout);
         m_old = *const_cast<volatile float*>(&sh.m_ref[srow]);
         if constexpr (F8) v_ref = *const_cast<volatile float*>(&sh.v_ref[wq]);
       }
@@ -335,17 +363,18 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
       }
       mx *= sl2;  // scale > 0
       if (!whole) {
-        const int first = max(L.n_valid(b), c0), lost = c0 + C::BU - first;
-        if (lost > 0) {
-          // V rows past the range are stale or foreign: 0 * NaN must not happen. Cleared before P is handed over.
-          const int vst = b % VS;
-          wait_bar(&sh.v_full[vst], uint32_t(b / VS) & 1u, kStatusTmaTimeout);
-          for (int i = srow; i < lost * 8 * C::VC; i += BM) {
-            const int r = first + i / (8 * C::VC), c = i % (8 * C::VC);
-            *reinterpret_cast<uint4*>(v_sm + vst * C::V_TILE + (c >> 3) * C::CHUNK + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+        // V rows past the range are stale or foreign: 0 * NaN must not happen. Cleared before P is handed over.
+#pragma unroll 1
+        for (int k0 = c0; k0 < c0 + C::BU; k0 += 64) {
+          const int first = max(L.n_valid(b) - k0, 0), q = b * C::SPB + k0 / C::VK;  // the q-th slot use
+          if (first >= 64) continue;
+          wait_bar(&sh.v_full[q % VS], uint32_t(q / VS) & 1u, kStatusTmaTimeout);
+          for (int i = srow; i < (64 - first) * 8 * C::VC; i += BM) {
+            const int r = k0 % C::VK + first + i / (8 * C::VC), c = i % (8 * C::VC);
+            *reinterpret_cast<uint4*>(v_sm + (q % VS) * C::V_SLOT + (c >> 3) * C::V_CHUNK + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
           }
-          fence_proxy_async_smem();
         }
+        fence_proxy_async_smem();
       }
       const bool grow = mx > m_old + kGrow;  // also the first finite maximum
       const float m_new = grow ? mx : m_old;
@@ -356,7 +385,7 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
       }
       *const_cast<volatile float*>(&sh.m_ref[srow]) = m_new;
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.m_ready[wg][wq]);
+      if (lane == 0) mbar_arrive(&sh.m_ready[wg]);
       if (m_new > m_seen) {
         l_run *= fast_exp2(m_seen - m_new);
         m_seen = m_new;
@@ -441,20 +470,20 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
       if (row_ok && wg == 0) *reinterpret_cast<float2*>(rec + HD) = make_float2(m_fin * kLn2, l);
     } else {
       constexpr int MINE = HD / 4;  // columns a thread finishes: CTA `map` has [map HD / 2, ..), group wg half of those
-      float* take = reinterpret_cast<float*>(v_sm);         // [HD / 2 columns][128 rows], lanes side by side; written by the peer
+      float* take = reinterpret_cast<float*>(v_sm);         // [HD / 8][128 rows][4 columns], lanes side by side; written by the peer
       float* sq = reinterpret_cast<float*>(q_sm);           // [CTA * 2 + group][128 rows]: the rows' sums of squares; written by both
       const float inv = l > 0.0f ? (map ? -diff_lam(args, row, head) : 1.0f) * v_ref / l : 0.0f;
       // the norm's weights into shared memory while the peer gets here (16-byte aligned, HD floats)
       float* w_sm = reinterpret_cast<float*>(k_sm) + 2 * BM;
       if (args.norm_w && tid < HD / 4) reinterpret_cast<float4*>(w_sm)[tid] = reinterpret_cast<const float4*>(args.norm_w)[tid];
       cluster_sync();  // neither CTA uses its tiles any more
-      const uint32_t peer_take = peer_addr(take, uint32_t(map ^ 1)) + uint32_t((wg * MINE * BM + srow) * 4);
+      const uint32_t peer_take = peer_addr(take, uint32_t(map ^ 1)) + uint32_t((wg * (MINE / 4) * BM + srow) * 16);
 #pragma unroll 1
       for (int q = 0; q < MINE / 32; ++q) {
         float v[32];
         load_o((map ^ 1) * C::MAP + wg * MINE + 32 * q, v);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) peer_store(peer_take + uint32_t((32 * q + i) * BM * 4), v[i] * inv);
+        for (int i = 0; i < 32; i += 4) peer_store4(peer_take + uint32_t((8 * q + i / 4) * BM * 16), v[i] * inv, v[i + 1] * inv, v[i + 2] * inv, v[i + 3] * inv);
       }
       float dv[MINE];
 #pragma unroll
@@ -467,9 +496,11 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
       cluster_sync();  // the peer's half has arrived
       float ss = 0.0f;
 #pragma unroll
-      for (int i = 0; i < MINE; ++i) {
-        dv[i] += take[(wg * MINE + i) * BM + srow];
-        ss = fmaf(dv[i], dv[i], ss);
+      for (int i = 0; i < MINE; i += 4) {
+        const float4 o = reinterpret_cast<const float4*>(take)[(wg * (MINE / 4) + i / 4) * BM + srow];
+        dv[i] += o.x, dv[i + 1] += o.y, dv[i + 2] += o.z, dv[i + 3] += o.w;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) ss = fmaf(dv[i + k], dv[i + k], ss);
       }
       sq[(map * 2 + wg) * BM + srow] = ss;
       peer_store(peer_addr(sq, uint32_t(map ^ 1)) + uint32_t(((map * 2 + wg) * BM + srow) * 4), ss);
@@ -512,7 +543,7 @@ cudaError_t setup_hd() {
   return e;
 }
 template <int HD>
-cudaError_t launch_hd(const DiffArgs& a, bool f8, const CUtensorMap& pool_map, const CUtensorMap& kb_map, const CUtensorMap& vb_map, cudaStream_t stream) {
+cudaError_t launch_hd(const DiffArgs& a, bool f8, const CUtensorMap& pool_map, const CUtensorMap& q_map, const CUtensorMap& kb_map, const CUtensorMap& vb_map, cudaStream_t stream) {
   const bool f16 = a.k.q_dtype == ESP_F16;
   auto kernel = f8 ? (f16 ? diff_umma_kernel<HD, ESP_F16, true> : diff_umma_kernel<HD, ESP_BF16, true>)
                    : (f16 ? diff_umma_kernel<HD, ESP_F16, false> : diff_umma_kernel<HD, ESP_BF16, false>);
@@ -525,7 +556,7 @@ cudaError_t launch_hd(const DiffArgs& a, bool f8, const CUtensorMap& pool_map, c
   attr[1].id = cudaLaunchAttributeClusterDimension;
   attr[1].val.clusterDim.x = 1, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 2;
   cfg.attrs = attr, cfg.numAttrs = 2;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, pool_map, kb_map, vb_map, a);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, pool_map, q_map, kb_map, vb_map, a);
   return e == cudaSuccess ? cudaGetLastError() : e;
 }
 
@@ -544,10 +575,10 @@ cudaError_t diff_umma_setup() {
   return e == cudaSuccess ? setup_hd<256>() : e;
 }
 
-cudaError_t launch_diff_umma(const DiffArgs& a, bool f8, const CUtensorMap& pool_map, const CUtensorMap& kb_map, const CUtensorMap& vb_map, cudaStream_t stream,
-                             uint64_t* launches) {
+cudaError_t launch_diff_umma(const DiffArgs& a, bool f8, const CUtensorMap& pool_map, const CUtensorMap& q_map, const CUtensorMap& kb_map, const CUtensorMap& vb_map,
+                             cudaStream_t stream, uint64_t* launches) {
   if (a.k.n_tiles <= 0) return cudaSuccess;
-  const cudaError_t e = a.k.HD == 128 ? launch_hd<128>(a, f8, pool_map, kb_map, vb_map, stream) : launch_hd<256>(a, f8, pool_map, kb_map, vb_map, stream);
+  const cudaError_t e = a.k.HD == 128 ? launch_hd<128>(a, f8, pool_map, q_map, kb_map, vb_map, stream) : launch_hd<256>(a, f8, pool_map, q_map, kb_map, vb_map, stream);
   if (e == cudaSuccess) ++*launches;
   return e;
 }

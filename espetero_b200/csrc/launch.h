@@ -223,13 +223,14 @@ cudaError_t launch_diff_general(const DiffArgs& a, cudaStream_t stream, uint64_t
 bool diff_decode_supports(int32_t HD, int32_t G, int32_t bt);
 cudaError_t diff_decode_setup();
 cudaError_t launch_diff_decode(const DiffArgs& a, const CUtensorMap& pool_map, cudaStream_t stream, uint64_t* launches);
-// tcgen05 kernels: tiles of 16 .. 128 rows. pool_map as flash_umma's; kb_map, vb_map the same view with boxes of 128 rows. f8: an E4M3 pool whose pages launch_diff_widen has laid out as 16-bit
+// tcgen05 kernels: tiles of 16 .. 128 rows. pool_map as flash_umma's; q_map, kb_map, vb_map the same view of Q, Kb and Vb
+// with boxes of 128 rows (Vb with 256-dim heads: 64). f8: an E4M3 pool whose pages launch_diff_widen has laid out as 16-bit
 // codes, one per entry of the block list; pool_map then covers those.
 cudaError_t launch_diff_widen(const KernelArgs& a, void* out, int32_t n_entries, cudaStream_t stream, uint64_t* launches);
 bool diff_umma_supports(int32_t HD, int32_t G, int32_t tile_rows, int32_t bt);
 cudaError_t diff_umma_setup();
-cudaError_t launch_diff_umma(const DiffArgs& a, bool f8, const CUtensorMap& pool_map, const CUtensorMap& kb_map, const CUtensorMap& vb_map, cudaStream_t stream,
-                             uint64_t* launches);
+cudaError_t launch_diff_umma(const DiffArgs& a, bool f8, const CUtensorMap& pool_map, const CUtensorMap& q_map, const CUtensorMap& kb_map, const CUtensorMap& vb_map,
+                             cudaStream_t stream, uint64_t* launches);
 cudaError_t launch_diff_combine(const DiffCombineArgs& a, cudaStream_t stream, uint64_t* launches);
 cudaError_t launch_diff_lambda(const float* q1, const float* k1, const float* q2, const float* k2, int32_t H, int32_t dim, int32_t ld,
                                float lambda_init, float* lam, cudaStream_t stream);

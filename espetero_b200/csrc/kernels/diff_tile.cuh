@@ -203,13 +203,22 @@ __device__ __forceinline__ float chunk_max(const uint32_t (&s)[32]) {
   return fmax3(fmaxf(m[0], m[1]), m[2], m[3]);
 }
 
-// 32 scores -> 16 packed pairs of weights exp2(sl2 s - m); `sum` (two partial sums) gains the unrounded weights. F8: v0, v1 = the V scales
-// of the chunk's two pages, in units of the tile's reference, on the weights that are handed on.
+// The same over an E4M3 pool: k0, k1 = the (positive) K scales of the chunk's two pages.
+__device__ __forceinline__ float chunk_max(const uint32_t (&s)[32], float k0, float k1) {
+  float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int c = 0; c < 32; c += 2) m[(c >> 4) * 2 + ((c >> 1) & 1)] = fmax3(m[(c >> 4) * 2 + ((c >> 1) & 1)], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+  return fmaxf(fmaxf(m[0], m[1]) * k0, fmaxf(m[2], m[3]) * k1);
+}
+
+// 32 scores -> 16 packed pairs of weights exp2(sl s - m), sl = sl_a for the chunk's first 16 columns and sl_b for the others (a page each);
+// `sum` (two partial sums) gains the unrounded weights. F8: v0, v1 = the V scales of the two pages, in units of the tile's reference, on
+// the weights that are handed on.
 template <int QDT, bool F8>
-__device__ __forceinline__ void chunk_weights(const uint32_t (&s)[32], uint32_t* pk, uint64_t sl2x2, uint64_t neg_m2, uint64_t (&sum)[2], float v0, float v1) {
+__device__ __forceinline__ void chunk_weights(const uint32_t (&s)[32], uint32_t* pk, uint64_t sl_a, uint64_t sl_b, uint64_t neg_m2, uint64_t (&sum)[2], float v0, float v1) {
 #pragma unroll
   for (int c = 0; c < 16; ++c) {
-    const uint64_t x2 = f32x2_fma(f32x2_pack(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1])), sl2x2, neg_m2);
+    const uint64_t x2 = f32x2_fma(f32x2_pack(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1])), c < 8 ? sl_a : sl_b, neg_m2);
     float x0, x1;
     f32x2_unpack(x2, x0, x1);
     const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);

@@ -321,25 +321,22 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
         m_old = *const_cast<volatile float*>(&sh.m_ref[srow]);
         if constexpr (F8) v_ref = *const_cast<volatile float*>(&sh.v_ref[wq]);
       }
-      float ks[2 * NS], vs[2 * NS], largest = 0.0f;
+      float ks[2 * NS] = {}, vs[2 * NS] = {}, largest = 0.0f;
       if constexpr (F8) {
         wait_bar(&sh.sc_full[b % kSlots], uint32_t(b / kSlots) & 1u, kStatusTmaTimeout);
 #pragma unroll
         for (int i = 0; i < 2 * NS; ++i) {
-          ks[i] = sh.k_scale[b % kSlots][c0 / 16 + i], vs[i] = sh.v_scale[b % kSlots][c0 / 16 + i];
+          ks[i] = fmaxf(sh.k_scale[b % kSlots][c0 / 16 + i], 1.17549435e-38f), vs[i] = sh.v_scale[b % kSlots][c0 / 16 + i];  // -inf * 0 must not happen
           largest = fmaxf(largest, vs[i]);
         }
       }
       wait_bar(&sh.s_full[wg], par, kStatusMmaTimeout);
       tc_fence_after_sync();
-      // 32 scores as they count: times their pages' K scales, hidden where the row does not see the key
+      // 32 scores, hidden where the row does not see the key; and their maximum, with the pages' K scales
       auto shape = [&](uint32_t (&x)[32], int i) {
-        if constexpr (F8) {
-#pragma unroll
-          for (int k = 0; k < 32; ++k) x[k] = __float_as_uint(__uint_as_float(x[k]) * ks[2 * i + (k >> 4)]);
-        }
         if (!whole) hide(x, visible32(L, b, c0 + 32 * i, dsc, am, use_anc, rr));
       };
+      auto top = [&](const uint32_t (&x)[32], int i) { return F8 ? chunk_max(x, ks[2 * i], ks[2 * i + 1]) : chunk_max(x); };
       constexpr int HELD = C::HOLD ? NS : 1;
       uint32_t s[HELD][32];
       float mx = -INFINITY;
@@ -350,7 +347,7 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
         for (int i = 0; i < NS; ++i) {
           tmem_wait_ld_of(s[i]);
           shape(s[i], i);
-          mx = fmaxf(mx, chunk_max(s[i]));
+          mx = fmaxf(mx, top(s[i], i));
         }
       } else {
 #pragma unroll
@@ -358,7 +355,7 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
           tmem_ld32(buf + 32 * i, s[0]);
           tmem_wait_ld_of(s[0]);
           shape(s[0], i);
-          mx = fmaxf(mx, chunk_max(s[0]));
+          mx = fmaxf(mx, top(s[0], i));
         }
       }
       mx *= sl2;  // scale > 0
@@ -416,7 +413,7 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
           shape(s[0], i);
         }
         uint32_t pk[16];
-        chunk_weights<QDT, F8>(s[C::HOLD ? i : 0], pk, sl2x2, neg_m2, sum, F8 ? vs[2 * i] * vinv : 1.0f, F8 ? vs[2 * i + 1] * vinv : 1.0f);
+        chunk_weights<QDT, F8>(s[C::HOLD ? i : 0], pk, F8 ? f32x2_pack(sl2 * ks[2 * i], sl2 * ks[2 * i]) : sl2x2, F8 ? f32x2_pack(sl2 * ks[2 * i + 1], sl2 * ks[2 * i + 1]) : sl2x2, neg_m2, sum, F8 ? vs[2 * i] * vinv : 1.0f, F8 ? vs[2 * i + 1] * vinv : 1.0f);
         tmem_st16(buf + 16 * i, pk);
         if ((i + 1) % (C::PART / 32) == 0) {  // a part is ready: its P . V starts under the rest
           tmem_wait_st();

@@ -4,7 +4,7 @@
 //   M = max m_s,  L = sum e^(m_s - M) l_s,  A = sum e^(m_s - M) O_s   (records in order, no atomics: the result does not
 // depend on scheduling), then D = A_1 / L_1 - lam A_2 / L_2 and the norm. HD / 4 threads (4 dims each) per slice of records, NSL slices
 // per map, two maps per (row, head), as many (row, head) pairs as fit a CTA; the slices are joined in order through shared memory.
-// A slice asks for up to eight records before it folds the first. Few long jobs (decode) are latency-bound and take many slices;
+// A slice asks for several records before it folds the first. Few long jobs (decode) are latency-bound and take many slices;
 // many short ones (trees: two records per row) are bound by the records' bytes and take one: 16 x (4096 + 16) trees, split in two,
 // 43.6 us with four slices and one pair per CTA.
 #include "diff.cuh"
@@ -43,10 +43,15 @@ __global__ void __launch_bounds__(kThreads) diff_combine_kernel(const DiffCombin
     acc.x = acc.x * f + w * o.x, acc.y = acc.y * f + w * o.y, acc.z = acc.z * f + w * o.z, acc.w = acc.w * f + w * o.w;
     M = mn;
   };
-  for (int s = sl; s < n; s += 8 * NSL) {
-    float2 ml[8], lo[8], hi[8];
+  // what the finish needs, asked for with the first records
+  const int row = job.r0 + r;
+  const float4 w = a.norm_w ? *reinterpret_cast<const float4*>(a.norm_w + 4 * d4) : make_float4(1.f, 1.f, 1.f, 1.f);
+  const float lam = live ? diff_lam(a, row, h) : 0.0f;
+  constexpr int AHEAD = NSL > 1 ? 8 : 4;
+  for (int s = sl; s < n; s += AHEAD * NSL) {
+    float2 ml[AHEAD], lo[AHEAD], hi[AHEAD];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < AHEAD; ++i) {
       ml[i] = make_float2(-INFINITY, 0.0f), lo[i] = hi[i] = make_float2(0.f, 0.f);
       if (s + i * NSL < n) {
         const float* rec = rec0 + size_t(s + i * NSL) * stride;  // records are 8-byte aligned (HD + 2 floats)
@@ -54,8 +59,19 @@ __global__ void __launch_bounds__(kThreads) diff_combine_kernel(const DiffCombin
         lo[i] = *reinterpret_cast<const float2*>(rec + 4 * d4), hi[i] = *reinterpret_cast<const float2*>(rec + 4 * d4 + 2);
       }
     }
+    float mx = M;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) fold(ml[i].x, ml[i].y, make_float4(lo[i].x, lo[i].y, hi[i].x, hi[i].y));
+    for (int i = 0; i < AHEAD; ++i) mx = fmaxf(mx, ml[i].x);
+    if (mx == -INFINITY) continue;  // nothing but empty records so far
+    const float f = __expf(M - mx);  // M = -inf: 0
+    L *= f, acc.x *= f, acc.y *= f, acc.z *= f, acc.w *= f, M = mx;
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      if (ml[i].x == -INFINITY) continue;  // an empty record
+      const float x = __expf(ml[i].x - mx);
+      L = fmaf(x, ml[i].y, L);
+      acc.x = fmaf(x, lo[i].x, acc.x), acc.y = fmaf(x, lo[i].y, acc.y), acc.z = fmaf(x, hi[i].x, acc.z), acc.w = fmaf(x, hi[i].y, acc.w);
+    }
   }
   float* mine = part[tid];
   if (NSL > 1) {
@@ -72,10 +88,9 @@ __global__ void __launch_bounds__(kThreads) diff_combine_kernel(const DiffCombin
   __syncthreads();
   const bool owner = sl == 0 && map == 0 && live;
   float d[4] = {0.f, 0.f, 0.f, 0.f};
-  const int row = job.r0 + r;
   if (owner) {
     const float* o = part[tid + PER_MAP];
-    const float inv1 = L > 0.0f ? 1.0f / L : 0.0f, inv2 = o[4] > 0.0f ? diff_lam(a, row, h) / o[4] : 0.0f;
+    const float inv1 = L > 0.0f ? 1.0f / L : 0.0f, inv2 = o[4] > 0.0f ? lam / o[4] : 0.0f;
     d[0] = acc.x * inv1 - o[0] * inv2, d[1] = acc.y * inv1 - o[1] * inv2, d[2] = acc.z * inv1 - o[2] * inv2, d[3] = acc.w * inv1 - o[3] * inv2;
   }
   // the row's sum of squares: over the TPD owners, which are whole warps or an aligned part of one
@@ -91,7 +106,6 @@ __global__ void __launch_bounds__(kThreads) diff_combine_kernel(const DiffCombin
   }
   if (!owner) return;
   const float f = diff_row_factor(a, ss, HD);
-  const float4 w = a.norm_w ? *reinterpret_cast<const float4*>(a.norm_w + 4 * d4) : make_float4(1.f, 1.f, 1.f, 1.f);
   *reinterpret_cast<uint2*>(static_cast<typename QE::T*>(k.O) + size_t(row) * k.p.q_ld + size_t(h) * HD + 4 * d4) =
       make_uint2(QE::pack2(d[0] * f * w.x, d[1] * f * w.y), QE::pack2(d[2] * f * w.z, d[3] * f * w.w));
 }

@@ -1215,8 +1215,12 @@ int esp_diff_plan_opts(const esp_attn_shape* s, const esp_attn_tree* trees, int3
   *o = esp_plan_opts{};
   o->mode = ESP_PLAN_B200, o->min_chunk = 32, o->max_parts = 64;
   const int G = s->H / s->Hkv;
-  if (single) {  // diff_decode: one wave of its CTAs (two per SM, four where a key block is 4 KB)
-    o->tile_rows = 8, o->groups = 148 * (s->kv_dtype == ESP_E4M3 && s->HD == 128 ? 4 : 2), o->split = 1 << 20;
+  if (single) {
+    // diff_decode: one wave of its CTAs. Their rings are 192 KB for blocks of 16 keys of 256 16-bit dims, so one CTA fills an SM (7 sequences
+    // of 1 .. 6001 keys, 8 kv heads: 13.2 us against 17.3 with two CTAs' worth of tiles); two do at half of that. At a quarter (E4M3,
+    // 128 dims) four fit, and three leave batches that fill the SMs anyway unsplit (64 x 500 .. 3000 keys, 8 kv heads: 49.0 us against 57.7;
+    // 1 x 32768: 23.0 against 21.4). Chunks below 64 keys only add records (2 kv heads, 1024 keys: 7.5 us at 32, 6.9 at 64).
+    o->tile_rows = 8, o->groups = 148 * std::max(1, std::min(3, 512 / row_bytes)), o->split = 1 << 20, o->min_chunk = 64;
     return ESP_OK;
   }
   if (cached <= 2 * fresh) {  // mostly its own rows: 128-row tiles, one head each, nothing split
@@ -1305,12 +1309,6 @@ int esp_diff_forward(esp_attn_ctx* c, void* stream, const esp_attn_args* ap, con
   if (decode) {
     if (int rc = pool_tensor_map(c, a)) return rc;
     c->last_kernel = "diff_decode";
-    // Jobs of few records are joined by the CTA that finishes last (option "fuse_combine": 0 never, 2 always); long ones take the
-    // join kernel's parallelism.
-    int most = 0;
-    for (int i = 0; a.jobs_host && i < a.n_jobs; ++i) most = std::max(most, a.jobs_host[i].nparts);
-    k.fuse = c->opt_fuse_combine && a.n_jobs > 0 && a.jobs && (c->opt_fuse_combine == 2 || most <= 16) &&
-             esp::plan_fusable(a.tiles_host, a.n_tiles, a.jobs_host, a.n_jobs, s.Hkv);
     ProfScope prof(c, st, c->last_kernel);
     e = esp::launch_diff_decode(d, c->pool_map, st, &c->launches);
   } else if (umma) {
@@ -1340,7 +1338,7 @@ int esp_diff_forward(esp_attn_ctx* c, void* stream, const esp_attn_args* ap, con
     e = esp::launch_diff_general(d, st, &c->launches);
   }
   if (e != cudaSuccess) return cuda_fail(e, c->last_kernel);
-  if (a.n_jobs > 0 && !k.fuse) {
+  if (a.n_jobs > 0) {
     esp::DiffCombineArgs m{d, a.n_jobs, c->tile_rows, 64};
     if (a.jobs_host) {
       m.rows_max = m.parts_max = 1;

@@ -47,8 +47,6 @@ __global__ void __launch_bounds__(C::NW * 32, C::CTAS) diff_decode_kernel(const 
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full_bar[NW][STAGES];
   __shared__ int gave_up;
-  __shared__ int fix[3];  // merged in the kernel: first record and record count of the tile's job, the ticket drawn
-  __shared__ float sq[NW];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const KernelArgs& a = d.k;
   const esp_attn_params& p = a.p;
@@ -78,14 +76,9 @@ __global__ void __launch_bounds__(C::NW * 32, C::CTAS) diff_decode_kernel(const 
   const int G = a.G, row = tile.r0;
   const float sl2 = a.scale * kLog2e;
   uint8_t* wsm = smem + size_t(warp) * C::WARP_BYTES;
-  const bool fused = a.fuse && tile.part >= 0;
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&pool_map);
     gave_up = 0;
-    if (fused) {  // needed only at the very end
-      const esp_attn_combine jb = a.jobs[tile.pad1 - 1];
-      fix[0] = jb.part0, fix[1] = jb.nparts;
-    }
   }
   if (lane == 0) {
 #pragma unroll
@@ -429,76 +422,6 @@ __global__ void __launch_bounds__(C::NW * 32, C::CTAS) diff_decode_kernel(const 
     typename QE::T* op = static_cast<typename QE::T*>(a.O) + size_t(row) * p.q_ld + size_t(h) * HD;
 #pragma unroll
     for (int i = 0; i < DPL; ++i) op[lane + 32 * i] = QE::from_f32(acc[0][i] * f * (d.norm_w ? d.norm_w[lane + 32 * i] : 1.0f));
-  }
-
-  // ---- the join, in the CTA that draws its job's last ticket: the records of this kv head in record order (the result does not depend
-  // on who came last), straight from L2. Saves the second launch where the jobs have few records.
-  if (!fused) return;
-  __threadfence();
-  __syncthreads();
-  const int part0 = fix[0], n_rec = fix[1];
-  if (threadIdx.x == 0) {
-    int* ticket = a.counters + (size_t(tile.pad1 - 1) * p.Hkv + kvh) * kFixupPerJob;
-    const int prev = atomicAdd(ticket, 1);
-    if (prev == n_rec - 1) *ticket = 0;  // ready for the next pass on this stream
-    fix[2] = prev;
-  }
-  __syncthreads();
-  if (fix[2] != n_rec - 1) return;
-  __threadfence();
-  constexpr int TPD = HD / 4, PER_PASS = NW * 32 / TPD;  // threads per head (4 dims each), heads at a time
-  static_assert(PER_PASS >= 1 && (TPD == 32 || TPD == 64), "a head is one warp or two");
-  const size_t stride = diff_record(a, 1, 0, 0, 0, 0);
-  for (int h0 = 0; h0 < G; h0 += PER_PASS) {
-    const int hg = h0 + int(threadIdx.x) / TPD, d4 = int(threadIdx.x) % TPD;
-    const bool live = hg < G;
-    float r[2][4], L[2];
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const float* rec = a.parts + diff_record(a, part0, kvh, 0, live ? hg : 0, c);
-      float M = -INFINITY;
-      L[c] = 0.0f;
-      r[c][0] = r[c][1] = r[c][2] = r[c][3] = 0.0f;
-      for (int q0 = 0; q0 < n_rec; q0 += 4) {
-        float2 ml[4], lo[4], hi[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float* x = rec + size_t(min(q0 + i, n_rec - 1)) * stride;
-          ml[i] = __ldcg(reinterpret_cast<const float2*>(x + HD));
-          lo[i] = __ldcg(reinterpret_cast<const float2*>(x + 4 * d4)), hi[i] = __ldcg(reinterpret_cast<const float2*>(x + 4 * d4 + 2));
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (q0 + i >= n_rec || ml[i].x == -INFINITY) continue;
-          const float mn = fmaxf(M, ml[i].x), f = __expf(M - mn), w = __expf(ml[i].x - mn);
-          L[c] = fmaf(L[c], f, w * ml[i].y);
-          r[c][0] = fmaf(r[c][0], f, w * lo[i].x), r[c][1] = fmaf(r[c][1], f, w * lo[i].y);
-          r[c][2] = fmaf(r[c][2], f, w * hi[i].x), r[c][3] = fmaf(r[c][3], f, w * hi[i].y);
-          M = mn;
-        }
-      }
-    }
-    const int h = kvh * G + (live ? hg : 0);
-    const float inv1 = L[0] > 0.0f ? 1.0f / L[0] : 0.0f, inv2 = L[1] > 0.0f ? diff_lam(d, row, h) / L[1] : 0.0f;
-    float v[4], ss = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[i] = r[0][i] * inv1 - r[1][i] * inv2;
-      ss = fmaf(v[i], v[i], ss);
-    }
-#pragma unroll
-    for (int off = 16; off; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
-    if constexpr (TPD == 64) {
-      if (lane == 0) sq[warp] = ss;
-      __syncthreads();
-      ss = sq[warp & ~1] + sq[warp | 1];
-      __syncthreads();
-    }
-    if (!live) continue;
-    const float f = diff_row_factor(d, ss, HD);
-    const float4 w = d.norm_w ? *reinterpret_cast<const float4*>(d.norm_w + 4 * d4) : make_float4(1.f, 1.f, 1.f, 1.f);
-    *reinterpret_cast<uint2*>(static_cast<typename QE::T*>(a.O) + size_t(row) * p.q_ld + size_t(h) * HD + 4 * d4) =
-        make_uint2(QE::pack2(v[0] * f * w.x, v[1] * f * w.y), QE::pack2(v[2] * f * w.z, v[3] * f * w.w));
   }
 }
 

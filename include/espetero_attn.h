@@ -505,10 +505,8 @@ int esp_kv_append(esp_attn_ctx* ctx, void* stream, const esp_kv_append_args* arg
  *    bidi and the sparse-attention arguments must be 0 / NULL (ESP_ERR_UNSUPPORTED);
  *  - tiles are never planned again: esp_diff_plan_opts says which tile height (a property of the context) and planner options
  *    suit a pass; every plan of esp_attn_plan is right, some are slow (see below).
- * Split passes of single tokens whose jobs have 16 records or fewer are joined inside diff_decode, with arrival counters of the context
- * (option "fuse_combine", 0 switches that off): such passes of one context must not overlap on the GPU, on two streams or in
- * two graphs, just as those of esp_attn_forward must not. The join is in record order either way: the same bits every time.
- * The page scales of an E4M3 pool are positive. A row that sees no key gets zeros. Rows that no tile covers are left as they were. Keys behind a tree's last row and pool
+ * The page scales of an E4M3 pool are positive.
+ * A row that sees no key gets zeros. Rows that no tile covers are left as they were. Keys behind a tree's last row and pool
  * rows past P are never mixed in, whatever they hold; keys that another row of the same tree sees must be finite.
  * Kernels: "diff_decode" (all trees have one row, G <= 8, HD 128 or 256, pages of 16 n keys), "diff_umma"
  * (HD 128 or 256, pages of 16 n keys, tile ranges that start at a multiple of 16) for tiles of 16, 32, 64 or 128 rows, 128 / tile_rows heads of

@@ -1220,6 +1220,7 @@ int esp_diff_plan_opts(const esp_attn_shape* s, const esp_attn_tree* trees, int3
     // of 1 .. 6001 keys, 8 kv heads: 13.2 us against 17.3 with two CTAs' worth of tiles); two do at half of that. At a quarter (E4M3,
     // 128 dims) four fit, and three leave batches that fill the SMs anyway unsplit (64 x 500 .. 3000 keys, 8 kv heads: 49.0 us against 57.7;
     // 1 x 32768: 23.0 against 21.4). Chunks below 64 keys only add records (2 kv heads, 1024 keys: 7.5 us at 32, 6.9 at 64).
+    const int row_bytes = s->HD * (s->kv_dtype == ESP_E4M3 ? 1 : 2);
     o->tile_rows = 8, o->groups = 148 * std::max(1, std::min(3, 512 / row_bytes)), o->split = 1 << 20, o->min_chunk = 64;
     return ESP_OK;
   }

@@ -1233,10 +1233,11 @@ int esp_diff_plan_opts(const esp_attn_shape* s, const esp_attn_tree* trees, int3
   o->tile_rows = 128 / c;
   // How far to split the cached keys, by the time each choice would take: CTAs (two per tile and head group) on the SMs' slots, a
   // fixed cost per CTA and one per 128 keys, and the join of the records. Microseconds, measured on diff_umma; with 128-dim heads two
-  // CTAs share an SM and each runs slower than alone.
+  // CTAs share an SM and each runs slower than alone. 700 rows behind 20001 keys, 8 kv heads, took 525 us unsplit, 484 in two, 515 in
+  // three and 533 in four parts; the rule gives 523, 475, 506 and 532.
   const bool wide = s->HD >= 256;
   const int per_tile = s->Hkv * (G / c) * 2;
-  const double t_block = 1.05, t_shared = 1.45, t_fixed = 9.0;  // per 128 keys alone / sharing an SM; start and end of a CTA
+  const double t_alone = wide ? 1.45 : 1.2, t_shared = 1.9, t_fixed = 9.0;  // per 128 keys alone / sharing an SM; start and end of a CTA
   double best = 0;
   for (int parts = 1; parts <= 32; ++parts) {
     int64_t tiles = 0, rows_split = 0;
@@ -1248,11 +1249,10 @@ int esp_diff_plan_opts(const esp_attn_shape* s, const esp_attn_tree* trees, int3
       if (ns > 1) rows_split += int64_t(trees[i].M) * ns;
       longest = std::max(longest, (trees[i].P / ns + 127) / 128 + (ns == 1 ? (std::min(trees[i].M, 1 << 20) + 127) / 128 : 1));
     }
-    const int64_t ctas = tiles * per_tile, slots = wide ? 148 : (ctas <= 148 ? 148 : 296);
-    const double waves = double((ctas + slots - 1) / slots);
-    const double per_block = wide ? t_block : (slots == 148 ? 0.9 * t_block : t_shared);
-    const double join = rows_split ? 6.0 + double(rows_split) * s->H * 2 * (s->HD + 2) * 4 * 2 / 4.0e6 : 0.0;  // written and read at about 4 TB/s
-    const double t = waves * (longest * per_block + t_fixed) + join;
+    const int64_t ctas = tiles * per_tile, slots = wide ? 148 : 296, rest = ctas % slots;
+    double t = double(ctas / slots) * (longest * (wide ? t_alone : t_shared) + t_fixed);
+    if (rest) t += longest * (rest <= 148 ? t_alone : t_shared) + t_fixed;
+    if (rows_split) t += 6.0 + double(rows_split) * s->H * 2 * (s->HD + 2) * 4 * 2 / 6.0e6;  // written and read at about 6 TB/s, mostly in L2
     if (parts == 1 || t < 0.97 * best) {
       best = t;
       // the planner sizes its chunks so that the tiles fit `groups / Hkv`

@@ -592,6 +592,18 @@ static bool stage_plan(esp_attn_ctx* c, esp_attn_args& a, int& TR, int new_TR, i
 
 }  // extern "C"
 
+// Option "check_finite": the pass's output is scanned; esp_attn_check_status reports.
+static int scan_output(esp_attn_ctx* c, const esp_attn_args& a, cudaStream_t stream) {
+  if (!c->opt_check_finite || a.n_rows <= 0) return ESP_OK;
+  const esp_attn_shape& s = c->shape;
+  const cudaError_t e = esp::launch_finite_check(a.O, uint32_t(a.n_rows), uint32_t(s.H * s.HD), uint64_t(a.p.q_ld),
+                                                 s.q_dtype == ESP_F16 ? ESP_FINITE_F16 : ESP_FINITE_BF16, 0x7F800000u,
+                                                 reinterpret_cast<uint32_t*>(c->d_status + kFiniteRecAt), stream, &c->launches);
+  if (e != cudaSuccess) return cuda_fail(e, "finite_check");
+  c->finite_armed = true;
+  return ESP_OK;
+}
+
 // xch != NULL: the pass is one rank's share of a sequence split over several GPUs and ends with the peer
 // exchange inside the decode kernel. *fused_out tells whether that happened; if not, nothing was launched
 // for the exchange and the caller takes the two-kernel route.
@@ -796,14 +808,7 @@ static int forward_impl(esp_attn_ctx* c, void* stream_v, const esp_attn_args* ap
     if (int rc = combine_impl(c, stream_v, a.parts, a.X, a.O, a.lse, &a.p, a.jobs, a.n_jobs, rows_max, parts_max, nullptr, 0, a.jobs_host, TR)) return rc;
   }
   if (replan_slot >= 0) cudaEventRecord(c->replan_done[replan_slot], stream);  // the slot's tiles and jobs have been read
-  if (c->opt_check_finite && a.n_rows > 0) {
-    const cudaError_t fe = esp::launch_finite_check(a.O, uint32_t(a.n_rows), uint32_t(s.H * s.HD), uint64_t(a.p.q_ld),
-                                                    s.q_dtype == ESP_F16 ? ESP_FINITE_F16 : ESP_FINITE_BF16, 0x7F800000u,
-                                                    reinterpret_cast<uint32_t*>(c->d_status + kFiniteRecAt), stream, &c->launches);
-    if (fe != cudaSuccess) return cuda_fail(fe, "finite_check");
-    c->finite_armed = true;
-  }
-  return ESP_OK;
+  return scan_output(c, a, stream);
 }
 
 extern "C" {
@@ -1349,7 +1354,7 @@ int esp_diff_forward(esp_attn_ctx* c, void* stream, const esp_attn_args* ap, con
     e = esp::launch_diff_combine(m, st, &c->launches);
     if (e != cudaSuccess) return cuda_fail(e, "diff_combine");
   }
-  return ESP_OK;
+  return scan_output(c, a, st);
 }
 
 int esp_diff_lambda(void* stream, const float* q1, const float* k1, const float* q2, const float* k2, int32_t H, int32_t dim, int32_t ld,

@@ -77,6 +77,14 @@ def diff_plan_options(trees: np.ndarray, H: int, Hkv: int, HD: int, kv_dtype: in
     return o.tile_rows, dict(mode=o.mode, split=o.split, min_chunk=o.min_chunk, groups=o.groups, tile_rows=o.tile_rows, max_parts=o.max_parts)
 
 
+def _check_rows(name: str, t, ld: int | None = None):
+    """Rows of contiguous elements, `ld` elements apart where the call takes no stride for them."""
+    if t is None:
+        return
+    if t.dim() != 2 or t.stride(1) != 1 or (ld is not None and t.shape[0] > 1 and t.stride(0) != ld):
+        raise ValueError(f"{name}: rows of contiguous elements{'' if ld is None else f', {ld} apart,'} expected, not strides {tuple(t.stride())}")
+
+
 @dataclass
 class Call:
     """Arguments of one call and what they point to (device tensors, host records), kept alive together."""
@@ -302,6 +310,11 @@ class AttnOp:
                     maps=1, adjacent=False, qscale=1.0, kv_base=0) -> Call:
         """Arguments of esp_kv_append from device tensors: Q / K / V are [rows, heads * HD] with any row stride, 16-bit or fp32."""
         s, a = self.shape, capi.AppendArgs()
+        for name, t in (("Q", Q), ("K", K), ("V", V)):
+            _check_rows(name, t)
+        _check_rows("Kb", Kb, s.Hkv * s.HD)
+        _check_rows("Vb", Vb, s.Hkv * s.HD)
+        _check_rows("Qo", Qo)
         a.Q, a.K, a.V, a.Qo, a.Kb, a.Vb = (_ptr(t) for t in (Q, K, V, Qo, Kb, Vb))
         a.kv, a.kv_scales, a.slots, a.pos, a.inv_freq = (_ptr(t) for t in (kv, kv_scales, slots, pos, inv_freq))
         a.q_src_ld, a.k_src_ld, a.v_src_ld = 0 if Q is None else Q.stride(0), K.stride(0), V.stride(0)
@@ -325,6 +338,10 @@ class AttnOp:
         """Arguments of esp_diff_forward from a plan and device tensors; `parts` (and, over an E4M3 pool, the scratch of
         multi-row passes) are allocated unless given."""
         s, a = self.shape, capi.Args()
+        _check_rows("Q", Q)
+        _check_rows("O", O, Q.stride(0))
+        _check_rows("Kb", Kb, s.Hkv * s.HD)
+        _check_rows("Vb", Vb, s.Hkv * s.HD)
         trees = np.ascontiguousarray(trees, dtype=TREE_DT)
         tiles_dev, trees_dev, jobs_dev = (_dev(x, self.device) if len(x) else None for x in (plan.tiles, trees, plan.jobs))
         if parts is None and plan.n_parts:

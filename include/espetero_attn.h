@@ -505,13 +505,16 @@ int esp_kv_append(esp_attn_ctx* ctx, void* stream, const esp_kv_append_args* arg
  *    bidi and the sparse-attention arguments must be 0 / NULL (ESP_ERR_UNSUPPORTED);
  *  - tiles are never planned again: esp_diff_plan_opts says which tile height (a property of the context) and planner options
  *    suit a pass; every plan of esp_attn_plan is right, some are slow (see below).
- * The page scales of an E4M3 pool are positive.
+ * The page scales of an E4M3 pool are positive. `blocks` may hold entries that no tile reads (a padded table's), whatever they are.
+ * Passes of one context may overlap on the GPU - two streams, two graphs - while their O, parts and dequant_scratch are apart.
  * A row that sees no key gets zeros. Rows that no tile covers are left as they were. Keys behind a tree's last row and pool
  * rows past P are never mixed in, whatever they hold; keys that another row of the same tree sees must be finite.
  * Kernels: "diff_decode" (all trees have one row, G <= 8, HD 128 or 256, pages of 16 n keys), "diff_umma"
- * (HD 128 or 256, pages of 16 n keys, tile ranges that start at a multiple of 16) for tiles of 16, 32, 64 or 128 rows, 128 / tile_rows heads of
- * one kv head each (16-bit pools; E4M3 pools through dequant_scratch, sized as for esp_attn_forward; passes without cached keys), "diff_general" for everything else, plus "diff_combine" for split plans.
- * esp_attn_last_kernel names the first of these. Sums, maxima and the difference are fp32; softmax weights are rounded to the
+ * (HD 128 or 256, pages of 16 n keys, tile ranges that start at a multiple of 16) for tiles of 16, 32, 64 or 128 rows, 128 / tile_rows
+ * heads of one kv head each (16-bit pools; E4M3 pools through dequant_scratch, sized as for esp_attn_forward; passes without
+ * cached keys), "diff_general" for everything else and for calls without the host mirrors of tiles and trees, plus "diff_combine"
+ * for split plans. esp_attn_last_kernel names the first of these. The option "attn_gqa" 0 keeps passes from diff_decode,
+ * "attn_umma" 0 from diff_umma; "check_finite" scans these passes' output, too. Sums, maxima and the difference are fp32; softmax weights are rounded to the
  * pass's 16-bit type (fp16 over E4M3 pools in diff_decode, not at all in diff_general) before they meet V. */
 typedef struct esp_diff_args {
   const float* lam;    /* lam[row * lam_ld + h]: per head, lam_ld = 0, or per row and head, lam_ld >= H */
@@ -709,7 +712,8 @@ int esp_attn_finite_check(void* stream, const void* x, uint32_t rows, uint32_t c
                           esp_finite_rec* rec_device);
 
 /* Name of the attention kernel the last esp_attn_forward on this context
- * launched ("decode_gqa", "flash_umma", "flash_umma_pair", "flash_umma_duo", "flash_general"), for tests and traces. */
+ * launched ("decode_gqa", "flash_umma", "flash_umma_pair", "flash_umma_duo", "flash_general"), or the last esp_diff_forward
+ * ("diff_decode", "diff_umma", "diff_general"), for tests and traces. */
 const char* esp_attn_last_kernel(const esp_attn_ctx* ctx);
 
 /* Reads and clears the context's device status word: a kernel whose bounded wait ran

@@ -369,6 +369,86 @@ def test_a_pass_again_and_replayed(HD):
 
 
 @gpu
+@pytest.mark.parametrize("options", [None, GENERAL], ids=["chosen", "general"])
+@pytest.mark.parametrize("shape", ["decode", "rows"])
+@pytest.mark.parametrize("pool", [None, wl.E4M3], ids=["16-bit", "e4m3"])
+def test_a_padded_block_table(pool, shape, options):
+    """Table entries that no tile reads may hold anything, NaN codes behind P are never mixed in."""
+    w = wl.make_pass("padded", 12, [(37, 1), (250, 1)] if shape == "decode" else [(37, 5), (250, 3)], 8, 2, 128, 16, wl.F16, pool, scale=0.125)
+    w.blocks = np.concatenate([w.blocks, np.array([-1, -7, w.n_blocks, 2 ** 30, -1], dtype=np.int32)])
+    if pool == wl.E4M3:
+        kv = w.kv.reshape(w.n_blocks, 2, w.bt, w.kv_ld)
+        for t in w.trees:
+            kv[w.blocks[int(t["table"]) + int(t["P"]) // w.bt], :, int(t["P"]) % w.bt:] = 0x7F
+    _check(w, options=options)
+
+
+@gpu
+def test_check_finite_scans_these_passes():
+    w = wl.make_pass("finite", 13, [(200, 1), (100, 1)], 8, 2, 128, 16, wl.BF16, scale=0.125)
+    w.kv.reshape(w.n_blocks, 2, w.bt, w.kv_ld)[int(w.blocks[int(w.trees[1]["table"])]), 1, 3, 5] = 0x7FC0
+    lam, nw = _weights(w, 1)
+    _launch(w, lam, nw)
+    with pytest.raises(capi.EspError, match="row 1, column 0"):  # the norm carries it into the whole head
+        _launch(w, lam, nw, options=dict(check_finite=1))
+
+
+@gpu
+def test_two_passes_of_one_context_at_once():
+    """Split passes that share a context, eagerly on two streams and as two graphs: each gives the bits it gives alone."""
+    ws = [wl.make_pass("left", 14, [(3000, 40)], 8, 2, 128, 16, wl.F16, wl.E4M3, scale=0.125), wl.make_pass("right", 15, [(2500, 24), (40, 3)], 8, 2, 128, 16, wl.F16, wl.E4M3, scale=0.125)]
+    op = host.AttnOp.for_workload(ws[0], 32)
+    calls, outs, want = [], [], []
+    for i, w in enumerate(ws):
+        lam, nw = _weights(w, i)
+        dp = op.upload(w)
+        O = torch.zeros((w.n_rows, w.q_ld), dtype=torch.int16, device=op.device)
+        plan = host.plan_tiles(w.trees, w.Hkv, **dict(host.diff_plan_options(w.trees, w.H, w.Hkv, w.HD, w.kv_dtype)[1], split=300, groups=64))
+        assert plan.n_parts
+        calls.append(op.diff_call(plan, w.trees, dp.Q, dp.Kb, dp.Vb, O, kv=dp.kv, kv_scales=dp.kv_scales, blocks=dp.blocks, n_blocks=w.n_blocks, desc=dp.desc,
+                                  lam=torch.from_numpy(lam).cuda(), norm_w=torch.from_numpy(nw).cuda(), eps=EPS, out_scale=SCALE))
+        op.diff_forward(calls[i])
+        torch.cuda.synchronize()
+        outs.append(O), want.append(O.clone())
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    graphs = []
+    for c in calls:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            op.diff_forward(c)
+    for turn in range(4):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for _ in range(5):
+            for s, c, g in zip(streams, calls, graphs):
+                with torch.cuda.stream(s):
+                    g.replay() if turn % 2 else op.diff_forward(c)
+        torch.cuda.synchronize()
+        for o, x in zip(outs, want):
+            assert torch.equal(o, x)
+    op.check_status()
+    op.close()
+
+
+@gpu
+def test_rows_with_other_strides_are_refused():
+    w = wl.make_pass("strides", 16, [(0, 4)], 8, 2, 128, 16, wl.F16, scale=0.125)
+    op = host.AttnOp.for_workload(w, 8)
+    dp = op.upload(w)
+    plan = host.plan_tiles(w.trees, w.Hkv)
+    wide = torch.zeros((4, 2 * w.q_ld), dtype=torch.int16, device=op.device)
+    good = dict(Q=dp.Q, Kb=dp.Kb, Vb=dp.Vb, O=torch.zeros_like(dp.Q), desc=dp.desc, lam=torch.zeros(8, device=op.device))
+    for name, t in (("Kb", wide[:, :w.kv_ld]), ("Vb", wide[:, :w.kv_ld]), ("O", wide[:, :w.q_ld]), ("Q", wide[:, ::2])):
+        with pytest.raises(ValueError, match=name):
+            op.diff_call(plan, w.trees, **dict(good, **{name: t}))
+    for name, t in (("Kb", wide[:, :w.kv_ld]), ("K", wide[:, :2 * w.kv_ld:2])):
+        with pytest.raises(ValueError, match=name):
+            op.append_call(**dict(dict(Q=dp.Q, K=dp.Kb, V=dp.Vb, Qo=dp.Q, Kb=dp.Kb, Vb=dp.Vb), **{name: t}))
+    op.close()
+
+
+@gpu
 @pytest.mark.parametrize("H,dim", [(1, 1), (32, 64), (7, 129)])
 def test_lambda(H, dim):
     rng = np.random.default_rng(H)

@@ -69,7 +69,7 @@ constexpr int kSlots = 4;
 static_assert(kSlots >= KS + 2, "page scales must outlive their readers");
 template <int VS>
 struct Shared {
-  uint64_t q_full, k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], s_full[2], p_full[2][2], o_done[2], sc_full[kSlots], m_ready[2];
+  uint64_t q_full, k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], s_full[2], p_full[2][2], o_done[2], sc_full[kSlots], m_ready[2], take_full;
   uint32_t tmem;
   volatile int dead;
   float k_scale[kSlots][kPages], v_scale[kSlots][kPages];
@@ -86,8 +86,9 @@ __device__ __forceinline__ uint32_t peer_addr(const void* p, uint32_t rank) {
   return r;
 }
 __device__ __forceinline__ void peer_store(uint32_t addr, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory"); }
-__device__ __forceinline__ void peer_store4(uint32_t addr, float x, float y, float z, float w) {
-  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(x), "f"(y), "f"(z), "f"(w) : "memory");
+// Asynchronous copy into the peer's shared memory; its barrier counts the bytes.
+__device__ __forceinline__ void peer_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "r"(smem_u32(src)), "r"(bytes), "r"(bar) : "memory");
 }
 
 template <int HD, int QDT, bool F8>
@@ -118,6 +119,7 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
       mbar_init(&sh.m_ready[i], 4);
     }
     for (int s = 0; s < kSlots; ++s) mbar_init(&sh.sc_full[s], 1);
+    mbar_init(&sh.take_full, 1);
     mbar_fence_init();
     sh.dead = 0;
   }
@@ -277,7 +279,7 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
         }
       }
     }
-    if (whole_rows) cluster_sync(), cluster_sync(), cluster_sync();  // the softmax warps' epilogue
+    if (whole_rows) cluster_sync(), cluster_sync();  // the softmax warps' epilogue
   } else {
     if constexpr (C::HOLD) regs_inc<kRegsSoftmax>();
     const int wg = tid >> 7, srow = tid & (BM - 1), fm = srow / HPC, head = int(blockIdx.y) * HPC + srow % HPC, wq = warp & 3;
@@ -453,6 +455,7 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
         for (int i = 0; i < 32; ++i) v[i] = 0.0f;
       }
     };
+    const int head0 = int(blockIdx.y) * HPC;
     if (!whole_rows) {
       float* rec = a.parts + diff_record(a, tile.part, kvh, fm, head % G, map);
 #pragma unroll 1
@@ -466,22 +469,28 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
       }
       if (row_ok && wg == 0) *reinterpret_cast<float2*>(rec + HD) = make_float2(m_fin * kLn2, l);
     } else {
-      constexpr int MINE = HD / 4;  // columns a thread finishes: CTA `map` has [map HD / 2, ..), group wg half of those
-      float* take = reinterpret_cast<float*>(v_sm);         // [HD / 8][128 rows][4 columns], lanes side by side; written by the peer
+      constexpr int MINE = HD / 4;               // columns a thread finishes: CTA `map` has [map HD / 2, ..), group wg half of those
+      constexpr int HALF = C::MAP * BM * 4;      // bytes that change sides
+      static_assert(2 * HALF <= VS * C::V_SLOT, "give and take lie in the V ring");
+      uint8_t* give = v_sm;                                 // [HD / 8][128 rows][4 columns], lanes side by side
+      float* take = reinterpret_cast<float*>(v_sm + HALF);  // the same, written by the peer
       float* sq = reinterpret_cast<float*>(q_sm);           // [CTA * 2 + group][128 rows]: the rows' sums of squares; written by both
       const float inv = l > 0.0f ? (map ? -diff_lam(args, row, head) : 1.0f) * v_ref / l : 0.0f;
       // the norm's weights into shared memory while the peer gets here (16-byte aligned, HD floats)
       float* w_sm = reinterpret_cast<float*>(k_sm) + 2 * BM;
       if (args.norm_w && tid < HD / 4) reinterpret_cast<float4*>(w_sm)[tid] = reinterpret_cast<const float4*>(args.norm_w)[tid];
-      cluster_sync();  // neither CTA uses its tiles any more
-      const uint32_t peer_take = peer_addr(take, uint32_t(map ^ 1)) + uint32_t((wg * (MINE / 4) * BM + srow) * 16);
+      if (tid == 0) mbar_arrive_expect_tx(&sh.take_full, HALF);
 #pragma unroll 1
       for (int q = 0; q < MINE / 32; ++q) {
         float v[32];
         load_o((map ^ 1) * C::MAP + wg * MINE + 32 * q, v);
 #pragma unroll
-        for (int i = 0; i < 32; i += 4) peer_store4(peer_take + uint32_t((8 * q + i / 4) * BM * 16), v[i] * inv, v[i + 1] * inv, v[i + 2] * inv, v[i + 3] * inv);
+        for (int i = 0; i < 32; i += 4)
+          reinterpret_cast<float4*>(give)[(wg * (MINE / 4) + 8 * q + i / 4) * BM + srow] = make_float4(v[i] * inv, v[i + 1] * inv, v[i + 2] * inv, v[i + 3] * inv);
       }
+      fence_proxy_async_smem();
+      cluster_sync();  // both halves lie ready, neither CTA uses its tiles any more
+      if (tid == 0) peer_copy(peer_addr(take, uint32_t(map ^ 1)), give, HALF, peer_addr(&sh.take_full, uint32_t(map ^ 1)));
       float dv[MINE];
 #pragma unroll
       for (int q = 0; q < MINE / 32; ++q) {
@@ -490,7 +499,7 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
 #pragma unroll
         for (int i = 0; i < 32; ++i) dv[32 * q + i] = v[i] * inv;
       }
-      cluster_sync();  // the peer's half has arrived
+      wait_bar(&sh.take_full, 0, kStatusMmaTimeout);
       float ss = 0.0f;
 #pragma unroll
       for (int i = 0; i < MINE; i += 4) {
@@ -501,24 +510,30 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
       }
       sq[(map * 2 + wg) * BM + srow] = ss;
       peer_store(peer_addr(sq, uint32_t(map ^ 1)) + uint32_t(((map * 2 + wg) * BM + srow) * 4), ss);
-      cluster_sync();
+      cluster_sync();  // and both copies have been received
       ss = sq[srow] + sq[BM + srow] + sq[2 * BM + srow] + sq[3 * BM + srow];  // the same order in both CTAs
       const float f = diff_row_factor(args, ss, HD);
-      if (row_ok) {
-        const int col = map * C::MAP + wg * MINE;
-        typename QE::T* op = static_cast<typename QE::T*>(a.O) + size_t(row) * p.q_ld + size_t(head) * HD + col;
-        const float* w = w_sm + col;  // every lane reads the same word
+      // The rows leave through shared memory, HD / 2 columns of a row side by side.
+      constexpr int PIECES = C::MAP / 8;  // of 16 bytes in a row, swizzled by row
+      uint4* rows = reinterpret_cast<uint4*>(k_sm + C::K_TILE);
+      const float* w = w_sm + map * C::MAP + wg * MINE;  // every lane reads the same word
 #pragma unroll
-        for (int i = 0; i < MINE; i += 8) {
-          float x[8];
+      for (int i = 0; i < MINE; i += 8) {
+        float x[8];
 #pragma unroll
-          for (int k = 0; k < 8; ++k) x[k] = dv[i + k] * f;
-          if (args.norm_w) {
-            const float4 w0 = *reinterpret_cast<const float4*>(w + i), w1 = *reinterpret_cast<const float4*>(w + i + 4);
-            x[0] *= w0.x, x[1] *= w0.y, x[2] *= w0.z, x[3] *= w0.w, x[4] *= w1.x, x[5] *= w1.y, x[6] *= w1.z, x[7] *= w1.w;
-          }
-          *reinterpret_cast<uint4*>(op + i) = make_uint4(QE::pack2(x[0], x[1]), QE::pack2(x[2], x[3]), QE::pack2(x[4], x[5]), QE::pack2(x[6], x[7]));
+        for (int k = 0; k < 8; ++k) x[k] = dv[i + k] * f;
+        if (args.norm_w) {
+          const float4 w0 = *reinterpret_cast<const float4*>(w + i), w1 = *reinterpret_cast<const float4*>(w + i + 4);
+          x[0] *= w0.x, x[1] *= w0.y, x[2] *= w0.z, x[3] *= w0.w, x[4] *= w1.x, x[5] *= w1.y, x[6] *= w1.z, x[7] *= w1.w;
         }
+        rows[srow * PIECES + ((wg * (MINE / 8) + i / 8) ^ (srow & 7))] = make_uint4(QE::pack2(x[0], x[1]), QE::pack2(x[2], x[3]), QE::pack2(x[4], x[5]), QE::pack2(x[6], x[7]));
+      }
+      named_barrier(2, kSoftmax);
+      typename QE::T* out = static_cast<typename QE::T*>(a.O) + size_t(tile.r0) * p.q_ld + size_t(head0) * HD + map * C::MAP;
+#pragma unroll 4
+      for (int i = tid; i < BM * PIECES; i += kSoftmax) {
+        const int r = i / PIECES, c = i % PIECES;
+        if (r / HPC < rows_live) *reinterpret_cast<uint4*>(out + size_t(r / HPC) * p.q_ld + size_t(r % HPC) * HD + 8 * c) = rows[r * PIECES + (c ^ (r & 7))];
       }
     }
   }

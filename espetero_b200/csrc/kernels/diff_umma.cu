@@ -126,10 +126,12 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
   __syncthreads();
   pdl_wait();  // the plan, Q and the mask records belong to the stream's order
 
-  const esp_attn_tile tile = a.tiles[int(gridDim.x) - 1 - int(blockIdx.x)];  // long (late) tiles first
+  // Long (late) tiles first, a tile's heads side by side: what runs last is short.
+  const int G = a.G, TR = a.tile_rows, HPC = BM / TR, groups = p.H / HPC;
+  const esp_attn_tile tile = a.tiles[a.n_tiles - 1 - int(blockIdx.x) / groups];
   const esp_attn_tree tree = a.trees[tile.tree];
-  const int G = a.G, TR = a.tile_rows, HPC = BM / TR;
-  const int kvh = (int(blockIdx.y) * HPC) / G;
+  const int head0 = (int(blockIdx.x) % groups) * HPC;  // the tile's heads, all of one kv head
+  const int kvh = head0 / G;
   const int end = tree.base + tree.M, rows_live = min(TR, end - tile.r0);
   const BlockList L = block_list(a, tile, tree, rows_live, lane);
   const int nb = L.n(), N = nb * C::UPB;
@@ -168,7 +170,7 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
       if (!is_v && TR == BM && N > 0 && lane == 0) {  // a tile of one head: its Q rows are contiguous, too
         mbar_arrive_expect_tx(&sh.q_full, C::K_TILE);
 #pragma unroll
-        for (int i = 0; i < C::QC; ++i) tma_load_3d(q_sm + i * C::CHUNK, &q_map, &sh.q_full, 0, tile.r0, int(blockIdx.y) * C::VC + map * C::QC + i);
+        for (int i = 0; i < C::QC; ++i) tma_load_3d(q_sm + i * C::CHUNK, &q_map, &sh.q_full, 0, tile.r0, head0 * C::VC + map * C::QC + i);
       }
       __syncwarp();
       walk_pages<F8>(
@@ -282,7 +284,7 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
     if (whole_rows) cluster_sync(), cluster_sync();  // the softmax warps' epilogue
   } else {
     if constexpr (C::HOLD) regs_inc<kRegsSoftmax>();
-    const int wg = tid >> 7, srow = tid & (BM - 1), fm = srow / HPC, head = int(blockIdx.y) * HPC + srow % HPC, wq = warp & 3;
+    const int wg = tid >> 7, srow = tid & (BM - 1), fm = srow / HPC, head = head0 + srow % HPC, wq = warp & 3;
     const bool row_ok = fm < rows_live;
     const int row = row_ok ? tile.r0 + fm : end - 1, rr = row - tree.base;
     int4 dsc = make_int4(0, 0, 0, 0);
@@ -455,7 +457,6 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
         for (int i = 0; i < 32; ++i) v[i] = 0.0f;
       }
     };
-    const int head0 = int(blockIdx.y) * HPC;
     if (!whole_rows) {
       float* rec = a.parts + diff_record(a, tile.part, kvh, fm, head % G, map);
 #pragma unroll 1
@@ -560,7 +561,7 @@ cudaError_t launch_hd(const DiffArgs& a, bool f8, const CUtensorMap& pool_map, c
   auto kernel = f8 ? (f16 ? diff_umma_kernel<HD, ESP_F16, true> : diff_umma_kernel<HD, ESP_BF16, true>)
                    : (f16 ? diff_umma_kernel<HD, ESP_F16, false> : diff_umma_kernel<HD, ESP_BF16, false>);
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(a.k.n_tiles), unsigned(a.k.p.H / (BM / a.k.tile_rows)), 2), cfg.blockDim = dim3(kThreads);
+  cfg.gridDim = dim3(unsigned(a.k.n_tiles) * unsigned(a.k.p.H / (BM / a.k.tile_rows)), 1, 2), cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = Geo<HD>::SMEM, cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -16,7 +16,7 @@
 // it forms its 4 or 8 sines and cosines once, in registers, addresses advance by a constant, and nothing is shared between warps.
 // 8192 rows of H32 / Hkv4 / HD128, fp16: 34.4 us = 5.37 TB/s = 0.82 of the copy peak (71.7 us with a table of sines per CTA and items
 // dealt out by division, which left the instruction issue and the CTAs' trips to memory in charge); 5001 fp32 rows of H16 / Hkv2 / HD256:
-// 34.4 us = 4.77 TB/s. kBatch items are asked for before the first is turned: 2 at three CTAs per SM; 4 and 8 measured 36.6 and 41.2 us, 1
+// 33.1 us = 4.95 TB/s. kBatch items are asked for before the first is turned: 2 at 24 warps per SM; 4 and 8 measured 36.6 and 41.2 us, 1
 // 43.0.
 // An item's reads precede its own writes and no other item touches its bytes, so outputs may lie over the sources.
 #include <type_traits>
@@ -27,7 +27,7 @@
 namespace esp {
 namespace {
 
-constexpr int kWarps = 8, kThreads = 32 * kWarps;
+constexpr int kWarps = 4, kThreads = 32 * kWarps;  // small CTAs: their slots free up one by one (with 8 warps 3 to 5 % slower past one wave)
 constexpr int kBatch = 2;  // items a lane asks for at once
 
 __device__ __forceinline__ float2 turn_of(int pos, float inv_freq) {
@@ -73,7 +73,7 @@ struct Raw<false> {
 };
 
 template <int QDT, bool SRC32, bool FP8_POOL, bool ADJ>
-__global__ void __launch_bounds__(kThreads, 3) kv_append_kernel(const AppendArgs args, const Steps st, const int HD) {
+__global__ void __launch_bounds__(kThreads, 6) kv_append_kernel(const AppendArgs args, const Steps st, const int HD) {
   using QE = Elem16<QDT>;
   using T = typename QE::T;
   using S = std::conditional_t<SRC32, float, T>;
@@ -298,7 +298,7 @@ cudaError_t launch_typed(const AppendArgs& args, int32_t HD, cudaStream_t stream
   // One and a bit times the warps that the SMs hold would leave them half empty the second time: such rows are halved. (5001 fp32 rows of
   // H16 / Hkv2 / HD256: 36.8 -> 34.4 us. Elsewhere the sines formed twice cost more: 3000 rows 13.9 -> 15.0 us, 6000 67.1 -> 72.2, 8192 34.5 ->
   // 35.9.)
-  const int64_t wave = 148 * 3 * kWarps;
+  const int64_t wave = 148 * 6 * kWarps;
   if (a.rows > wave && 2 * int64_t(a.rows) <= 3 * wave) st.parts = std::min(2, steps);
   st.per_part = (steps + st.parts - 1) / st.parts;
   st.parts = (steps + st.per_part - 1) / st.per_part;

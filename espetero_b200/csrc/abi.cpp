@@ -1229,40 +1229,47 @@ int esp_diff_plan_opts(const esp_attn_shape* s, const esp_attn_tree* trees, int3
     o->tile_rows = 8, o->groups = 148 * std::max(1, std::min(3, 512 / row_bytes)), o->split = 1 << 20, o->min_chunk = 64;
     return ESP_OK;
   }
-  if (cached <= 2 * fresh) {  // mostly its own rows: 128-row tiles, one head each, nothing split
-    o->tile_rows = 128, o->groups = 148, o->split = 0;
-    return ESP_OK;
-  }
-  int c = 8;  // heads per tile
-  while (c > 1 && (c > G || G % c)) c >>= 1;
-  o->tile_rows = 128 / c;
-  // How far to split the cached keys, by the time each choice would take: CTAs (two per tile and head group) on the SMs' slots, a
-  // fixed cost per CTA and one per 128 keys, and the join of the records. Microseconds, measured on diff_umma; with 128-dim heads two
-  // CTAs share an SM and each runs slower than alone. 700 rows behind 20001 keys, 8 kv heads, took 525 us unsplit, 484 in two, 515 in
-  // three and 533 in four parts; the rule gives 523, 475, 506 and 532.
-  const bool wide = s->HD >= 256;
-  const int per_tile = s->Hkv * (G / c) * 2;
-  const double t_alone = wide ? 1.45 : 1.2, t_shared = 1.9, t_fixed = 9.0;  // per 128 keys alone / sharing an SM; start and end of a CTA
+  // diff_umma: how many heads of a kv head share a tile, and - where cached keys are most of the work - how far to split them, by the
+  // time each choice would take: CTAs (two per tile and head group) on the SMs' slots, a fixed cost per CTA and one per 128 keys,
+  // and the join of the records. Microseconds, measured; with 128-dim heads two CTAs share an SM and each runs slower than
+  // alone. 700 rows behind 20001 keys, 8 kv heads, took 525 us unsplit, 484 in two, 515 in three and 533 in four parts; the rule
+  // gives 523, 475, 506 and 532. Small prompts share their tiles between heads: 4 x 33 rows, 256 dims, 24.5 us in tiles of one head, 13.0 of two;
+  // 8 x 20 .. 100 rows, 128 dims, 24.2 us of one, 21.0 of two, 13.8 of four. Near ties keep taller tiles and fewer parts.
+  const bool wide = s->HD >= 256, split = cached > 2 * fresh;
+  const double t_alone = wide ? 1.45 : 1.2, t_shared = wide ? 1.45 : 1.9, t_fixed = 9.0;  // per 128 keys alone / sharing an SM; start and end of a CTA
+  const int64_t slots = wide ? 148 : 296;
   double best = 0;
-  for (int parts = 1; parts <= 32; ++parts) {
-    int64_t tiles = 0, rows_split = 0;
-    int longest = 0;
-    for (int i = 0; i < n_trees; ++i) {
-      const int64_t groups = (trees[i].M + o->tile_rows - 1) / o->tile_rows;
-      const int ns = trees[i].P >= 64 ? std::min(parts, std::max(1, trees[i].P / 128)) : 1;
-      tiles += groups * ns;
-      if (ns > 1) rows_split += int64_t(trees[i].M) * ns;
-      longest = std::max(longest, (trees[i].P / ns + 127) / 128 + (ns == 1 ? (std::min(trees[i].M, 1 << 20) + 127) / 128 : 1));
-    }
-    const int64_t ctas = tiles * per_tile, slots = wide ? 148 : 296, rest = ctas % slots;
-    double t = double(ctas / slots) * (longest * (wide ? t_alone : t_shared) + t_fixed);
-    if (rest) t += longest * (rest <= 148 ? t_alone : t_shared) + t_fixed;
-    if (rows_split) t += 6.0 + double(rows_split) * s->H * 2 * (s->HD + 2) * 4 * 2 / 6.0e6;  // written and read at about 6 TB/s, mostly in L2
-    if (parts == 1 || t < 0.97 * best) {
-      best = t;
-      // the planner sizes its chunks so that the tiles fit `groups / Hkv`
-      o->split = parts == 1 ? 0 : 1 << 20;
-      o->groups = int(std::min<int64_t>(tiles, 1 << 24)) * s->Hkv;
+  o->tile_rows = 0;
+  for (int TR = 128; TR >= 16; TR >>= 1) {
+    const int c = 128 / TR;
+    if (c > G || G % c) continue;
+    for (int parts = 1; parts <= (split ? 32 : 1); ++parts) {
+      int64_t tiles = 0, blocks = 0, rows_split = 0, longest = 0;
+      for (int i = 0; i < n_trees; ++i) {
+        const esp_attn_tree& t = trees[i];
+        const int64_t groups = (t.M + TR - 1) / TR, own = (int64_t(t.M) + 127) / 128;
+        const int ns = split && t.P >= 64 ? std::min(parts, std::max(1, t.P / 128)) : 1;
+        const int64_t part = (t.P / ns + 127) / 128;
+        tiles += groups * ns;
+        blocks += groups * ns * part + groups * (own + 1) / 2;  // its own rows: a triangle
+        if (ns > 1) rows_split += int64_t(t.M) * ns;
+        longest = std::max(longest, part + (ns == 1 ? own : 1));
+      }
+      const int64_t ctas = tiles * (s->H / c) * 2, rest = ctas % slots;
+      double t;
+      if (4 * longest * tiles <= 5 * blocks) {  // tiles of one length: wave by wave
+        t = double(ctas / slots) * (double(longest) * t_shared + t_fixed);
+        if (rest) t += double(longest) * (rest <= 148 ? t_alone : t_shared) + t_fixed;
+      } else {
+        t = (double(blocks) * (s->H / c) * 2 * t_shared + double(ctas) * t_fixed) / double(slots) + 0.5 * double(longest) * t_alone + t_fixed;
+      }
+      if (rows_split) t += 6.0 + double(rows_split) * s->H * 2 * (s->HD + 2) * 4 * 2 / 6.0e6;  // written and read at about 6 TB/s, mostly in L2
+      if (o->tile_rows && t > 1.5 * best) break;
+      if (!o->tile_rows || t < 0.97 * best) {
+        best = t;
+        // the planner sizes its chunks so that the tiles fit `groups / Hkv`
+        o->tile_rows = TR, o->split = parts == 1 ? 0 : 1 << 20, o->groups = int(std::clamp<int64_t>(tiles, 1, 1 << 24)) * s->Hkv;
+      }
     }
   }
   return ESP_OK;

@@ -41,8 +41,8 @@ __device__ __forceinline__ void tmem_wait_ld_of(uint32_t (&r)[32]) {
 }
 
 // MMA issue by a whole converged warp, of which one lane (`one` = 1) issues. The warp's loop counters and descriptors then stay in
-// uniform registers; a loop that only one lane runs spends about 100 clocks per instruction group on moving them there, more than
-// the tensor pipe takes (3794 against 3411 clocks per 128 keys in diff_umma).
+// uniform registers; a loop that only one lane runs spends about 100 clocks per instruction group on moving them there: a tenth of
+// diff_umma's loop when it was measured.
 __device__ __forceinline__ uint32_t elect_one() {
   uint32_t one;
   asm volatile(

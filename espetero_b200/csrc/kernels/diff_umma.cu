@@ -19,6 +19,14 @@
 //
 // Bound per 128 keys of a tile: 256-dim heads 1536 clocks of MMA per map (8 instructions of N = 128 and 8 of N = 256, 64 and 128
 // clocks each) on an SM, 1024 of exponentials; 128-dim heads 1024 of exponentials per map, two maps per SM, against 1600 of MMA.
+// Measured, causal rows of 16 heads: 128 dims, 4096 rows 129 us (797 TFLOP/s), 8192 rows 421 us (979); 256 dims 199 us (1035) and 655 us
+// (1260). 256-dim heads run at 1800 clocks a unit, 85 % of the MMA bound, but one CTA per SM hides nothing of a CTA's start and end:
+// 6 k clocks until the first scores (plan, masks and page table, one dependent load after another), 14 k for the last P . V, the
+// exchange of halves (64 KB each way at 21 bytes a clock) and the output. 128-dim heads hide that under the SM's other CTA; there the
+// exponentials' pipe is 54 % busy and the issue slots 53 %: a warp's chain of load, maximum, exponentials and store is what four
+// warps per scheduler do not cover. Dropped: both maps in one CTA, a warpgroup each, K and V loaded once (2 x 8192 rows, H16: 953 us
+// against 880; with the next scores fetched ahead 1009), turns between the maps by barrier (970), exponentials by polynomial on the FMA
+// pipe (equal or slower).
 // Warps 0-7 softmax, 8 MMA issue (owns tensor memory), 9 / 10 K / V producers (TMA, one load per 16-key page and 64-dim chunk of the pool,
 // one per 64 or 128 rows of the batch; the Q tile, too, where it is 128 rows of one head), 11 idle (it
 // completes the warpgroup that hands registers over). Hand-offs by mbarrier; every wait is bounded: after a timeout the CTA records a

@@ -403,7 +403,7 @@ def test_two_passes_of_one_context_at_once():
         lam, nw = _weights(w, i)
         dp = op.upload(w)
         O = torch.zeros((w.n_rows, w.q_ld), dtype=torch.int16, device=op.device)
-        plan = host.plan_tiles(w.trees, w.Hkv, **dict(host.diff_plan_options(w.trees, w.H, w.Hkv, w.HD, w.kv_dtype)[1], split=300, groups=64))
+        plan = host.plan_tiles(w.trees, w.Hkv, **dict(host.diff_plan_options(w.trees, w.H, w.Hkv, w.HD, w.kv_dtype)[1], tile_rows=32, split=300, groups=64))
         assert plan.n_parts
         calls.append(op.diff_call(plan, w.trees, dp.Q, dp.Kb, dp.Vb, O, kv=dp.kv, kv_scales=dp.kv_scales, blocks=dp.blocks, n_blocks=w.n_blocks, desc=dp.desc,
                                   lam=torch.from_numpy(lam).cuda(), norm_w=torch.from_numpy(nw).cuda(), eps=EPS, out_scale=SCALE))

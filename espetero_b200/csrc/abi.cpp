@@ -1297,6 +1297,7 @@ int esp_diff_forward(esp_attn_ctx* c, void* stream, const esp_attn_args* ap, con
   k.p = a.p, k.HD = s.HD, k.G = c->G, k.tile_rows = c->tile_rows, k.n_tiles = a.n_tiles;
   k.q_dtype = s.q_dtype, k.kv_dtype = s.kv_dtype, k.n_blocks = a.n_blocks, k.scale = s.scale;
   k.n_trees = a.n_trees, k.n_block_entries = a.n_block_entries;
+  d.n_rows = a.n_rows;
   d.lam = dp->lam, d.norm_w = dp->norm_w, d.lam_ld = dp->lam_ld, d.eps = dp->eps, d.out_scale = dp->out_scale;
 
   bool single = a.trees_host != nullptr && a.tiles_host != nullptr;

@@ -131,12 +131,26 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
     mbar_fence_init();
     sh.dead = 0;
   }
+  // While the kernel before this one drains: the lines that the first steps read, one address after another, are brought into L2, every
+  // index checked. A stale plan costs a wasted hint, never a result.
+  const int groups = p.H / (BM / a.tile_rows);
+  const esp_attn_tile* my_tile = a.tiles + (a.n_tiles - 1 - int(blockIdx.x) / groups);
+  if (warp == kWarpK) {
+    const int4 t0 = __ldcg(reinterpret_cast<const int4*>(my_tile));  // tree, r0, k0, k1
+    if (t0.x >= 0 && t0.x < a.n_trees) {
+      const int4 tr = __ldcg(reinterpret_cast<const int4*>(a.trees + t0.x));  // base, P, table, M
+      const long long row = (long long)t0.y + lane * 8;  // eight records to a line
+      if (a.desc && t0.y >= 0 && lane * 8 < a.tile_rows && row < args.n_rows) prefetch_l2(a.desc + 4 * row);
+      const long long at = (long long)tr.z + t0.z / p.bt + lane * 32;
+      if (a.blocks && tr.z >= 0 && t0.z >= 0 && t0.z + lane * 32 * p.bt < t0.w && at < a.n_block_entries) prefetch_l2(a.blocks + at);
+    }
+  }
   __syncthreads();
   pdl_wait();  // the plan, Q and the mask records belong to the stream's order
 
   // Long (late) tiles first, a tile's heads side by side: what runs last is short.
-  const int G = a.G, TR = a.tile_rows, HPC = BM / TR, groups = p.H / HPC;
-  const esp_attn_tile tile = a.tiles[a.n_tiles - 1 - int(blockIdx.x) / groups];
+  const int G = a.G, TR = a.tile_rows, HPC = BM / TR;
+  const esp_attn_tile tile = *my_tile;
   const esp_attn_tree tree = a.trees[tile.tree];
   const int head0 = (int(blockIdx.x) % groups) * HPC;  // the tile's heads, all of one kv head
   const int kvh = head0 / G;
@@ -440,6 +454,10 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
 
     // ---- epilogue
     pdl_launch_dependents();
+    // what the finish needs of memory, asked for before the waits
+    const float lam = whole_rows && map ? diff_lam(args, row, head) : 0.0f;
+    float4 w4 = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (whole_rows && args.norm_w && tid < HD / 4) w4 = reinterpret_cast<const float4*>(args.norm_w)[tid];
     named_barrier(2, kSoftmax);  // both groups are through: the reference is final, and all but the last two P . V are known to be done
     float m_fin = -INFINITY, v_ref = 1.0f;
     if (N > 0) {
@@ -484,10 +502,9 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
       uint8_t* give = v_sm;                                 // [HD / 8][128 rows][4 columns], lanes side by side
       float* take = reinterpret_cast<float*>(v_sm + HALF);  // the same, written by the peer
       float* sq = reinterpret_cast<float*>(q_sm);           // [CTA * 2 + group][128 rows]: the rows' sums of squares; written by both
-      const float inv = l > 0.0f ? (map ? -diff_lam(args, row, head) : 1.0f) * v_ref / l : 0.0f;
-      // the norm's weights into shared memory while the peer gets here (16-byte aligned, HD floats)
-      float* w_sm = reinterpret_cast<float*>(k_sm) + 2 * BM;
-      if (args.norm_w && tid < HD / 4) reinterpret_cast<float4*>(w_sm)[tid] = reinterpret_cast<const float4*>(args.norm_w)[tid];
+      const float inv = l > 0.0f ? (map ? -lam : 1.0f) * v_ref / l : 0.0f;
+      float* w_sm = reinterpret_cast<float*>(k_sm) + 2 * BM;  // the norm's weights
+      if (args.norm_w && tid < HD / 4) reinterpret_cast<float4*>(w_sm)[tid] = w4;
       if (tid == 0) mbar_arrive_expect_tx(&sh.take_full, HALF);
 #pragma unroll 1
       for (int q = 0; q < MINE / 32; ++q) {

@@ -213,6 +213,7 @@ struct DiffArgs {
   const float* norm_w;
   int32_t lam_ld;
   float eps, out_scale;
+  int32_t n_rows;        // of the pass
 };
 struct DiffCombineArgs {
   DiffArgs d;

@@ -12,8 +12,8 @@
 // V and K arrive by TMA (two bulk tensor loads per block, 128-byte swizzle, rows through the page table) in rings that belong to
 // single warps, so nothing in the loop waits for another warp. Softmax in the exp2 domain over the key lanes; P^T re-enters as the
 // B operand (movmatrix), rounded to 16 bits: what the MMA takes; sums and the rows' totals stay fp32 and unrounded. E4M3 codes
-// are widened to fp16 in registers (exact), the K scale goes on the score, the V scale on p (in units that
-// follow the largest scale, so that p stays in fp16's range).
+// are widened to fp16 in registers (exact), the K scale goes on the score, the V scale on the block's P . V:
+// p is rounded as it is, and the largest, 1, exactly.
 // All waits are bounded; a CTA that gives up writes empty records and says so in the status word.
 #include "diff.cuh"
 
@@ -152,7 +152,6 @@ __global__ void __launch_bounds__(C::NW * 32, C::CTAS) diff_decode_kernel(const 
 #pragma unroll
     for (int i = 0; i < NMT; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.0f;
   }
-  float v_ref = C::FP8 ? 0.0f : 1.0f;
   const int mi = lane >> 3, rj = lane & 7;
   const uint32_t key_k = rj + 8 * (mi & 1), sel_k = mi >> 1;  // K: ldmatrix
   const uint32_t key_v = rj + 8 * (mi >> 1), sel_v = mi & 1;  // V: ldmatrix.trans
@@ -227,16 +226,6 @@ __global__ void __launch_bounds__(C::NW * 32, C::CTAS) diff_decode_kernel(const 
     const bool out_lo = g >= n_valid || g < n_skip, out_hi = g + 8 >= n_valid || g + 8 < n_skip;
     uint32_t pb[NT][2];
     float corr[NT][2];
-    // E4M3: O is summed in units of the largest V scale's power of two so far, so p times its page's scale stays in fp16's range
-    float vfac = 1.0f;
-    if constexpr (C::FP8) {
-      if (!(vscale <= v_ref)) {  // uniform over the warp
-        const float now = __uint_as_float(__float_as_uint(fminf(fmaxf(vscale, 1.17549435e-38f), 1.0e38f)) & 0x7F800000u);
-        vfac = v_ref > 0.0f ? v_ref * __uint_as_float(0x7F000000u - __float_as_uint(now)) : 1.0f;
-        v_ref = now;
-      }
-      vscale *= __uint_as_float(0x7F000000u - __float_as_uint(v_ref));
-    }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       // lane: (key g, columns 2t, 2t + 1), (key g + 8, the same)
@@ -256,9 +245,8 @@ __global__ void __launch_bounds__(C::NW * 32, C::CTAS) diff_decode_kernel(const 
       l[n][0] = fmaf(l[n][0], corr[n][0], p0 + p2);
       l[n][1] = fmaf(l[n][1], corr[n][1], p1 + p3);
       m[n][0] = n0, m[n][1] = n1;
-      if constexpr (C::FP8) corr[n][0] *= vfac, corr[n][1] *= vfac;
-      pb[n][0] = movmatrix_trans(CE::pack2(p0 * vscale, p1 * vscale));
-      pb[n][1] = movmatrix_trans(CE::pack2(p2 * vscale, p3 * vscale));
+      pb[n][0] = movmatrix_trans(CE::pack2(p0, p1));
+      pb[n][1] = movmatrix_trans(CE::pack2(p2, p3));
     }
 
     // ---- O^T = O^T * corr + V^T . P^T
@@ -275,6 +263,16 @@ __global__ void __launch_bounds__(C::NW * 32, C::CTAS) diff_decode_kernel(const 
         }
       }
     } else {
+      // A maximum grows less and less often: the sums are only moved when one of the warp's has.
+      bool grown = false;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) grown = grown || corr[n][0] != 1.0f || corr[n][1] != 1.0f;
+      if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < NMT; ++i) o[n][i][0] *= corr[n][0], o[n][i][1] *= corr[n][1], o[n][i][2] *= corr[n][0], o[n][i][3] *= corr[n][1];
+      }
       // per 32 dims: dims 32u + 4g .. + 3 of keys 2t, 2t + 1, 2t + 8, 2t + 9, paired by key: m-tile 2u has rows
       // g <-> dim 32u + 4g, g + 8 <-> 32u + 4g + 1, m-tile 2u + 1 the two dims after them
 #pragma unroll
@@ -291,10 +289,11 @@ __global__ void __launch_bounds__(C::NW * 32, C::CTAS) diff_decode_kernel(const 
         for (int n = 0; n < NT; ++n) {
           float(&x)[4] = o[n][2 * u];
           float(&y)[4] = o[n][2 * u + 1];
-          x[0] *= corr[n][0], x[1] *= corr[n][1], x[2] *= corr[n][0], x[3] *= corr[n][1];
-          mma_16816<C::CDT>(x, fa, pb[n][0], pb[n][1]);
-          y[0] *= corr[n][0], y[1] *= corr[n][1], y[2] *= corr[n][0], y[3] *= corr[n][1];
-          mma_16816<C::CDT>(y, fb, pb[n][0], pb[n][1]);
+          float dx[4] = {0.f, 0.f, 0.f, 0.f}, dy[4] = {0.f, 0.f, 0.f, 0.f};
+          mma_16816<C::CDT>(dx, fa, pb[n][0], pb[n][1]);
+          mma_16816<C::CDT>(dy, fb, pb[n][0], pb[n][1]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] = fmaf(dx[i], vscale, x[i]), y[i] = fmaf(dy[i], vscale, y[i]);
         }
       }
     }
@@ -336,7 +335,7 @@ __global__ void __launch_bounds__(C::NW * 32, C::CTAS) diff_decode_kernel(const 
 #pragma unroll
       for (int i = 0; i < NMT; ++i) {
         const int lo = C::FP8 ? 32 * (i >> 1) + 4 * g + 2 * (i & 1) : 16 * i + g, hi = C::FP8 ? lo + 1 : lo + 8;
-        on[lo] = o[n][i][0] * v_ref, on[OLD + lo] = o[n][i][1] * v_ref, on[hi] = o[n][i][2] * v_ref, on[OLD + hi] = o[n][i][3] * v_ref;
+        on[lo] = o[n][i][0], on[OLD + lo] = o[n][i][1], on[hi] = o[n][i][2], on[OLD + hi] = o[n][i][3];
       }
       if (g == 0) {
         msm[8 * n + 2 * t] = m[n][0], msm[8 * n + 2 * t + 1] = m[n][1];

@@ -1234,7 +1234,8 @@ int esp_diff_plan_opts(const esp_attn_shape* s, const esp_attn_tree* trees, int3
   // and the join of the records. Microseconds, measured; with 128-dim heads two CTAs share an SM and each runs slower than
   // alone. 700 rows behind 20001 keys, 8 kv heads, took 525 us unsplit, 484 in two, 515 in three and 533 in four parts; the rule
   // gives 523, 475, 506 and 532. Small prompts share their tiles between heads: 4 x 33 rows, 256 dims, 24.5 us in tiles of one head, 13.0 of two;
-  // 8 x 20 .. 100 rows, 128 dims, 24.2 us of one, 21.0 of two, 13.8 of four. Near ties keep taller tiles and fewer parts.
+  // 8 x 20 .. 100 rows, 128 dims, 24.2 us of one, 21.0 of two, 13.8 of four. Near ties keep taller tiles and fewer parts (without a cached prefix
+  // ties within a tenth: 2 x 8192 and 5 x 33 .. 4001 rows measured 1 to 4 % faster in tiles of one head).
   const bool wide = s->HD >= 256, split = cached > 2 * fresh;
   const double t_alone = wide ? 1.45 : 1.2, t_shared = wide ? 1.45 : 1.9, t_fixed = 9.0;  // per 128 keys alone / sharing an SM; start and end of a CTA
   const int64_t slots = wide ? 148 : 296;
@@ -1265,7 +1266,7 @@ int esp_diff_plan_opts(const esp_attn_shape* s, const esp_attn_tree* trees, int3
       }
       if (rows_split) t += 6.0 + double(rows_split) * s->H * 2 * (s->HD + 2) * 4 * 2 / 6.0e6;  // written and read at about 6 TB/s, mostly in L2
       if (o->tile_rows && t > 1.5 * best) break;
-      if (!o->tile_rows || t < 0.97 * best) {
+      if (!o->tile_rows || t < (split ? 0.97 : 0.9) * best) {
         best = t;
         // the planner sizes its chunks so that the tiles fit `groups / Hkv`
         o->tile_rows = TR, o->split = parts == 1 ? 0 : 1 << 20, o->groups = int(std::clamp<int64_t>(tiles, 1, 1 << 24)) * s->Hkv;

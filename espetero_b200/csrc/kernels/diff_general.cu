@@ -3,7 +3,10 @@
 //
 // One warp owns one (row, head): 32 keys per step, lane = key for the two scores (q1 . k1 and q2 . k2, halves of one K row, read
 // once), two online softmaxes in the exp2 domain by warp shuffles, lane = HD / 32 dims for P_1 V and P_2 V, which share every V
-// row they read. Sums are fp32 and the weights are not rounded. Bound by the CUDA cores' fp32 rate and by K rows read lane by lane.
+// row they read. Sums are fp32 and the weights are not rounded. Bound by the CUDA cores' fp32 rate and by K rows read lane by lane:
+// 2048 causal rows of 16 heads take 6.2 ms with 128 dims (diff_umma: 49 us) and 3.7 ms with 64; 32 tokens behind 4096 keys 3.3 ms (diff_decode:
+// 85 us). Even for 16 rows without a cache (10.2 us against 10.1) or one key (10.4 against 10.2) it wins nothing, so it takes only what the
+// others do not.
 #include "diff.cuh"
 
 namespace esp {

@@ -219,9 +219,9 @@ def prepare(c, seed):
     st["flat"] = torch.from_numpy(np.concatenate([b * M + np.arange(m) for b, m in enumerate(ms)])).to(DEV)
     st["ms"], st["ps"], st["tab"], st["base"], st["n_blocks"] = ms, ps, tab, base, n_blocks
     if own:
-        from espetero_b200 import capi, host
+        from espetero_b200 import host
         trees = host.make_trees(ms, ps, tab)
-        tile_rows, opts = host.diff_plan_options(trees, H, Hkv, HD, capi.ESP_E4M3 if c["pool"] == "e4m3" else capi.ESP_F16)
+        tile_rows, opts = host.diff_plan_options(trees, H, Hkv, HD)
         st["op"] = handle(H, Hkv, HD, bt, c["dtype"], c["pool"], st["scale"], tree, tile_rows)
         plan = host.plan_tiles(trees, Hkv, **opts)
         st["call"] = st["op"].diff_call(plan, trees, st["Q"], st["Kb"], st["Vb"], st["O"], kv=st["pool"], kv_scales=st["scales"], blocks=st["blocks"], n_blocks=n_blocks,

@@ -8,7 +8,6 @@ Three operations of one layer, as a serving loop runs them:
 A differential head of HD dims holds two queries and two keys of HD / 2 dims and one value of HD dims:
   O = out_scale * w * D / sqrt(mean D^2 + eps),  D = softmax(scale q1.k1) V - lambda_h softmax(scale q2.k2) V.
 """
-import functools
 import math
 
 import numpy as np
@@ -126,14 +125,6 @@ def work(c):
 
 
 # ------------------------------------------------------------------------------------------------ inputs
-@functools.lru_cache(maxsize=None)
-def handle(H, Hkv, HD, bt, dtype, pool, scale, tree, tile_rows):
-    """The context of a layer's shape: a program makes it once and keeps it for all inputs."""
-    from espetero_b200 import capi, host
-    dt = {"f16": capi.ESP_F16, "bf16": capi.ESP_BF16, "e4m3": capi.ESP_E4M3}
-    return host.AttnOp(H, Hkv, HD, bt, dt[dtype], dt[pool], scale, capi.ESP_ATTN_FLAG_ANC_MASK if tree else 0, tile_rows)
-
-
 def pool_of(g, n_blocks, c):
     """A cache whose pages all hold something, and - 8-bit - the scale of every page and key head."""
     shape = (n_blocks, 2, c["bt"], c["Hkv"], c["HD"])
@@ -176,7 +167,9 @@ def prepare(c, seed):
         st["q"] = torch.empty((rows, H * HD), dtype=T16[c["dtype"]], device=DEV)
         st["k"], st["v"] = (torch.empty((rows, Hkv * HD), dtype=T16[c["dtype"]], device=DEV) for _ in range(2))
         if own:
-            st["op"] = handle(H, Hkv, HD, bt, c["dtype"], c["pool"], 1.0, False, 8)
+            from espetero_b200 import capi, host
+            dt = {"f16": capi.ESP_F16, "bf16": capi.ESP_BF16, "e4m3": capi.ESP_E4M3}
+            st["op"] = host.AttnOp(H, Hkv, HD, bt, dt[c["dtype"]], dt[c["pool"]], 1.0)
             q, k, v = st["X"].split([H * HD, Hkv * HD, Hkv * HD], dim=1)
             st["call"] = st["op"].append_call(Q=q, K=k, V=v, Qo=st["q"], Kb=st["k"], Vb=st["v"], kv=st["pool"], kv_scales=st["scales"], n_blocks=st["n_blocks"],
                                               slots=st["slots"], pos=st["pos"], inv_freq=st["inv_freq"], maps=c["maps"], adjacent=c["pairs"] == "adjacent")
@@ -219,10 +212,11 @@ def prepare(c, seed):
     st["flat"] = torch.from_numpy(np.concatenate([b * M + np.arange(m) for b, m in enumerate(ms)])).to(DEV)
     st["ms"], st["ps"], st["tab"], st["base"], st["n_blocks"] = ms, ps, tab, base, n_blocks
     if own:
-        from espetero_b200 import host
+        from espetero_b200 import capi, host
+        dt = {"f16": capi.ESP_F16, "bf16": capi.ESP_BF16, "e4m3": capi.ESP_E4M3}
         trees = host.make_trees(ms, ps, tab)
         tile_rows, opts = host.diff_plan_options(trees, H, Hkv, HD)
-        st["op"] = handle(H, Hkv, HD, bt, c["dtype"], c["pool"], st["scale"], tree, tile_rows)
+        st["op"] = host.AttnOp(H, Hkv, HD, bt, dt[c["dtype"]], dt[c["pool"]], st["scale"], capi.ESP_ATTN_FLAG_ANC_MASK if tree else 0, tile_rows)
         plan = host.plan_tiles(trees, Hkv, **opts)
         st["call"] = st["op"].diff_call(plan, trees, st["Q"], st["Kb"], st["Vb"], st["O"], kv=st["pool"], kv_scales=st["scales"], blocks=st["blocks"], n_blocks=n_blocks,
                                         desc=st["desc"], anc_mask=st["anc"] if tree else None, lam=st["lam"], norm_w=st["w"], eps=EPS, out_scale=OUT_SCALE)

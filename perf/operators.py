@@ -170,9 +170,6 @@ def prepare(c, seed):
             from espetero_b200 import capi, host
             dt = {"f16": capi.ESP_F16, "bf16": capi.ESP_BF16, "e4m3": capi.ESP_E4M3}
             st["op"] = host.AttnOp(H, Hkv, HD, bt, dt[c["dtype"]], dt[c["pool"]], 1.0)
-            q, k, v = st["X"].split([H * HD, Hkv * HD, Hkv * HD], dim=1)
-            st["call"] = st["op"].append_call(Q=q, K=k, V=v, Qo=st["q"], Kb=st["k"], Vb=st["v"], kv=st["pool"], kv_scales=st["scales"], n_blocks=st["n_blocks"],
-                                              slots=st["slots"], pos=st["pos"], inv_freq=st["inv_freq"], maps=c["maps"], adjacent=c["pairs"] == "adjacent")
         return st
 
     ms, ps = lengths(c)
@@ -215,7 +212,7 @@ def prepare(c, seed):
         from espetero_b200 import capi, host
         dt = {"f16": capi.ESP_F16, "bf16": capi.ESP_BF16, "e4m3": capi.ESP_E4M3}
         trees = host.make_trees(ms, ps, tab)
-        tile_rows, opts = host.diff_plan_options(trees, H, Hkv, HD)
+        tile_rows, opts = host.diff_plan_options(trees, H, Hkv, HD, dt[c["pool"]])
         st["op"] = host.AttnOp(H, Hkv, HD, bt, dt[c["dtype"]], dt[c["pool"]], st["scale"], capi.ESP_ATTN_FLAG_ANC_MASK if tree else 0, tile_rows)
         plan = host.plan_tiles(trees, Hkv, **opts)
         st["call"] = st["op"].diff_call(plan, trees, st["Q"], st["Kb"], st["Vb"], st["O"], kv=st["pool"], kv_scales=st["scales"], blocks=st["blocks"], n_blocks=n_blocks,
@@ -287,7 +284,11 @@ def run(st):
     c = st["c"]
     if c["op"] == "append":
         if own:
-            st["op"].kv_append(st["call"])
+            H, Hkv, HD = c["H"], c["Hkv"], c["HD"]
+            q, k, v = st["X"].split([H * HD, Hkv * HD, Hkv * HD], dim=1)
+            call = st["op"].append_call(Q=q, K=k, V=v, Qo=st["q"], Kb=st["k"], Vb=st["v"], kv=st["pool"], kv_scales=st["scales"], n_blocks=st["n_blocks"], slots=st["slots"],
+                                        pos=st["pos"], inv_freq=st["inv_freq"], maps=c["maps"], adjacent=c["pairs"] == "adjacent")
+            st["op"].kv_append(call)
             q, k, v = st["q"], st["k"], st["v"]
         else:
             q, k, v = plain_append(st)

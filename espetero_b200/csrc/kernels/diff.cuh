@@ -16,6 +16,14 @@ __device__ __forceinline__ size_t diff_record(const KernelArgs& k, int part, int
   return ((((size_t(part) * k.p.Hkv + kvh) * k.tile_rows + r) * k.G + hg) * 2 + map) * (k.HD + 2);
 }
 
+// A row's mask record (segment start, -, ancestors, -), brought into its tree of M rows: records that say "none" or "all" by numbers outside
+// it mean the same, and sums with them stay in range.
+__device__ __forceinline__ int4 row_record(const KernelArgs& a, int row, int M) {
+  int4 d = reinterpret_cast<const int4*>(a.desc)[row];
+  d.x = min(max(d.x, 0), M), d.z = min(max(d.z, 0), M);
+  return d;
+}
+
 __device__ __forceinline__ float diff_lam(const DiffArgs& a, int row, int h) { return a.lam[size_t(row) * a.lam_ld + h]; }
 
 // The factor that turns D into the normalised row (before the weight), from the sum of D^2 over the head.

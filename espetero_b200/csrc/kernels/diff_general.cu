@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(kWarps * 32) diff_general_kernel(const DiffArg
         am = k.anc_mask[row];
         k_last = min(tree.M, 64) - 1;
       } else {
-        d = reinterpret_cast<const int4*>(k.desc)[row];
+        d = row_record(k, row, tree.M);
         k_last = min(tree.M - 1, max(rr, d.z - 1));
       }
       for (int j0 = 0; j0 <= k_last; j0 += 32) {

@@ -122,9 +122,9 @@ __device__ __forceinline__ BlockList block_list(const KernelArgs& a, const esp_a
     L.nbb = L.a_hi = (L.k_last + BN) / BN;
     return L;
   }
-  int anc_max = 0, seg_min = 1 << 30, anc_min = 1 << 30, seg_max = 0;
+  int anc_max = 0, seg_min = tree.M, anc_min = tree.M, seg_max = 0;
   for (int r = lane; r < rows_live; r += 32) {
-    const int4 d = reinterpret_cast<const int4*>(a.desc)[tile.r0 + r];
+    const int4 d = row_record(a, tile.r0 + r, tree.M);
     anc_max = max(anc_max, d.z), anc_min = min(anc_min, d.z), seg_min = min(seg_min, d.x), seg_max = max(seg_max, d.x);
   }
 #pragma unroll
@@ -136,12 +136,12 @@ __device__ __forceinline__ BlockList block_list(const KernelArgs& a, const esp_a
   L.anc_min = anc_min, L.seg_max = seg_max;
   L.k_last = min(tree.M - 1, max(r_last, anc_max - 1));
   const int n_all = (L.k_last + BN) / BN;
-  L.a_hi = min((max(anc_max, 0) + BN - 1) / BN, n_all);
-  L.b_lo = max(L.a_hi, max(seg_min, 0) / BN);
+  L.a_hi = min((anc_max + BN - 1) / BN, n_all);
+  L.b_lo = max(L.a_hi, seg_min / BN);
   L.nbb = L.a_hi + max(0, min(r_last / BN, n_all - 1) - L.b_lo + 1);
   // whole blocks: those that end below every row's ancestors, and - batch blocks [lo, hi) of the rows' segments - those that start
   // at or after every segment's start and end at or before the first row
-  L.full_a = min(L.a_hi, min(anc_min, tree.M) / BN);
+  L.full_a = min(L.a_hi, anc_min / BN);
   const int lo = max(L.b_lo, (seg_max + BN - 1) / BN), hi = (L.r_first + 1) / BN;
   L.seg_0 = L.nbc + L.a_hi + (lo - L.b_lo), L.seg_n = max(0, hi - lo);
   return L;

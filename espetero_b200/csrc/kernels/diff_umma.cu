@@ -325,7 +325,7 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
     }
     if (tile.last) {
       if (use_anc) am = a.anc_mask[row];
-      else dsc = reinterpret_cast<const int4*>(a.desc)[row];
+      else dsc = row_record(a, row, tree.M);
     }
     tc_fence_before_sync();
     named_barrier(1, kSoftmax + 32);

@@ -1,0 +1,76 @@
+"""Differential attention at the edges of what its documentation allows: mask records outside their tree, garbage in rows that nobody
+sees, page scales and queries of every magnitude, layers behind the pool's first, wide row strides; and the plans and refusals that
+go with them."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+from espetero_b200 import capi, host, workloads as wl
+
+from .diff_ref import SUB16, U16, call_checks, diff64, keys_values, visible  # noqa: F401 (a fixture)
+
+gpu = pytest.mark.gpu
+EPS, SCALE = 1e-5, 0.6
+GENERAL = dict(attn_gqa=0, attn_umma=0)
+
+
+def _weights(w, seed):
+    rng = np.random.default_rng(seed)
+    return rng.uniform(0.1, 0.9, size=w.H).astype(np.float32), (1 + 0.2 * rng.standard_normal(w.HD)).astype(np.float32)
+
+
+def _run(w, lam, norm_w, options=None, tile_rows=None, split=None, eps=EPS):
+    """One pass as its plan options say, or in tiles of `tile_rows`; (O as float64, kernel)."""
+    auto_rows, opts = host.diff_plan_options(w.trees, w.H, w.Hkv, w.HD, w.kv_dtype)
+    opts.update(tile_rows=tile_rows or auto_rows)
+    if split is not None:
+        opts.update(split=split, groups=4096 if split else 1)
+    op = host.AttnOp.for_workload(w, opts["tile_rows"])
+    try:
+        for k, v in (options or {}).items():
+            op.set_option(k, v)
+        dp = op.upload(w)
+        t = lambda a: torch.from_numpy(np.ascontiguousarray(a)).to(op.device)
+        O = torch.full((w.n_rows, w.q_ld), 0x1234, dtype=torch.int16, device=op.device)
+        call = op.diff_call(host.plan_tiles(w.trees, w.Hkv, **opts), w.trees, dp.Q, dp.Kb, dp.Vb, O, kv=dp.kv, kv_scales=dp.kv_scales, blocks=dp.blocks, n_blocks=w.n_blocks,
+                            desc=dp.desc, anc_mask=dp.anc_mask, lam=t(lam), norm_w=t(norm_w), eps=eps, out_scale=SCALE, kv_base=w.kv_base)
+        op.diff_forward(call)
+        torch.cuda.synchronize()
+        op.check_status()
+        return wl.from_bits16(O.cpu().numpy().view(np.uint16), w.q_dtype).astype(np.float64), op.last_kernel
+    finally:
+        op.close()
+
+
+def _unit(w, ran):
+    """Half a step of the type that the softmax weights are rounded to."""
+    return 0.0 if ran == "diff_general" else (2.0 ** -11 if (ran == "diff_decode" and w.kv_dtype == wl.E4M3) else U16[w.q_dtype])
+
+
+def _check(w, kernel=None, seed=3, **kw):
+    lam, norm_w = _weights(w, seed)
+    got, ran = _run(w, lam, norm_w, **kw)
+    assert kernel is None or ran == kernel, ran
+    O64, tol = diff64(w, lam, norm_w, EPS, SCALE, _unit(w, ran))
+    bad = ~(np.abs(got - O64) <= tol)
+    assert not bad.any(), f"{ran}: {int(bad.sum())} of {bad.size} off, first at {np.argwhere(bad)[0]}"
+    return got, ran
+
+
+@gpu
+@pytest.mark.parametrize("options", [None, GENERAL], ids=["chosen", "general"])
+@pytest.mark.parametrize("HD", [128, 256])
+def test_mask_records_outside_their_tree(options, HD):
+    """desc records whose ancestor length is negative (none) or past the tree (all of it), and whose segment starts past the row (a row
+    that sees nothing; in the third tree all of them) or before the tree. 300 and 200 rows end inside a block of 128 keys."""
+    w = wl.make_pass("records", 21, [(0, 300), (40, 200), (0, 3)], 4, 2, HD, 16, wl.BF16, scale=(HD // 2) ** -0.5)
+    far = 2 ** 31 - 1
+    w.desc[:, 2] = -1000
+    w.desc[260:, 0] = -far - 1
+    w.desc[[5, 299, 310, 500, 501, 502], 0] = far
+    w.desc[[130, 320], 2] = far
+    w.desc[131, 2] = -far - 1
+    got, _ = _check(w, None if options else "diff_umma", options=options, tile_rows=128, split=0)
+    assert not got[[5, 299, 500, 501, 502]].any() and got[310].any()  # row 310 sees its 40 cached keys

@@ -99,6 +99,7 @@ struct BlockList {
   int a_hi, b_lo;       // batch blocks [0, a_hi) and from b_lo on
   int anc_min, seg_max; // keys below anc_min are seen by every row; segments start at seg_max at the latest
   int r_first;          // the tile's first row, relative to its tree
+  uint64_t nodes;       // ancestor masks: the tree's rows that some row of the tile sees; else all ones
   int full_c, full_a, seg_0, seg_n;  // blocks every row sees whole: [0, full_c), nbc + [0, full_a), seg_0 + [0, seg_n)
   __device__ __forceinline__ bool whole(int b) const { return b < full_c || uint32_t(b - nbc) < uint32_t(full_a) || uint32_t(b - seg_0) < uint32_t(seg_n); }
   __device__ __forceinline__ int n() const { return nbc + nbb; }
@@ -108,6 +109,8 @@ struct BlockList {
     return BN * (i < a_hi ? i : b_lo + (i - a_hi));
   }
   __device__ __forceinline__ int n_valid(int b) const { return min(BN, (b < nbc ? k1 : k_last + 1) - j0(b)); }
+  // Which of 64 keys of block b from column c on (a multiple of 64) any row of the tile may see.
+  __device__ __forceinline__ uint64_t seen64(int b, int c) const { return low_bits64(n_valid(b) - c) & (b < nbc || c > 0 ? ~0ull : nodes); }
 };
 
 // Whole-warp call; every warp forms the list for itself from the rows' records.
@@ -116,10 +119,14 @@ __device__ __forceinline__ BlockList block_list(const KernelArgs& a, const esp_a
   L.k0 = tile.k0, L.k1 = tile.k1, L.nbc = (tile.k1 - tile.k0 + BN - 1) / BN;
   L.nbb = 0, L.k_last = -1, L.a_hi = L.b_lo = 0, L.anc_min = 0, L.seg_max = 0, L.r_first = tile.r0 - tree.base;
   L.full_c = (tile.k1 - tile.k0) / BN, L.full_a = L.seg_n = 0, L.seg_0 = 0;
+  L.nodes = ~0ull;
   if (!tile.last) return L;
   if (a.anc_mask) {
     L.k_last = min(tree.M, 64) - 1;
     L.nbb = L.a_hi = (L.k_last + BN) / BN;
+    uint64_t any = 0;
+    for (int r = lane; r < rows_live; r += 32) any |= a.anc_mask[tile.r0 + r];
+    L.nodes = uint64_t(__reduce_or_sync(0xffffffffu, uint32_t(any))) | uint64_t(__reduce_or_sync(0xffffffffu, uint32_t(any >> 32))) << 32;
     return L;
   }
   int anc_max = 0, seg_min = tree.M, anc_min = tree.M, seg_max = 0;

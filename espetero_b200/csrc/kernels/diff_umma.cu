@@ -386,15 +386,18 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
       }
       mx *= sl2;  // scale > 0
       if (!whole) {
-        // V rows past the range are stale or foreign: 0 * NaN must not happen. Cleared before P is handed over.
+        // V rows that no row of the tile sees - past the range: stale or foreign; tree nodes in nobody's mask - may hold anything, and 0 * NaN must
+        // not happen. Cleared before P is handed over.
 #pragma unroll 1
         for (int k0 = c0; k0 < c0 + C::BU; k0 += 64) {
-          const int first = max(L.n_valid(b) - k0, 0), q = b * C::SPB + k0 / C::VK;  // the q-th slot use
-          if (first >= 64) continue;
+          const uint64_t seen = L.seen64(b, k0);
+          if (seen == ~0ull) continue;
+          const int first = __ffsll((long long)~seen) - 1, q = b * C::SPB + k0 / C::VK;  // the q-th slot use
           wait_bar(&sh.v_full[q % VS], uint32_t(q / VS) & 1u, kStatusTmaTimeout);
           for (int i = srow; i < (64 - first) * 8 * C::VC; i += BM) {
-            const int r = k0 % C::VK + first + i / (8 * C::VC), c = i % (8 * C::VC);
-            *reinterpret_cast<uint4*>(v_sm + (q % VS) * C::V_SLOT + (c >> 3) * C::V_CHUNK + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+            const int r = first + i / (8 * C::VC), c = i % (8 * C::VC);
+            if (!((seen >> r) & 1ull))
+              *reinterpret_cast<uint4*>(v_sm + (q % VS) * C::V_SLOT + (c >> 3) * C::V_CHUNK + (k0 % C::VK + r) * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
           }
         }
         fence_proxy_async_smem();

@@ -74,3 +74,21 @@ def test_mask_records_outside_their_tree(options, HD):
     w.desc[131, 2] = -far - 1
     got, _ = _check(w, None if options else "diff_umma", options=options, tile_rows=128, split=0)
     assert not got[[5, 299, 500, 501, 502]].any() and got[310].any()  # row 310 sees its 40 cached keys
+
+
+@gpu
+@pytest.mark.parametrize("options", [None, GENERAL], ids=["chosen", "general"])
+@pytest.mark.parametrize("tile_rows", [16, 128])
+@pytest.mark.parametrize("HD", [128, 256])
+def test_garbage_in_tree_nodes_that_nobody_sees(options, tile_rows, HD):
+    """Padding nodes: their mask is empty and in no other node's mask; their keys and values hold NaN and infinities."""
+    w = wl.make_pass("padding nodes", 22, [(0, 16), (64, 40), (20, 64)], 8, 1, HD, 16, wl.BF16, scale=(HD // 2) ** -0.5, mask="tree")
+    unseen = {0: [3, 15], 16: [0, 31, 32, 39], 56: [17, 63]}
+    for base, nodes in unseen.items():
+        rows = w.anc_mask[base:base + 64 if base == 56 else base + (16 if base == 0 else 40)]
+        for j in nodes:
+            rows &= ~np.uint64(1 << j)
+            rows[j] = 0
+            w.Kb[base + j], w.Vb[base + j] = 0x7FC0, np.resize(np.array([0x7FC0, 0x7F80, 0xFF80], dtype=np.uint16), w.kv_ld)
+    got, _ = _check(w, None if options else "diff_umma", options=options, tile_rows=tile_rows, split=0)
+    assert not got[[3, 15]].any() and got[[16, 55, 73]].any(axis=1).all()

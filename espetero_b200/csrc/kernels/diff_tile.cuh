@@ -210,17 +210,20 @@ __device__ __forceinline__ float chunk_max(const uint32_t (&s)[32]) {
   return fmax3(fmaxf(m[0], m[1]), m[2], m[3]);
 }
 
-// The same over an E4M3 pool: k0, k1 = the (positive) K scales of the chunk's two pages.
-__device__ __forceinline__ float chunk_max(const uint32_t (&s)[32], float k0, float k1) {
+// Over an E4M3 pool a row's reference is the largest scaled score + log2 of the page's V scale: the scale of a page goes on the weights before
+// they are rounded to 16 bits, and what has to stay in fp16's range is their product. (Against the scores' maximum alone, a page of large values
+// that a row hardly attends would push the weights of the others under fp16's.) k0, k1 = scale of the softmax, in log2 units, times the
+// (positive) K scales of the chunk's two pages, v0, v1 their log2_scale.
+__device__ __forceinline__ float log2_scale(float v) { return fminf(fmaxf(float(int((__float_as_uint(v) >> 23) & 0xFFu) - 127), -100.0f), 100.0f); }  // rounded down
+__device__ __forceinline__ float chunk_max(const uint32_t (&s)[32], float k0, float k1, float v0, float v1) {
   float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
   for (int c = 0; c < 32; c += 2) m[(c >> 4) * 2 + ((c >> 1) & 1)] = fmax3(m[(c >> 4) * 2 + ((c >> 1) & 1)], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
-  return fmaxf(fmaxf(m[0], m[1]) * k0, fmaxf(m[2], m[3]) * k1);
+  return fmaxf(fmaf(fmaxf(m[0], m[1]), k0, v0), fmaf(fmaxf(m[2], m[3]), k1, v1));
 }
 
 // 32 scores -> 16 packed pairs of weights exp2(sl s - m), sl = sl_a for the chunk's first 16 columns and sl_b for the others (a page each);
-// `sum` (two partial sums) gains the unrounded weights. F8: v0, v1 = the V scales of the two pages, in units of the tile's reference, on
-// the weights that are handed on.
+// `sum` (two partial sums) gains the unrounded weights. F8: v0, v1 = the V scales of the two pages, on the weights that are handed on.
 template <int QDT, bool F8>
 __device__ __forceinline__ void chunk_weights(const uint32_t (&s)[32], uint32_t* pk, uint64_t sl_a, uint64_t sl_b, uint64_t neg_m2, uint64_t (&sum)[2], float v0, float v1) {
 #pragma unroll
@@ -233,21 +236,6 @@ __device__ __forceinline__ void chunk_weights(const uint32_t (&s)[32], uint32_t*
     const float v = c < 8 ? v0 : v1;
     pk[c] = F8 ? Elem16<QDT>::pack2(p0 * v, p1 * v) : Elem16<QDT>::pack2(p0, p1);
   }
-}
-
-// 2^floor(log2 x), and its reciprocal, for a positive normal x.
-__device__ __forceinline__ float pow2_floor(float x) { return __uint_as_float(__float_as_uint(x) & 0x7F800000u); }
-__device__ __forceinline__ float pow2_inverse(float p) { return __uint_as_float(0x7F000000u - __float_as_uint(p)); }
-
-// The reference of a tile's V scales over an E4M3 pool. The weights of a page are multiplied by its scale before they are rounded to 16
-// bits, relative to a power of two that follows the largest scale seen so far (within a factor of 16): neither tiny nor huge scales
-// leave fp16's range. Returns the factor for what has been summed in the old unit.
-__device__ __forceinline__ float follow_scale(float& ref, float largest) {
-  if (ref > 0.0f && !(largest > 16.0f * ref)) return 1.0f;
-  const float now = pow2_floor(fminf(fmaxf(largest, 1.17549435e-38f), 1.0e38f));
-  const float f = ref > 0.0f ? ref * pow2_inverse(now) : 1.0f;
-  ref = now;
-  return f;
 }
 
 }  // namespace difft

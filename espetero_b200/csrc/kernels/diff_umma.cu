@@ -32,7 +32,7 @@
 // completes the warpgroup that hands registers over). Hand-offs by mbarrier; every wait is bounded: after a timeout the CTA records a
 // code, stops waiting, finishes its loop, frees its tensor memory and returns.
 // E4M3 pools (F8): the pages are 16-bit codes (diff_widen.cu); the K producer leaves each block's page scales in shared memory, the
-// K scale goes on the score and the V scale on the weight.
+// K scale goes on the score and the V scale on the weight, whose reference is the largest product of the two.
 #include "diff_tile.cuh"
 
 namespace esp {
@@ -81,7 +81,7 @@ struct Shared {
   uint32_t tmem;
   volatile int dead;
   float k_scale[kSlots][kPages], v_scale[kSlots][kPages];
-  float m_ref[BM], v_ref[4];
+  float m_ref[BM];
 };
 
 __device__ __forceinline__ void cluster_sync() {
@@ -341,28 +341,26 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
       const uint32_t par = uint32_t(n >> 1) & 1u;
       const bool whole = L.whole(b);
       // the reference, from the partner warp that had the unit before: its maximum has long been known when these scores arrive
-      float m_old = -INFINITY, v_ref = 0.0f;
+      float m_old = -INFINITY;
       if (n > 0) {
         wait_bar(&sh.m_ready[wg ^ 1], uint32_t((n - 1) >> 1) & 1u, kStatusMmaTimeout);
         m_old = *const_cast<volatile float*>(&sh.m_ref[srow]);
-        if constexpr (F8) v_ref = *const_cast<volatile float*>(&sh.v_ref[wq]);
       }
-      float ks[2 * NS] = {}, vs[2 * NS] = {}, largest = 0.0f;
+      float ks[2 * NS] = {}, vs[2 * NS] = {};  // the pages' K scales, times the softmax's, and V scales
       if constexpr (F8) {
         wait_bar(&sh.sc_full[b % kSlots], uint32_t(b / kSlots) & 1u, kStatusTmaTimeout);
 #pragma unroll
         for (int i = 0; i < 2 * NS; ++i) {
-          ks[i] = fmaxf(sh.k_scale[b % kSlots][c0 / 16 + i], 1.17549435e-38f), vs[i] = sh.v_scale[b % kSlots][c0 / 16 + i];  // -inf * 0 must not happen
-          largest = fmaxf(largest, vs[i]);
+          ks[i] = fmaxf(sl2 * sh.k_scale[b % kSlots][c0 / 16 + i], 1.17549435e-38f), vs[i] = sh.v_scale[b % kSlots][c0 / 16 + i];  // -inf * 0 must not happen
         }
       }
       wait_bar(&sh.s_full[wg], par, kStatusMmaTimeout);
       tc_fence_after_sync();
-      // 32 scores, hidden where the row does not see the key; and their maximum, with the pages' K scales
+      // 32 scores, hidden where the row does not see the key; and their maximum in log2 units
       auto shape = [&](uint32_t (&x)[32], int i) {
         if (!whole) hide(x, visible32(L, b, c0 + 32 * i, dsc, am, use_anc, rr));
       };
-      auto top = [&](const uint32_t (&x)[32], int i) { return F8 ? chunk_max(x, ks[2 * i], ks[2 * i + 1]) : chunk_max(x); };
+      auto top = [&](const uint32_t (&x)[32], int i) { return F8 ? chunk_max(x, ks[2 * i], ks[2 * i + 1], log2_scale(vs[2 * i]), log2_scale(vs[2 * i + 1])) : sl2 * chunk_max(x); };  // scale > 0
       constexpr int HELD = C::HOLD ? NS : 1;
       uint32_t s[HELD][32];
       float mx = -INFINITY;
@@ -384,7 +382,6 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
           mx = fmaxf(mx, top(s[0], i));
         }
       }
-      mx *= sl2;  // scale > 0
       if (!whole) {
         // V rows that no row of the tile sees - past the range: stale or foreign; tree nodes in nobody's mask - may hold anything, and 0 * NaN must
         // not happen. Cleared before P is handed over.
@@ -404,11 +401,6 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
       }
       const bool grow = mx > m_old + kGrow;  // also the first finite maximum
       const float m_new = grow ? mx : m_old;
-      float vfac = 1.0f;
-      if constexpr (F8) {
-        vfac = follow_scale(v_ref, largest);
-        if (lane == 0) *const_cast<volatile float*>(&sh.v_ref[wq]) = v_ref;
-      }
       *const_cast<volatile float*>(&sh.m_ref[srow]) = m_new;
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.m_ready[wg]);
@@ -416,10 +408,10 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
         l_run *= fast_exp2(m_seen - m_new);
         m_seen = m_new;
       }
-      if (n > 0 && __any_sync(0xffffffffu, grow || vfac != 1.0f)) {
+      if (n > 0 && __any_sync(0xffffffffu, grow)) {
         wait_bar(&sh.o_done[wg ^ 1], uint32_t((n - 1) >> 1) & 1u, kStatusMmaTimeout);  // every unit before this one is in O
         tc_fence_after_sync();
-        const float factor = (grow ? fast_exp2(m_old - m_new) : 1.0f) * vfac;
+        const float factor = grow ? fast_exp2(m_old - m_new) : 1.0f;
 #pragma unroll 1
         for (int c = 0; c < HD / 32; ++c) {
           uint32_t o[32];
@@ -433,7 +425,6 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
       const float neg_m = m_new == -INFINITY ? 0.0f : -m_new;
       const uint64_t neg_m2 = f32x2_pack(neg_m, neg_m);
       uint64_t sum[2] = {f32x2_pack(0.0f, 0.0f), f32x2_pack(0.0f, 0.0f)};
-      const float vinv = F8 ? pow2_inverse(v_ref) : 1.0f;
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
         if constexpr (!C::HOLD) {  // P of chunk i lies in columns the chunks to come do not use
@@ -442,7 +433,7 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
           shape(s[0], i);
         }
         uint32_t pk[16];
-        chunk_weights<QDT, F8>(s[C::HOLD ? i : 0], pk, F8 ? f32x2_pack(sl2 * ks[2 * i], sl2 * ks[2 * i]) : sl2x2, F8 ? f32x2_pack(sl2 * ks[2 * i + 1], sl2 * ks[2 * i + 1]) : sl2x2, neg_m2, sum, F8 ? vs[2 * i] * vinv : 1.0f, F8 ? vs[2 * i + 1] * vinv : 1.0f);
+        chunk_weights<QDT, F8>(s[C::HOLD ? i : 0], pk, F8 ? f32x2_pack(ks[2 * i], ks[2 * i]) : sl2x2, F8 ? f32x2_pack(ks[2 * i + 1], ks[2 * i + 1]) : sl2x2, neg_m2, sum, vs[2 * i], vs[2 * i + 1]);
         tmem_st16(buf + 16 * i, pk);
         if ((i + 1) % (C::PART / 32) == 0) {  // a part is ready: its P . V starts under the rest
           tmem_wait_st();
@@ -462,12 +453,11 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
     float4 w4 = make_float4(0.f, 0.f, 0.f, 0.f);
     if (whole_rows && args.norm_w && tid < HD / 4) w4 = reinterpret_cast<const float4*>(args.norm_w)[tid];
     named_barrier(2, kSoftmax);  // both groups are through: the reference is final, and all but the last two P . V are known to be done
-    float m_fin = -INFINITY, v_ref = 1.0f;
+    float m_fin = -INFINITY;
     if (N > 0) {
       wait_bar(&sh.o_done[(N - 1) & 1], uint32_t((N - 1) >> 1) & 1u, kStatusMmaTimeout);
       tc_fence_after_sync();
       m_fin = *const_cast<volatile float*>(&sh.m_ref[srow]);
-      if constexpr (F8) v_ref = *const_cast<volatile float*>(&sh.v_ref[wq]);
     }
     // the groups' sums (the rings are idle: every load has been waited for and every MMA that reads them is done)
     float* lsum = reinterpret_cast<float*>(k_sm);
@@ -494,7 +484,7 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
         load_o(col, v);
         if (row_ok) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) *reinterpret_cast<float2*>(rec + col + i) = make_float2(v[i] * v_ref, v[i + 1] * v_ref);
+          for (int i = 0; i < 32; i += 2) *reinterpret_cast<float2*>(rec + col + i) = make_float2(v[i], v[i + 1]);
         }
       }
       if (row_ok && wg == 0) *reinterpret_cast<float2*>(rec + HD) = make_float2(m_fin * kLn2, l);
@@ -505,7 +495,7 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
       uint8_t* give = v_sm;                                 // [HD / 8][128 rows][4 columns], lanes side by side
       float* take = reinterpret_cast<float*>(v_sm + HALF);  // the same, written by the peer
       float* sq = reinterpret_cast<float*>(q_sm);           // [CTA * 2 + group][128 rows]: the rows' sums of squares; written by both
-      const float inv = l > 0.0f ? (map ? -lam : 1.0f) * v_ref / l : 0.0f;
+      const float inv = l > 0.0f ? (map ? -lam : 1.0f) / l : 0.0f;
       float* w_sm = reinterpret_cast<float*>(k_sm) + 2 * BM;  // the norm's weights
       if (args.norm_w && tid < HD / 4) reinterpret_cast<float4*>(w_sm)[tid] = w4;
       if (tid == 0) mbar_arrive_expect_tx(&sh.take_full, HALF);

@@ -92,3 +92,52 @@ def test_garbage_in_tree_nodes_that_nobody_sees(options, tile_rows, HD):
             w.Kb[base + j], w.Vb[base + j] = 0x7FC0, np.resize(np.array([0x7FC0, 0x7F80, 0xFF80], dtype=np.uint16), w.kv_ld)
     got, _ = _check(w, None if options else "diff_umma", options=options, tile_rows=tile_rows, split=0)
     assert not got[[3, 15]].any() and got[[16, 55, 73]].any(axis=1).all()
+
+
+@gpu
+@pytest.mark.parametrize("split", [0, 32], ids=["whole", "split"])
+@pytest.mark.parametrize("rows", [1, 20])
+@pytest.mark.parametrize("HD", [128, 256])
+def test_a_page_of_large_values_that_is_hardly_attended(HD, rows, split):
+    """An fp16 pass over E4M3 pages. The first page's V scale is 2^6 and its keys score 60 below the others', whose V scale is 2^-20; so do the
+    pass's own keys. The rows are what the small pages hold: every weight has to keep its bits beside the large page's.
+    The bound: weights p_j s_j are rounded to half a step of fp16, or to half a subnormal step in units of at most twice the row's largest
+    p_j s_j; a code is at most 448. The rest as in diff64."""
+    w = wl.make_pass("uneven", 23, [(96, rows)], 8, 2, HD, 16, wl.F16, wl.E4M3, scale=1.0)
+    d = HD // 2
+    Q = np.full((rows, w.H, 2, d), 0.125, dtype=np.float32)
+    w.Q = wl.to_bits16(Q.reshape(rows, -1), wl.F16)
+    pool = w.kv.reshape(w.n_blocks, 2, w.bt, w.Hkv, HD)
+    rng = np.random.default_rng(5)
+    for i, b in enumerate(w.blocks):
+        k = rng.uniform(-1.0, 1.0, size=(w.bt, w.Hkv, HD)) - (480.0 / d if i == 0 else 0.0)
+        pool[b, 0] = wl.e4m3_encode((k * 8).astype(np.float32))
+        w.kv_scales[b, 0], w.kv_scales[b, 1] = 0.125, 2.0 ** (6 if i == 0 else -20)
+    w.Kb = wl.to_bits16((rng.uniform(-1, 1, size=(rows, w.kv_ld)) - 480.0 / d).astype(np.float32), wl.F16)
+    lam, norm_w = _weights(w, 3)
+    eps = 1e-14
+    got, ran = _run(w, lam, norm_w, tile_rows=8 if rows == 1 else 128, split=split, eps=eps)
+    assert ran == ("diff_decode" if rows == 1 else "diff_umma")
+    O64, _ = diff64(w, lam, norm_w, eps, SCALE, 0.0)
+    unit, n = U16[wl.F16], 96 + rows
+    for kvh in range(w.Hkv):
+        K, V, _ = keys_values(w, 0, kvh)
+        size = np.ones(n)  # the page's scale beside every key
+        size[:96] = np.repeat(w.kv_scales[w.blocks, 1, kvh], w.bt)
+        for h in range(kvh * 4, kvh * 4 + 4):
+            D, e = 0.0, 0.0
+            for c, f in ((0, 1.0), (1, float(lam[h]))):
+                s = np.where(visible(w, 0), Q[:, h, c].astype(np.float64) @ K[:, c * d:(c + 1) * d].T, -np.inf)
+                p = np.exp(s - s.max(axis=1, keepdims=True))
+                p /= p.sum(axis=1, keepdims=True)
+                es = 0.125 * np.abs(K[:, c * d:(c + 1) * d]).sum(axis=1).max() * (d + 2) * 2.0 ** -24
+                D = D + (f if c == 0 else -f) * (p @ V)
+                e = e + f * ((2 * es + 2.0 ** -21 + (n + 8) * 2.0 ** -24 + unit) * (p @ np.abs(V)) + n * 448 * 2.0 ** -24 * (p * size).max(axis=1, keepdims=True))
+            norm = np.sqrt((D * D).sum(axis=1, keepdims=True))
+            assert (norm < 1e-3).all()  # the large page is not in it
+            fac = SCALE / np.sqrt((D * D).mean(axis=1, keepdims=True) + eps) * norm_w
+            tol = 1.02 * np.abs(fac) * (e + np.abs(D) * np.sqrt((e * e).sum(axis=1, keepdims=True)) / norm) + (unit + 2.0 ** -20) * np.abs(fac * D) + SUB16[wl.F16]
+            cols = slice(h * HD, (h + 1) * HD)
+            assert np.allclose(O64[:, cols], fac * D, rtol=1e-9, atol=1e-12)
+            err = np.abs(got[:, cols] - O64[:, cols])
+            assert (err <= tol).all(), (ran, float((err / tol).max()), float(np.abs(got[:, cols]).max()))

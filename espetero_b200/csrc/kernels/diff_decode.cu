@@ -12,8 +12,8 @@
 // V and K arrive by TMA (two bulk tensor loads per block, 128-byte swizzle, rows through the page table) in rings that belong to
 // single warps, so nothing in the loop waits for another warp. Softmax in the exp2 domain over the key lanes; P^T re-enters as the
 // B operand (movmatrix), rounded to 16 bits: what the MMA takes; sums and the rows' totals stay fp32 and unrounded. E4M3 codes
-// are widened to fp16 in registers (exact), the K scale goes on the score, the V scale on the block's P . V:
-// p is rounded as it is, and the largest, 1, exactly.
+// are widened to fp16 in registers (exact), and bf16 queries scaled into its range, the K scale goes on the score, the V scale on the block's
+// P . V: p is rounded as it is, and the largest, 1, exactly.
 // 32 sequences of 512 .. 32768 keys, H32 / Hkv4 / HD128, bf16: 92 us with the join = 5.7 TB/s, 0.87 of the copy peak; 131072 keys, Hkv8 / HD256, E4M3:
 // 94 us = 5.7 TB/s. 16 x 8192 E4M3 keys of 128 dims: 72 us = 3.7 TB/s, bound by the widening's instructions.
 // All waits are bounded; a CTA that gives up writes empty records and says so in the status word.
@@ -27,6 +27,7 @@ struct Cfg {
   static constexpr int HD = HD_, QDT = QDT_, NT = NT_, NW = NW_, STAGES = STAGES_, CTAS = CTAS_;
   static constexpr bool FP8 = KVDT_ == ESP_E4M3;
   static constexpr int CDT = FP8 ? ESP_F16 : KVDT_;   // MMA operand type
+  static constexpr bool SCALED_Q = FP8 && QDT == ESP_BF16;  // queries beyond the operand type's range
   static constexpr int ROW_BYTES = HD * (FP8 ? 1 : 2);
   static constexpr int NCH = ROW_BYTES / 128;         // 128-byte lines per key
   static constexpr int TILE = 16 * ROW_BYTES;         // K or V of a block
@@ -139,10 +140,37 @@ __global__ void __launch_bounds__(C::NW * 32, C::CTAS) diff_decode_kernel(const 
         // K fragments of an E4M3 tile hold dims 4t .. 4t + 3 of each 16: fragment columns (2t, 2t + 1) and (2t + 8, 2t + 9)
         // stand for dims (4t, 4t + 1) and (4t + 2, 4t + 3)
         const uint2 w = *reinterpret_cast<const uint2*>(q + 16 * ks + 4 * t);
-        const float2 f0 = QE::unpack2(w.x), f1 = QE::unpack2(w.y);
-        qf[ks][0] = mine ? CE::pack2(f0.x, f0.y) : 0u;
-        qf[ks][1] = mine ? CE::pack2(f1.x, f1.y) : 0u;
+        qf[ks][0] = mine ? w.x : 0u;
+        qf[ks][1] = mine ? w.y : 0u;
       }
+    }
+  }
+  // bf16 queries become fp16 operands: exactly, after each (head, map) has been brought to a largest magnitude of 2^14 .. 2^15 by a power of two,
+  // which the scores take back. What lies more than 2^31 below a query's largest element is rounded.
+  float q_back[NT][2];  // columns 2t, 2t + 1
+  if constexpr (C::SCALED_Q) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int k0 = n * (HD / 32), k1 = NT == 1 ? HD / 16 : k0 + HD / 32;
+      uint32_t top = 0;  // of |q|, as bits: bf16 pairs
+#pragma unroll
+      for (int ks = 0; ks < HD / 16; ++ks)
+        if (ks >= k0 && ks < k1) top = __vmaxu2(__vmaxu2(top, qf[ks][0] & 0x7FFF7FFFu), qf[ks][1] & 0x7FFF7FFFu);
+      top = max(top & 0xFFFFu, top >> 16);
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const int up = min(14 + 127 - int(top >> 7), 126);  // log2 of the factor
+      const float f = __uint_as_float(uint32_t(127 + up) << 23), back = __uint_as_float(uint32_t(127 - up) << 23);
+#pragma unroll
+      for (int ks = 0; ks < HD / 16; ++ks)
+        if (ks >= k0 && ks < k1) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float2 x = QE::unpack2(qf[ks][i]);
+            qf[ks][i] = CE::pack2(x.x * f, x.y * f);
+          }
+        }
+      q_back[n][0] = __shfl_sync(0xffffffffu, back, 8 * t), q_back[n][1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);
     }
   }
 
@@ -231,8 +259,9 @@ __global__ void __launch_bounds__(C::NW * 32, C::CTAS) diff_decode_kernel(const 
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       // lane: (key g, columns 2t, 2t + 1), (key g + 8, the same)
-      float s0 = (s[n][0][0] + s[n][1][0]) * sc, s1 = (s[n][0][1] + s[n][1][1]) * sc;
-      float s2 = (s[n][0][2] + s[n][1][2]) * sc, s3 = (s[n][0][3] + s[n][1][3]) * sc;
+      const float sc0 = C::SCALED_Q ? sc * q_back[n][0] : sc, sc1 = C::SCALED_Q ? sc * q_back[n][1] : sc;
+      float s0 = (s[n][0][0] + s[n][1][0]) * sc0, s1 = (s[n][0][1] + s[n][1][1]) * sc1;
+      float s2 = (s[n][0][2] + s[n][1][2]) * sc0, s3 = (s[n][0][3] + s[n][1][3]) * sc1;
       if (out_lo) s0 = s1 = -INFINITY;
       if (out_hi) s2 = s3 = -INFINITY;
       float x0 = fmaxf(s0, s2), x1 = fmaxf(s1, s3);

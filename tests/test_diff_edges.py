@@ -141,3 +141,19 @@ def test_a_page_of_large_values_that_is_hardly_attended(HD, rows, split):
             assert np.allclose(O64[:, cols], fac * D, rtol=1e-9, atol=1e-12)
             err = np.abs(got[:, cols] - O64[:, cols])
             assert (err <= tol).all(), (ran, float((err / tol).max()), float(np.abs(got[:, cols]).max()))
+
+
+@gpu
+@pytest.mark.parametrize("power", [-40, 0, 30])
+@pytest.mark.parametrize("heads", [(8, 2), (8, 1)], ids=["4 heads", "8 heads"])
+@pytest.mark.parametrize("HD", [128, 256])
+def test_queries_of_every_magnitude_over_e4m3(HD, heads, power):
+    """bf16 queries far outside fp16's range, their keys as far the other way: the scores are ordinary. One head is all zeros."""
+    w = wl.make_pass("magnitude", 24, [(100, 1), (33, 1), (0, 1)], heads[0], heads[1], HD, 16, wl.BF16, wl.E4M3, scale=(HD // 2) ** -0.5)
+    f = np.float32(2.0 ** power)
+    Q = wl.from_bits16(w.Q, wl.BF16) * f
+    Q[0, :HD] = 0.0
+    w.Q = wl.to_bits16(Q, wl.BF16)
+    w.Kb = wl.to_bits16(wl.from_bits16(w.Kb, wl.BF16) / f, wl.BF16)
+    w.kv_scales[:, 0] /= f
+    _check(w, "diff_decode")

@@ -160,7 +160,8 @@ int check_params(const esp_attn_ctx* c, const esp_attn_params& p) { return check
 
 bool windowed_lists(const esp_attn_args& a) { return a.qsa_tlist != nullptr; }
 
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+bool aligned_to(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+bool aligned16(const void* p) { return aligned_to(p, 16); }
 
 }  // namespace
 
@@ -1134,6 +1135,8 @@ int esp::check_kv_append(const esp_attn_shape& s, const esp_kv_append_args& a) {
   if (a.maps != 1 && a.maps != 2) return fail(ESP_ERR_INVALID, "esp_kv_append: maps=%d (1 or 2)", a.maps);
   if (a.rot_half < 0 || 2 * int64_t(a.rot_half) > s.HD / a.maps) return fail(ESP_ERR_INVALID, "esp_kv_append: rot_half=%d (2 * rot_half <= %d)", a.rot_half, s.HD / a.maps);
   if (a.rot_half > 0 && (!a.pos || !a.inv_freq)) return fail(ESP_ERR_INVALID, "esp_kv_append: a rotation needs pos and inv_freq");
+  if (!aligned_to(a.pos, 4) || !aligned_to(a.inv_freq, 4) || !aligned_to(a.kv_scales, 4))
+    return fail(ESP_ERR_INVALID, "esp_kv_append: pos, inv_freq and kv_scales must be aligned to their types");
   const int64_t ssz = a.src_f32 ? 4 : 2;
   const struct { const void* p; int64_t ld, heads, align; const char* name; } src[3] = {
       {a.Q, a.q_src_ld, s.H, ssz, "Q"}, {a.K, a.k_src_ld, s.Hkv, ssz, "K"}, {a.V, a.v_src_ld, s.Hkv, ssz, "V"}};
@@ -1166,6 +1169,10 @@ int esp::check_diff_pass(const esp_attn_shape& s, int TR, bool deep, const esp_a
   if (!d.lam || (d.lam_ld != 0 && d.lam_ld < s.H)) return fail(ESP_ERR_INVALID, "esp_diff_forward: lam is null, or lam_ld=%d (0, or >= H=%d)", d.lam_ld, s.H);
   if (!(d.eps >= 0.0f) || !(d.out_scale == d.out_scale)) return fail(ESP_ERR_INVALID, "esp_diff_forward: eps / out_scale");
   if (!aligned16(d.norm_w)) return fail(ESP_ERR_INVALID, "esp_diff_forward: norm_w must be 16-byte aligned");
+  // records are read 16 bytes at a time
+  if (!aligned16(a.tiles) || !aligned16(a.trees) || !aligned16(a.desc)) return fail(ESP_ERR_INVALID, "esp_diff_forward: tiles, trees and desc must be 16-byte aligned");
+  if (!aligned_to(a.anc_mask, 8) || !aligned_to(a.jobs, 4) || !aligned_to(a.blocks, 4) || !aligned_to(a.kv_scales, 4) || !aligned_to(d.lam, 4))
+    return fail(ESP_ERR_INVALID, "esp_diff_forward: anc_mask, jobs, blocks, kv_scales and lam must be aligned to their types");
   if (int rc = check_params(s, a.p)) return rc;
   return esp::validate_pass(s, TR, deep, a);
 }

@@ -509,8 +509,8 @@ int esp_kv_append(esp_attn_ctx* ctx, void* stream, const esp_kv_append_args* arg
  * Passes of one context may overlap on the GPU - two streams, two graphs - while their O, parts and dequant_scratch are apart.
  * A row that sees no key gets zeros. Rows that no tile covers are left as they were. Keys behind a tree's last row, pool rows past P and,
  * with ancestor masks, rows in nobody's mask are never mixed in, whatever they hold; keys that another row of the same tree sees must be
- * finite. desc records may say "no ancestors" or "the whole tree" by any number below 0 or above M, "sees nothing of the pass" by a
- * segment start behind the row.
+ * finite. tiles, trees and desc are 16-byte aligned. desc records may say "no ancestors" or "the whole tree" by any number below 0 or
+ * above M, "sees nothing of the pass" by a segment start behind the row.
  * Kernels: "diff_decode" (all trees have one row, G <= 8, HD 128 or 256, pages of 16 n keys), "diff_umma"
  * (HD 128 or 256, pages of 16 n keys, tile ranges that start at a multiple of 16) for tiles of 16, 32, 64 or 128 rows, 128 / tile_rows
  * heads of one kv head each (16-bit pools; E4M3 pools through dequant_scratch, sized as for esp_attn_forward; passes without

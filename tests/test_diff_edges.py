@@ -157,3 +157,40 @@ def test_queries_of_every_magnitude_over_e4m3(HD, heads, power):
     w.Kb = wl.to_bits16(wl.from_bits16(w.Kb, wl.BF16) / f, wl.BF16)
     w.kv_scales[:, 0] /= f
     _check(w, "diff_decode")
+
+
+# ---------------------------------------------------------------------------------------------- without a GPU
+def _append_args(**more):
+    a = capi.AppendArgs(Q=0x10000, K=0x20000, V=0x30000, Qo=0x40000, Kb=0x50000, Vb=0x60000, kv=0x70000, kv_scales=0x80000, slots=0x90000, pos=0xA0000, inv_freq=0xB0000,
+                        q_src_ld=1536, k_src_ld=1536, v_src_ld=1536, rows=4, maps=1, rot_half=64, n_blocks=9, qscale=1.0)
+    a.p = capi.Params(8, 2, 1024, 256, 0, 16, 0)
+    for k, v in more.items():
+        setattr(a, k, v)
+    return a
+
+
+def _diff_args(trees, plan, /, **more):
+    a = capi.Args(Q=0x10000, Kb=0x20000, Vb=0x30000, kv=0x40000, kv_scales=0x48000, blocks=0x50000, desc=0x60000, anc_mask=0x68000, O=0x70000, tiles=0x80000, trees=0x90000,
+                  jobs=0x98000, tiles_host=plan.tiles.ctypes.data, trees_host=trees.ctypes.data, n_tiles=len(plan.tiles), n_trees=len(trees),
+                  n_rows=int(trees["M"].sum()), n_blocks=9, n_block_entries=3)
+    a.p = capi.Params(8, 2, 1024, 256, 2048, 16, 0)
+    for k, v in more.items():
+        setattr(a, k, v)
+    return a
+
+
+def test_misaligned_pointers_are_refused(call_checks):  # noqa: F811
+    """What the kernels read in words of 4, 8 or 16 bytes has to lie on their multiples: anything else faults on the device."""
+    shape = capi.Shape(8, 2, 128, 16, wl.BF16, wl.E4M3, 8, 0, 0.125)
+    assert call_checks.append(shape, _append_args()) == 0
+    for name in ("pos", "inv_freq", "kv_scales"):
+        for off in (1, 2):
+            assert call_checks.append(shape, _append_args(**{name: getattr(_append_args(), name) + off})) == capi.ESP_ERR_INVALID, name
+    trees = host.make_trees([4, 1], [20, 3], [0, 2])
+    plan = host.plan_tiles(trees, 2)
+    good, d = _diff_args(trees, plan), capi.DiffArgs(0x100000, 0x110000, 0, 1e-5, 1.0)
+    assert call_checks.diff(shape, good, d) == 0
+    for name, unit in (("tiles", 16), ("trees", 16), ("desc", 16), ("anc_mask", 8), ("jobs", 4), ("blocks", 4), ("kv_scales", 4)):
+        assert call_checks.diff(shape, _diff_args(trees, plan, **{name: getattr(good, name) + unit // 2}), d) == capi.ESP_ERR_INVALID, name
+        assert call_checks.diff(shape, _diff_args(trees, plan, **{name: getattr(good, name) + unit}), d) == 0, name
+    assert call_checks.diff(shape, good, capi.DiffArgs(0x100002, 0x110000, 0, 1e-5, 1.0)) == capi.ESP_ERR_INVALID

@@ -15,7 +15,7 @@ import numpy as np
 import torch
 
 from . import capi
-from .workloads import COMBINE_DT, E4M3, F16, KVSAVE_DT, TILE_DT, TREE_DT, Workload
+from .workloads import BF16, COMBINE_DT, E4M3, F16, KVSAVE_DT, TILE_DT, TREE_DT, Workload
 
 
 @dataclass
@@ -77,12 +77,31 @@ def diff_plan_options(trees: np.ndarray, H: int, Hkv: int, HD: int, kv_dtype: in
     return o.tile_rows, dict(mode=o.mode, split=o.split, min_chunk=o.min_chunk, groups=o.groups, tile_rows=o.tile_rows, max_parts=o.max_parts)
 
 
-def _check_rows(name: str, t, ld: int | None = None):
+_INT32, _F32, _BITS16 = (torch.int32,), (torch.float32,), (torch.int16, torch.uint16)
+_ROWS = {F16: (torch.float16,) + _BITS16, BF16: (torch.bfloat16,) + _BITS16}  # rows of a context's 16-bit type, or their bits
+_POOL = {**_ROWS, E4M3: (torch.uint8, torch.int8, torch.float8_e4m3fn)}
+
+
+def _check(name: str, t, device, dtypes, numel: int):
+    """A flat array of a call: the kernels read `numel` elements from its address, whatever lies there."""
+    if t is None:
+        return
+    if t.device != device or t.dtype not in dtypes:
+        raise ValueError(f"{name}: a tensor of {' / '.join(str(d) for d in dtypes)} on {device} expected, not {t.dtype} on {t.device}")
+    if t.numel() < numel or not t.is_contiguous():
+        raise ValueError(f"{name}: {numel} contiguous elements expected, not {tuple(t.shape)} with strides {tuple(t.stride())}")
+
+
+def _check_rows(name: str, t, device, dtypes, rows: int, width: int, ld: int | None = None):
     """Rows of contiguous elements, `ld` elements apart where the call takes no stride for them."""
     if t is None:
         return
     if t.dim() != 2 or t.stride(1) != 1 or (ld is not None and t.shape[0] > 1 and t.stride(0) != ld):
         raise ValueError(f"{name}: rows of contiguous elements{'' if ld is None else f', {ld} apart,'} expected, not strides {tuple(t.stride())}")
+    if t.device != device or t.dtype not in dtypes:
+        raise ValueError(f"{name}: a tensor of {' / '.join(str(d) for d in dtypes)} on {device} expected, not {t.dtype} on {t.device}")
+    if t.shape[0] < rows or t.shape[1] < width:
+        raise ValueError(f"{name}: {rows} rows of {width} elements expected, not {tuple(t.shape)}")
 
 
 @dataclass
@@ -308,17 +327,27 @@ class AttnOp:
 
     def append_call(self, Q, K, V, Qo=None, Kb=None, Vb=None, kv=None, kv_scales=None, n_blocks=0, slots=None, pos=None, inv_freq=None,
                     maps=1, adjacent=False, qscale=1.0, kv_base=0) -> Call:
-        """Arguments of esp_kv_append from device tensors: Q / K / V are [rows, heads * HD] with any row stride, 16-bit or fp32."""
-        s, a = self.shape, capi.AppendArgs()
-        for name, t in (("Q", Q), ("K", K), ("V", V)):
-            _check_rows(name, t)
-        _check_rows("Kb", Kb, s.Hkv * s.HD)
-        _check_rows("Vb", Vb, s.Hkv * s.HD)
-        _check_rows("Qo", Qo)
+        """Arguments of esp_kv_append from device tensors: Q / K / V are [rows, heads * HD] with any row stride, all of the context's 16-bit type (or its
+        bits as int16) or all fp32; types, lengths and devices are checked."""
+        s, a, dev, rows = self.shape, capi.AppendArgs(), self.device, K.shape[0]
+        row16, kv_ld = _ROWS[s.q_dtype], s.Hkv * s.HD
+        src = _F32 if K.dtype == torch.float32 else row16
+        _check_rows("Q", Q, dev, src, rows, s.H * s.HD)
+        _check_rows("K", K, dev, src, rows, kv_ld)
+        _check_rows("V", V, dev, src, rows, kv_ld)
+        _check_rows("Qo", Qo, dev, row16, rows, s.H * s.HD)
+        _check_rows("Kb", Kb, dev, row16, rows, kv_ld, kv_ld)
+        _check_rows("Vb", Vb, dev, row16, rows, kv_ld, kv_ld)
+        if kv is not None:
+            _check("kv", kv, dev, _POOL[s.kv_dtype], kv_base + n_blocks * 2 * s.bt * kv_ld)
+            _check("kv_scales", kv_scales, dev, _F32, n_blocks * 2 * s.Hkv)
+            _check("slots", slots, dev, _INT32, 2 * rows)
+        _check("pos", pos, dev, _INT32, rows)
+        _check("inv_freq", inv_freq, dev, _F32, 0)
         a.Q, a.K, a.V, a.Qo, a.Kb, a.Vb = (_ptr(t) for t in (Q, K, V, Qo, Kb, Vb))
         a.kv, a.kv_scales, a.slots, a.pos, a.inv_freq = (_ptr(t) for t in (kv, kv_scales, slots, pos, inv_freq))
         a.q_src_ld, a.k_src_ld, a.v_src_ld = 0 if Q is None else Q.stride(0), K.stride(0), V.stride(0)
-        a.rows, a.src_f32, a.maps, a.adjacent = K.shape[0], int(K.dtype == torch.float32), maps, int(adjacent)
+        a.rows, a.src_f32, a.maps, a.adjacent = rows, int(src is _F32), maps, int(adjacent)
         a.rot_half, a.n_blocks, a.qscale = 0 if inv_freq is None else inv_freq.numel(), n_blocks, qscale
         a.p = capi.Params(s.H, s.Hkv, s.H * s.HD if Qo is None else Qo.stride(0), s.Hkv * s.HD, 2 * s.H * s.HD, s.bt, kv_base)
         return Call(a, None, (Q, K, V, Qo, Kb, Vb, kv, kv_scales, slots, pos, inv_freq))
@@ -336,12 +365,21 @@ class AttnOp:
     def diff_call(self, plan: Plan, trees: np.ndarray, Q, Kb, Vb, O, kv=None, kv_scales=None, blocks=None, n_blocks=0, desc=None,
                   anc_mask=None, lam=None, lam_ld=0, norm_w=None, eps=0.0, out_scale=1.0, kv_base=0, parts=None, scratch=None) -> Call:
         """Arguments of esp_diff_forward from a plan and device tensors; `parts` (and, over an E4M3 pool, the scratch of
-        multi-row passes) are allocated unless given."""
-        s, a = self.shape, capi.Args()
-        _check_rows("Q", Q)
-        _check_rows("O", O, Q.stride(0))
-        _check_rows("Kb", Kb, s.Hkv * s.HD)
-        _check_rows("Vb", Vb, s.Hkv * s.HD)
+        multi-row passes) are allocated on torch's current stream unless given. Types, lengths and devices are checked."""
+        s, a, dev, rows, row16, kv_ld = self.shape, capi.Args(), self.device, Q.shape[0], _ROWS[self.shape.q_dtype], self.shape.Hkv * self.shape.HD
+        _check_rows("Q", Q, dev, row16, rows, s.H * s.HD)
+        _check_rows("O", O, dev, row16, rows, s.H * s.HD, Q.stride(0))
+        _check_rows("Kb", Kb, dev, row16, rows, kv_ld, kv_ld)
+        _check_rows("Vb", Vb, dev, row16, rows, kv_ld, kv_ld)
+        _check("kv", kv, dev, _POOL[s.kv_dtype], kv_base + n_blocks * 2 * s.bt * kv_ld)
+        _check("kv_scales", kv_scales, dev, _F32, n_blocks * 2 * s.Hkv)
+        _check("blocks", blocks, dev, _INT32, 0)
+        _check("desc", desc, dev, _INT32, 4 * rows)
+        _check("anc_mask", anc_mask, dev, (torch.int64, torch.uint64), rows)
+        _check("lam", lam, dev, _F32, s.H + max(lam_ld, 0) * max(rows - 1, 0))
+        _check("norm_w", norm_w, dev, _F32, s.HD)
+        _check("parts", parts, dev, _F32, int(self.lib.esp_diff_parts_floats(C.byref(s), plan.n_parts)))
+        _check("scratch", scratch, dev, (torch.uint8,), 0)
         trees = np.ascontiguousarray(trees, dtype=TREE_DT)
         tiles_dev, trees_dev, jobs_dev = (_dev(x, self.device) if len(x) else None for x in (plan.tiles, trees, plan.jobs))
         if parts is None and plan.n_parts:
@@ -369,12 +407,20 @@ class AttnOp:
             capi.check(rc)
 
     def diff_lambda(self, q1, k1, q2, k2, lambda_init: float, H: int | None = None, stream: int | None = None):
-        """esp_diff_lambda: [H, dim] vectors, or one [dim] vector for every head."""
-        s = torch.cuda.current_stream(self.device).cuda_stream if stream is None else stream
+        """esp_diff_lambda: [H, dim] vectors, or one [dim] vector for every head, all laid out alike."""
         n = self.shape.H if H is None else H
-        lam = torch.empty(n, dtype=torch.float32, device=self.device)
-        ld = 0 if q1.dim() == 1 else q1.stride(0)
-        capi.check(self.lib.esp_diff_lambda(C.c_void_p(s), _ptr(q1), _ptr(k1), _ptr(q2), _ptr(k2), n, q1.shape[-1], ld, lambda_init, _ptr(lam)))
+        for name, t in (("q1", q1), ("k1", k1), ("q2", q2), ("k2", k2)):
+            if t.shape != q1.shape or t.stride() != q1.stride():
+                raise ValueError(f"{name}: shape and strides of q1 expected, {tuple(q1.shape)} with {tuple(q1.stride())}, not {tuple(t.shape)} with {tuple(t.stride())}")
+            if t.dim() == 1:
+                _check(name, t, self.device, _F32, 1)
+            else:
+                _check_rows(name, t, self.device, _F32, n, 1)
+        ld = 0 if q1.dim() == 1 else max(q1.stride(0), q1.shape[-1])
+        with torch.cuda.device(self.device), torch.cuda.stream(None if stream is None else torch.cuda.ExternalStream(stream, self.device)):
+            lam = torch.empty(n, dtype=torch.float32, device=self.device)
+            capi.check(self.lib.esp_diff_lambda(C.c_void_p(torch.cuda.current_stream().cuda_stream), _ptr(q1), _ptr(k1), _ptr(q2), _ptr(k2), n, q1.shape[-1], ld, lambda_init,
+                                                _ptr(lam)))
         return lam
 
     def kv_save(self, dp: DevicePass, entries: np.ndarray, stream: int | None = None):

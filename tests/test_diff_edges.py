@@ -194,3 +194,76 @@ def test_misaligned_pointers_are_refused(call_checks):  # noqa: F811
         assert call_checks.diff(shape, _diff_args(trees, plan, **{name: getattr(good, name) + unit // 2}), d) == capi.ESP_ERR_INVALID, name
         assert call_checks.diff(shape, _diff_args(trees, plan, **{name: getattr(good, name) + unit}), d) == 0, name
     assert call_checks.diff(shape, good, capi.DiffArgs(0x100002, 0x110000, 0, 1e-5, 1.0)) == capi.ESP_ERR_INVALID
+
+
+def _bare(kv_dtype=wl.BF16):
+    """An AttnOp without a context: it makes calls of CPU tensors, which nothing here launches."""
+    op = object.__new__(host.AttnOp)
+    op.lib, op.device, op.shape = capi.load(), torch.device("cpu"), capi.Shape(8, 2, 128, 16, wl.BF16, kv_dtype, 8, 0, 0.125)
+    return op
+
+
+
+
+@pytest.mark.parametrize("pool", [wl.BF16, wl.E4M3], ids=["16-bit", "e4m3"])
+def test_append_tensors_of_other_types_and_lengths_are_refused(pool):
+    """The kernel reads rows of its own types from the addresses it gets: another type is read as garbage, a shorter tensor past its end."""
+    op, n, z = _bare(pool), 5, torch.zeros
+    kv = z(9 * 2 * 16 * 256, dtype=torch.uint8 if pool == wl.E4M3 else torch.bfloat16)
+    good = dict(Q=z(n, 1024, dtype=torch.bfloat16), K=z(n, 256, dtype=torch.bfloat16), V=z(n, 256, dtype=torch.bfloat16), Qo=z(n, 1024, dtype=torch.bfloat16),
+                Kb=z(n, 256, dtype=torch.bfloat16), Vb=z(n, 256, dtype=torch.bfloat16), kv=kv, kv_scales=z(9, 2, 2) if pool == wl.E4M3 else None, n_blocks=9,
+                slots=z(n, 2, dtype=torch.int32), pos=z(n, dtype=torch.int32), inv_freq=z(64))
+    more = [(name, good[name].to(t)) for name in ("Q", "V", "Qo", "Kb", "Vb") for t in (torch.float16, torch.float32, torch.int32)]
+    more += [(name, good[name][:n - 1]) for name in ("Q", "V", "Qo", "Kb", "Vb", "slots", "pos")]
+    more += [(name, good[name][:, :255]) for name in ("Q", "K", "V", "Qo")] + [("Kb", good["Kb"][:, :128]), ("Vb", good["Vb"][:, :128].contiguous())]
+    more += [("slots", good["slots"].long()), ("pos", good["pos"].long()), ("pos", z(2 * n, dtype=torch.int32)[::2]), ("inv_freq", good["inv_freq"].double()),
+             ("inv_freq", z(128)[::2]), ("kv", kv[1:]), ("kv", kv.float()), ("n_blocks", 10)]
+    if pool == wl.E4M3:
+        more += [("kv_scales", z(8, 2, 2)), ("kv_scales", z(9, 2, 2).double())]
+    more += [(name, torch.empty_like(good[name], device="meta")) for name in ("Q", "K", "V", "Qo", "Kb", "Vb", "kv", "slots", "pos", "inv_freq")]
+    for name, bad in more:
+        call = dict(good, **{name: bad})
+        with pytest.raises(ValueError, match="^(kv|K|V|Q|%s)" % name):  # a wrong K may show at the tensors that have to go with it
+            op.append_call(**call)
+    op.append_call(**good)
+    f32 = {k: good[k].float() for k in "QKV"}
+    assert op.append_call(**dict(good, **f32)).args.src_f32 == 1
+    bits = {k: good[k].view(torch.int16) for k in ("Q", "K", "V", "Qo", "Kb", "Vb")}
+    assert op.append_call(**dict(good, **bits)).args.src_f32 == 0
+    assert op.append_call(None, good["K"], good["V"], Kb=good["Kb"], Vb=good["Vb"]).args.rot_half == 0
+
+
+@pytest.mark.parametrize("pool", [wl.BF16, wl.E4M3], ids=["16-bit", "e4m3"])
+def test_attention_tensors_of_other_types_and_lengths_are_refused(pool):
+    op, n, z = _bare(pool), 5, torch.zeros
+    trees = host.make_trees([4, 1], [200, 3], [0, 13])
+    plan = host.plan_tiles(trees, 2, mode=capi.ESP_PLAN_B200, split=1 << 20, min_chunk=16, groups=64)
+    assert plan.n_parts
+    kv = z(9 * 2 * 16 * 256, dtype=torch.uint8 if pool == wl.E4M3 else torch.int16)
+    parts = int(op.lib.esp_diff_parts_floats(C.byref(op.shape), plan.n_parts))
+    good = dict(Q=z(n, 1024, dtype=torch.bfloat16), Kb=z(n, 256, dtype=torch.bfloat16), Vb=z(n, 256, dtype=torch.int16), O=z(n, 1024, dtype=torch.bfloat16), kv=kv, n_blocks=9,
+                kv_scales=z(9, 2, 2) if pool == wl.E4M3 else None, blocks=z(14, dtype=torch.int32), desc=z(n, 4, dtype=torch.int32), anc_mask=z(n, dtype=torch.int64), lam=z(8),
+                norm_w=z(128), parts=z(parts), scratch=z(8, dtype=torch.uint8))
+    more = [(name, good[name].to(t)) for name in ("Q", "Kb", "Vb", "O") for t in (torch.float16, torch.float32, torch.int64)]
+    more += [(name, good[name][:n - 1]) for name in ("Kb", "Vb", "O", "desc", "anc_mask")] + [("O", good["O"][:, :1016]), ("Q", z(n, 1016, dtype=torch.bfloat16))]
+    more += [("blocks", good["blocks"].long()), ("desc", good["desc"].long()), ("desc", good["desc"].t()), ("anc_mask", good["anc_mask"].int()), ("lam", z(7)), ("lam", z(8).double()),
+             ("norm_w", z(127)), ("norm_w", z(128, dtype=torch.bfloat16)), ("parts", z(parts - 1)), ("parts", z(parts).double()), ("kv", kv[1:]), ("kv", kv.float()),
+             ("scratch", z(8)), ("kv_scales", z(8, 2, 2)), ("kv_scales", z(9, 2, 2).half())]
+    more += [(name, torch.empty_like(t, device="meta")) for name, t in good.items() if isinstance(t, torch.Tensor)]
+    for name, bad in more:
+        with pytest.raises(ValueError, match="^(O|%s)" % name):
+            op.diff_call(plan, trees, **dict(good, **{name: bad}))
+    op.diff_call(plan, trees, **good)
+    op.diff_call(plan, trees, **dict(good, lam=z(n, 8), lam_ld=8))
+    with pytest.raises(ValueError, match="^lam"):
+        op.diff_call(plan, trees, **dict(good, lam=z(n - 1, 8), lam_ld=8))
+
+
+def test_lambda_vectors_laid_out_differently_are_refused():
+    op, z = _bare(), torch.zeros
+    for more in (dict(k1=z(8, 65)[:, :64]), dict(q2=z(7, 64)), dict(k2=z(8, 64).half()), dict(q1=z(64)), dict(k1=z(64, 8).t())):
+        v = dict(dict(q1=z(8, 64), k1=z(8, 64), q2=z(8, 64), k2=z(8, 64)), **more)
+        with pytest.raises(ValueError, match="^[qk][12]"):
+            op.diff_lambda(lambda_init=0.1, **v)
+    with pytest.raises(ValueError, match="^q1"):
+        op.diff_lambda(z(4, 64), z(4, 64), z(4, 64), z(4, 64), lambda_init=0.1)

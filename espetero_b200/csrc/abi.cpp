@@ -1237,22 +1237,26 @@ int esp_diff_plan_opts(const esp_attn_shape* s, const esp_attn_tree* trees, int3
     return ESP_OK;
   }
   // diff_umma: how many heads of a kv head share a tile, and - where cached keys are most of the work - how far to split them, by the
-  // time each choice would take: CTAs (two per tile and head group) on the SMs' slots, a fixed cost per CTA and one per 128 keys,
-  // and the join of the records. Microseconds, measured; with 128-dim heads two CTAs share an SM and each runs slower than
-  // alone. 700 rows behind 20001 keys, 8 kv heads, took 525 us unsplit, 484 in two, 515 in three and 533 in four parts; the rule
-  // gives 523, 475, 506 and 532. Small prompts share their tiles between heads: 4 x 33 rows, 256 dims, 24.5 us in tiles of one head, 13.0 of two;
-  // 8 x 20 .. 100 rows, 128 dims, 24.2 us of one, 21.0 of two, 13.8 of four. Near ties keep taller tiles and fewer parts (without a cached prefix
-  // ties within a tenth: 2 x 8192 and 5 x 33 .. 4001 rows measured 1 to 4 % faster in tiles of one head).
+  // time each choice would take: CTAs (two per tile and head group) on the SMs' slots, a fixed cost per CTA, one per 128 keys and one for its
+  // records, and the join. Microseconds, measured; with 128-dim heads two CTAs share an SM and each runs slower than alone. Every height is
+  // searched with its own splits: 16 rows behind 16384 keys, 4 kv heads of 8, 128 dims, take 67 us in 4 parts of 128-row tiles, 30 in 16 parts
+  // of 16-row tiles; 5 rows behind 32768 keys 121 and 29. Over 75 passes of 1 .. 16 prompts and trees behind 200 .. 100000 keys (all heights,
+  // 1 .. 32 parts) the choice is 1.05 times the best one's time in the geometric mean, 1.33 times at most. 700 rows behind 20001 E4M3 keys, 8 kv heads: 508 us
+  // unsplit, 477 in two parts, 508 in three; it takes two. Small prompts share their tiles between heads: 4 x 33 rows, 256 dims, 24.5 us in tiles of
+  // one head, 13.0 of two; 8 x 20 .. 100 rows, 128 dims, 24.2 us of one, 21.0 of two, 13.8 of four. Near ties keep taller tiles and fewer parts
+  // (without a cached prefix ties within a tenth: 2 x 8192 and 5 x 33 .. 4001 rows measured 1 to 4 % faster in tiles of one head).
   const bool wide = s->HD >= 256, split = cached > 2 * fresh;
-  const double t_alone = wide ? 1.45 : 1.2, t_shared = wide ? 1.45 : 1.9, t_fixed = 9.0;  // per 128 keys alone / sharing an SM; start and end of a CTA
+  const double t_alone = wide ? 1.45 : 1.2, t_shared = wide ? 1.45 : 1.9, t_ends = 9.0;  // per 128 keys alone / sharing an SM; start and end of a CTA
+  const double t_records = 40000.0;  // bytes of records that a CTA writes in a microsecond, a lane per row
   const int64_t slots = wide ? 148 : 296;
   double best = 0;
   o->tile_rows = 0;
   for (int TR = 128; TR >= 16; TR >>= 1) {
     const int c = 128 / TR;
     if (c > G || G % c) continue;
+    double best_here = 0;
     for (int parts = 1; parts <= (split ? 32 : 1); ++parts) {
-      int64_t tiles = 0, blocks = 0, rows_split = 0, longest = 0;
+      int64_t tiles = 0, blocks = 0, rows_split = 0, longest = 0, lanes = 0;
       for (int i = 0; i < n_trees; ++i) {
         const esp_attn_tree& t = trees[i];
         const int64_t groups = (t.M + TR - 1) / TR, own = (int64_t(t.M) + 127) / 128;
@@ -1260,10 +1264,11 @@ int esp_diff_plan_opts(const esp_attn_shape* s, const esp_attn_tree* trees, int3
         const int64_t part = (t.P / ns + 127) / 128;
         tiles += groups * ns;
         blocks += groups * ns * part + groups * (own + 1) / 2;  // its own rows: a triangle
-        if (ns > 1) rows_split += int64_t(t.M) * ns;
+        if (ns > 1) rows_split += int64_t(t.M) * ns, lanes = std::max<int64_t>(lanes, std::min(t.M, TR) * c);
         longest = std::max(longest, part + (ns == 1 ? own : 1));
       }
       const int64_t ctas = tiles * (s->H / c) * 2, rest = ctas % slots;
+      const double t_fixed = t_ends + double(lanes) * (s->HD + 2) * 4 / t_records;
       double t;
       if (4 * longest * tiles <= 5 * blocks) {  // tiles of one length: wave by wave
         t = double(ctas / slots) * (double(longest) * t_shared + t_fixed);
@@ -1271,8 +1276,9 @@ int esp_diff_plan_opts(const esp_attn_shape* s, const esp_attn_tree* trees, int3
       } else {
         t = (double(blocks) * (s->H / c) * 2 * t_shared + double(ctas) * t_fixed) / double(slots) + 0.5 * double(longest) * t_alone + t_fixed;
       }
-      if (rows_split) t += 6.0 + double(rows_split) * s->H * 2 * (s->HD + 2) * 4 * 2 / 6.0e6;  // written and read at about 6 TB/s, mostly in L2
-      if (o->tile_rows && t > 1.5 * best) break;
+      if (rows_split) t += 1.0 + double(rows_split) * s->H * 2 * (s->HD + 2) * 4 * 2 / 6.0e6;  // written and read at about 6 TB/s, mostly in L2
+      if (best_here == 0 || t < best_here) best_here = t;
+      else if (t > 1.5 * best_here) break;  // more parts of this height only add records
       if (!o->tile_rows || t < (split ? 0.97 : 0.9) * best) {
         best = t;
         // the planner sizes its chunks so that the tiles fit `groups / Hkv`

@@ -267,3 +267,22 @@ def test_lambda_vectors_laid_out_differently_are_refused():
             op.diff_lambda(lambda_init=0.1, **v)
     with pytest.raises(ValueError, match="^q1"):
         op.diff_lambda(z(4, 64), z(4, 64), z(4, 64), z(4, 64), lambda_init=0.1)
+
+
+def _planned(rows, cached, H, Hkv, HD, kv_dtype=wl.BF16):
+    """(tile rows, parts of the longest list) that the options give."""
+    trees = host.make_trees(rows, cached, [0] * len(rows))
+    tile_rows, opts = host.diff_plan_options(trees, H, Hkv, HD, kv_dtype)
+    plan = host.plan_tiles(trees, Hkv, **opts)
+    return tile_rows, int(max(plan.jobs["nparts"])) if len(plan.jobs) else 1
+
+
+def test_few_rows_behind_a_long_prefix_share_tiles_and_split():
+    """One user's draft tree: the heads of a kv head share a tile, and the prefix is cut for the whole GPU."""
+    for rows, cached, HD in ((16, 16384, 128), (5, 32768, 128), (16, 16384, 256)):
+        tile_rows, parts = _planned([rows], [cached], 32, 4, HD)
+        assert tile_rows == 16 and parts >= 16, (rows, cached, HD, tile_rows, parts)
+    # what was planned well before stays: prompts in tiles of one head, a chunk in two parts, a batch of trees unsplit
+    assert _planned([8192] * 2, [0] * 2, 16, 4, 128) == (128, 1)
+    assert _planned([700], [20001], 32, 8, 128, wl.E4M3) == (64, 2)
+    assert _planned([16] * 16, [4096] * 16, 32, 4, 128) == (16, 1)

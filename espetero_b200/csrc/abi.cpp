@@ -1227,7 +1227,9 @@ int esp_diff_plan_opts(const esp_attn_shape* s, const esp_attn_tree* trees, int3
   *o = esp_plan_opts{};
   o->mode = ESP_PLAN_B200, o->min_chunk = 32, o->max_parts = 64;
   const int G = s->H / s->Hkv;
-  if (single) {
+  // diff_decode takes up to 8 heads to a kv head. Single rows of more run in diff_umma's tiles, 128 / tile_rows heads each: 32 tokens behind 4096 keys,
+  // 128 dims, 16 heads to one kv head 46 us, 9 heads 136 (diff_general, all that 8-row tiles leave: 446 and 430).
+  if (single && (G <= 8 || (s->HD != 128 && s->HD != 256))) {
     // diff_decode: one wave of its CTAs. Their rings are 192 KB for blocks of 16 keys of 256 16-bit dims, so one CTA fills an SM (7 sequences
     // of 1 .. 6001 keys, 8 kv heads: 13.2 us against 17.3 with two CTAs' worth of tiles); two do at half of that. At a quarter (E4M3,
     // 128 dims) four fit, and three leave batches that fill the SMs anyway unsplit (64 x 500 .. 3000 keys, 8 kv heads: 49.0 us against 57.7;

@@ -365,7 +365,7 @@ class AttnOp:
     def diff_call(self, plan: Plan, trees: np.ndarray, Q, Kb, Vb, O, kv=None, kv_scales=None, blocks=None, n_blocks=0, desc=None,
                   anc_mask=None, lam=None, lam_ld=0, norm_w=None, eps=0.0, out_scale=1.0, kv_base=0, parts=None, scratch=None) -> Call:
         """Arguments of esp_diff_forward from a plan and device tensors; `parts` (and, over an E4M3 pool, the scratch of
-        multi-row passes) are allocated on torch's current stream unless given. Types, lengths and devices are checked."""
+        multi-row tiles) are allocated on torch's current stream unless given. Types, lengths and devices are checked."""
         s, a, dev, rows, row16, kv_ld = self.shape, capi.Args(), self.device, Q.shape[0], _ROWS[self.shape.q_dtype], self.shape.Hkv * self.shape.HD
         _check_rows("Q", Q, dev, row16, rows, s.H * s.HD)
         _check_rows("O", O, dev, row16, rows, s.H * s.HD, Q.stride(0))
@@ -384,7 +384,7 @@ class AttnOp:
         tiles_dev, trees_dev, jobs_dev = (_dev(x, self.device) if len(x) else None for x in (plan.tiles, trees, plan.jobs))
         if parts is None and plan.n_parts:
             parts = torch.empty(int(self.lib.esp_diff_parts_floats(C.byref(s), plan.n_parts)), dtype=torch.float32, device=self.device)
-        if scratch is None and s.kv_dtype == E4M3 and blocks is not None and bool((trees["M"] > 1).any()) and bool((trees["P"] > 0).any()):
+        if scratch is None and s.kv_dtype == E4M3 and blocks is not None and bool((trees["P"] > 0).any()) and (s.H // s.Hkv > 8 or bool((trees["M"] > 1).any())):
             scratch = torch.empty(int(self.lib.esp_attn_dequant_scratch_bytes(C.byref(s), blocks.numel())), dtype=torch.uint8, device=self.device)
         a.Q, a.Kb, a.Vb, a.O, a.kv, a.kv_scales, a.blocks, a.desc, a.anc_mask, a.parts = (
             _ptr(t) for t in (Q, Kb, Vb, O, kv, kv_scales, blocks, desc, anc_mask, parts))

@@ -159,6 +159,16 @@ def test_queries_of_every_magnitude_over_e4m3(HD, heads, power):
     _check(w, "diff_decode")
 
 
+@gpu
+@pytest.mark.parametrize("types", [(wl.F16, None), (wl.BF16, wl.E4M3)], ids=["f16", "bf16-e4m3"])
+@pytest.mark.parametrize("heads", [(32, 2), (32, 1), (12, 1), (9, 1)], ids=lambda x: "H%d/%d" % x)
+@pytest.mark.parametrize("HD", [128, 256])
+def test_single_rows_of_many_heads(HD, heads, types):
+    """More than 8 query heads to a kv head, as the options plan them: on the tensor cores."""
+    w = wl.make_pass("many heads", 25, [(n, 1) for n in (0, 1, 15, 16, 17, 130, 333, 2000)], heads[0], heads[1], HD, 16, types[0], types[1], scale=(HD // 2) ** -0.5)
+    _check(w, "diff_umma")
+
+
 # ---------------------------------------------------------------------------------------------- without a GPU
 def _append_args(**more):
     a = capi.AppendArgs(Q=0x10000, K=0x20000, V=0x30000, Qo=0x40000, Kb=0x50000, Vb=0x60000, kv=0x70000, kv_scales=0x80000, slots=0x90000, pos=0xA0000, inv_freq=0xB0000,
@@ -286,3 +296,11 @@ def test_few_rows_behind_a_long_prefix_share_tiles_and_split():
     assert _planned([8192] * 2, [0] * 2, 16, 4, 128) == (128, 1)
     assert _planned([700], [20001], 32, 8, 128, wl.E4M3) == (64, 2)
     assert _planned([16] * 16, [4096] * 16, 32, 4, 128) == (16, 1)
+
+
+def test_single_rows_of_many_heads_are_planned_for_tiles_that_run_fast():
+    """diff_decode takes 8 heads to a kv head; tiles of 8 rows would leave the rest to diff_general."""
+    for H, Hkv, rows in ((32, 2, 16), (32, 1, 16), (12, 1, 32), (9, 1, 128)):
+        for kv_dtype in (wl.BF16, wl.E4M3):
+            assert _planned([1] * 8, [4096] * 8, H, Hkv, 128, kv_dtype)[0] == rows, (H, Hkv)
+    assert _planned([1], [4096], 32, 4, 128)[0] == 8 and _planned([1], [4096], 32, 1, 64)[0] == 8

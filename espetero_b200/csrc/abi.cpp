@@ -1221,7 +1221,7 @@ int esp_diff_plan_opts(const esp_attn_shape* s, const esp_attn_tree* trees, int3
   for (int i = 0; i < n_trees; ++i) {
     const esp_attn_tree& t = trees[i];
     if (t.M < 0 || t.P < 0) return fail(ESP_ERR_INVALID, "esp_diff_plan_opts: tree %d has a negative field", i);
-    single = single && t.M == 1;
+    single = single && t.M <= 1;  // a tree without rows (an idle slot of a batch) gets no tiles
     cached += int64_t(t.P) * t.M, fresh += int64_t(t.M) * t.M / 2;
   }
   *o = esp_plan_opts{};
@@ -1261,6 +1261,7 @@ int esp_diff_plan_opts(const esp_attn_shape* s, const esp_attn_tree* trees, int3
       int64_t tiles = 0, blocks = 0, rows_split = 0, longest = 0, lanes = 0;
       for (int i = 0; i < n_trees; ++i) {
         const esp_attn_tree& t = trees[i];
+        if (t.M == 0) continue;
         const int64_t groups = (t.M + TR - 1) / TR, own = (int64_t(t.M) + 127) / 128;
         const int ns = split && t.P >= 64 ? std::min(parts, std::max(1, t.P / 128)) : 1;
         const int64_t part = (t.P / ns + 127) / 128;
@@ -1317,7 +1318,7 @@ int esp_diff_forward(esp_attn_ctx* c, void* stream, const esp_attn_args* ap, con
   d.lam = dp->lam, d.norm_w = dp->norm_w, d.lam_ld = dp->lam_ld, d.eps = dp->eps, d.out_scale = dp->out_scale;
 
   bool single = a.trees_host != nullptr && a.tiles_host != nullptr;
-  for (int i = 0; single && i < a.n_trees; ++i) single = a.trees_host[i].M == 1;
+  for (int i = 0; single && i < a.n_trees; ++i) single = a.trees_host[i].M <= 1;
   const bool decode = single && c->opt_attn_gqa && esp::diff_decode_supports(s.HD, c->G, s.bt) && a.kv != nullptr && a.n_blocks > 0 &&
                       (size_t(a.p.kv_ld) * elem_bytes(s.kv_dtype)) % 128 == 0 && (a.p.kv_base * elem_bytes(s.kv_dtype)) % 128 == 0;
 

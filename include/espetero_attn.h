@@ -511,7 +511,7 @@ int esp_kv_append(esp_attn_ctx* ctx, void* stream, const esp_kv_append_args* arg
  * with ancestor masks, rows in nobody's mask are never mixed in, whatever they hold; keys that another row of the same tree sees must be
  * finite. tiles, trees and desc are 16-byte aligned. desc records may say "no ancestors" or "the whole tree" by any number below 0 or
  * above M, "sees nothing of the pass" by a segment start behind the row.
- * Kernels: "diff_decode" (all trees have one row, G <= 8, HD 128 or 256, pages of 16 n keys), "diff_umma"
+ * Kernels: "diff_decode" (no tree has more than one row, G <= 8, HD 128 or 256, pages of 16 n keys), "diff_umma"
  * (HD 128 or 256, pages of 16 n keys, tile ranges that start at a multiple of 16) for tiles of 16, 32, 64 or 128 rows, 128 / tile_rows
  * heads of one kv head each (16-bit pools; E4M3 pools through dequant_scratch, sized as for esp_attn_forward; passes without
  * cached keys), "diff_general" for everything else and for calls without the host mirrors of tiles and trees, plus "diff_combine"

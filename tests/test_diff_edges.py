@@ -169,6 +169,17 @@ def test_single_rows_of_many_heads(HD, heads, types):
     _check(w, "diff_umma")
 
 
+@gpu
+@pytest.mark.parametrize("pool", [None, wl.E4M3], ids=["16-bit", "e4m3"])
+@pytest.mark.parametrize("tile_rows", [None, 16])
+def test_idle_slots_of_a_batch(pool, tile_rows):
+    """Trees without rows beside single tokens: the same kernel as without them, and right."""
+    w = wl.make_pass("idle", 26, [(0, 0), (300, 1), (50, 0), (1, 1), (0, 0), (64, 1), (9, 0)], 8, 2, 128, 16, wl.BF16, pool, scale=0.125)
+    _check(w, "diff_decode", tile_rows=tile_rows)
+    w = wl.make_pass("idle rows", 26, [(0, 0), (300, 20), (50, 0), (1, 1)], 8, 2, 128, 16, wl.BF16, pool, scale=0.125)
+    _check(w, "diff_general" if tile_rows else "diff_umma", tile_rows=tile_rows)  # tiles of 16 rows want 8 heads to a kv head
+
+
 # ---------------------------------------------------------------------------------------------- without a GPU
 def _append_args(**more):
     a = capi.AppendArgs(Q=0x10000, K=0x20000, V=0x30000, Qo=0x40000, Kb=0x50000, Vb=0x60000, kv=0x70000, kv_scales=0x80000, slots=0x90000, pos=0xA0000, inv_freq=0xB0000,
@@ -304,3 +315,9 @@ def test_single_rows_of_many_heads_are_planned_for_tiles_that_run_fast():
         for kv_dtype in (wl.BF16, wl.E4M3):
             assert _planned([1] * 8, [4096] * 8, H, Hkv, 128, kv_dtype)[0] == rows, (H, Hkv)
     assert _planned([1], [4096], 32, 4, 128)[0] == 8 and _planned([1], [4096], 32, 1, 64)[0] == 8
+
+
+def test_idle_slots_do_not_change_the_plan():
+    for rows, cached in (([1] * 31, [4096] * 31), ([1], [100]), ([16] * 3, [4096, 9000, 5]), ([300], [0])):
+        idle_rows, idle_cached = [0] + rows + [0, 0], [700] + cached + [0, 4096]
+        assert _planned(idle_rows, idle_cached, 32, 4, 128) == _planned(rows, cached, 32, 4, 128)

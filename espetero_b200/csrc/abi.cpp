@@ -2,6 +2,7 @@
 // kernel selection and launches. Mirrors the attention() / kv_save() / kv_cow_copy()
 // dispatch code of the reference (src/model/impl/forest.h:2855-2947, :1438-1449).
 #include <algorithm>
+#include <climits>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -1262,9 +1263,9 @@ int esp_diff_plan_opts(const esp_attn_shape* s, const esp_attn_tree* trees, int3
       for (int i = 0; i < n_trees; ++i) {
         const esp_attn_tree& t = trees[i];
         if (t.M == 0) continue;
-        const int64_t groups = (t.M + TR - 1) / TR, own = (int64_t(t.M) + 127) / 128;
+        const int64_t groups = (int64_t(t.M) + TR - 1) / TR, own = (int64_t(t.M) + 127) / 128;
         const int ns = split && t.P >= 64 ? std::min(parts, std::max(1, t.P / 128)) : 1;
-        const int64_t part = (t.P / ns + 127) / 128;
+        const int64_t part = (int64_t(t.P) / ns + 127) / 128;
         tiles += groups * ns;
         blocks += groups * ns * part + groups * (own + 1) / 2;  // its own rows: a triangle
         if (ns > 1) rows_split += int64_t(t.M) * ns, lanes = std::max<int64_t>(lanes, std::min(t.M, TR) * c);
@@ -1285,7 +1286,7 @@ int esp_diff_plan_opts(const esp_attn_shape* s, const esp_attn_tree* trees, int3
       if (!o->tile_rows || t < (split ? 0.97 : 0.9) * best) {
         best = t;
         // the planner sizes its chunks so that the tiles fit `groups / Hkv`
-        o->tile_rows = TR, o->split = parts == 1 ? 0 : 1 << 20, o->groups = int(std::clamp<int64_t>(tiles, 1, 1 << 24)) * s->Hkv;
+        o->tile_rows = TR, o->split = parts == 1 ? 0 : 1 << 20, o->groups = int(std::clamp<int64_t>(tiles * s->Hkv, 1, INT_MAX));
       }
     }
   }

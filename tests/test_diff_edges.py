@@ -321,3 +321,10 @@ def test_idle_slots_do_not_change_the_plan():
     for rows, cached in (([1] * 31, [4096] * 31), ([1], [100]), ([16] * 3, [4096, 9000, 5]), ([300], [0])):
         idle_rows, idle_cached = [0] + rows + [0, 0], [700] + cached + [0, 4096]
         assert _planned(idle_rows, idle_cached, 32, 4, 128) == _planned(rows, cached, 32, 4, 128)
+
+
+def test_plan_options_of_the_largest_passes():
+    """Counts near 2^31 do not wrap: 2^24 tiles and more want as many places."""
+    for cached, H in ((0, 128), (2 ** 31 - 1, 256)):
+        tile_rows, o = host.diff_plan_options(host.make_trees([2 ** 31 - 1], [cached], [0]), H, 128, 128, wl.BF16)
+        assert tile_rows == 128 and o["groups"] >= 2 ** 24

@@ -69,7 +69,8 @@ def make_trees(rows, cached, tables) -> np.ndarray:
 
 
 def diff_plan_options(trees: np.ndarray, H: int, Hkv: int, HD: int, kv_dtype: int = F16):
-    """esp_diff_plan_opts: (tile_rows for the context, keyword arguments for plan_tiles)."""
+    """esp_diff_plan_opts: (tile_rows for the context, keyword arguments for plan_tiles). kv_dtype is the pool's type: single tokens over an E4M3 pool
+    planned as for a 16-bit one, the default, are slow (131072 keys of 8 heads, 256 dims: 149 us against 95). AttnOp.diff_plan knows it."""
     o = capi.PlanOpts()
     shape = capi.Shape(H, Hkv, HD, kv_dtype=kv_dtype)
     trees = np.ascontiguousarray(trees, dtype=TREE_DT)
@@ -361,6 +362,15 @@ class AttnOp:
         rc = self.lib.esp_kv_append(self.ctx, self._stream(stream), call.args)
         if rc:
             capi.check(rc)
+
+    def diff_plan(self, trees: np.ndarray) -> Plan:
+        """The plan that esp_diff_plan_opts asks for over this context's pool. A context's tile height is fixed: a pass that wants another one
+        (diff_plan_options names it) is refused, since it would run on the general kernel or in tiles that are mostly empty."""
+        s = self.shape
+        rows, opts = diff_plan_options(trees, s.H, s.Hkv, s.HD, s.kv_dtype)
+        if rows != s.tile_rows:
+            raise ValueError(f"diff_plan: this pass wants a context with tile_rows={rows}, not {s.tile_rows}")
+        return plan_tiles(trees, s.Hkv, **opts)
 
     def diff_call(self, plan: Plan, trees: np.ndarray, Q, Kb, Vb, O, kv=None, kv_scales=None, blocks=None, n_blocks=0, desc=None,
                   anc_mask=None, lam=None, lam_ld=0, norm_w=None, eps=0.0, out_scale=1.0, kv_base=0, parts=None, scratch=None) -> Call:

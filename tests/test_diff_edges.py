@@ -180,6 +180,16 @@ def test_idle_slots_of_a_batch(pool, tile_rows):
     _check(w, "diff_general" if tile_rows else "diff_umma", tile_rows=tile_rows)  # tiles of 16 rows want 8 heads to a kv head
 
 
+@gpu
+@pytest.mark.parametrize("heads", [(8, 2), (8, 1)], ids=["4 heads", "8 heads"])
+@pytest.mark.parametrize("HD", [128, 256])
+def test_e4m3_steps_as_they_are_planned(HD, heads):
+    """Plans for the pool's own type: three or two CTAs to an SM, uneven lengths split for them."""
+    w = wl.make_pass("planned", 27, [(n, 1) for n in (9000, 1, 2500, 0, 4097)], heads[0], heads[1], HD, 16, wl.BF16, wl.E4M3, scale=(HD // 2) ** -0.5)
+    assert _planned([1] * 5, w.trees["P"], *heads, HD, wl.E4M3)[1] > 8
+    _check(w, "diff_decode")
+
+
 # ---------------------------------------------------------------------------------------------- without a GPU
 def _append_args(**more):
     a = capi.AppendArgs(Q=0x10000, K=0x20000, V=0x30000, Qo=0x40000, Kb=0x50000, Vb=0x60000, kv=0x70000, kv_scales=0x80000, slots=0x90000, pos=0xA0000, inv_freq=0xB0000,
@@ -328,3 +338,18 @@ def test_plan_options_of_the_largest_passes():
     for cached, H in ((0, 128), (2 ** 31 - 1, 256)):
         tile_rows, o = host.diff_plan_options(host.make_trees([2 ** 31 - 1], [cached], [0]), H, 128, 128, wl.BF16)
         assert tile_rows == 128 and o["groups"] >= 2 ** 24
+
+
+def test_plans_know_the_type_of_the_pool():
+    """A context plans for its own pool: 131072 E4M3 keys of 8 kv heads and 256 dims for two CTAs to an SM, 16-bit ones for one. Passes that want
+    another tile height are refused."""
+    step, prompt = host.make_trees([1], [131072], [0]), host.make_trees([700], [0], [0])
+    for kv_dtype, ctas in ((wl.E4M3, 296), (wl.BF16, 148)):
+        op = _bare(kv_dtype)
+        op.shape = capi.Shape(32, 8, 256, 16, wl.BF16, kv_dtype, 8, 0, 0.088)
+        plan = op.diff_plan(step)
+        assert ctas - 8 <= len(plan.tiles) * 8 <= ctas and plan.tile_rows == 8
+        with pytest.raises(ValueError, match="tile_rows=128, not 8"):
+            op.diff_plan(prompt)
+        op.shape.tile_rows = 128
+        assert op.diff_plan(prompt).tile_rows == 128

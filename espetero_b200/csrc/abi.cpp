@@ -1347,7 +1347,17 @@ int esp_diff_forward(esp_attn_ctx* c, void* stream, const esp_attn_args* ap, con
     esp_attn_args w = a;  // the pool as the kernel sees it: 16-bit pages, or none
     if (widen) {
       ProfScope prof(c, st, "diff_widen");
-      e = esp::launch_diff_widen(k, a.dequant_scratch, a.n_block_entries, st, &c->launches);
+      int64_t pages = 0;
+      int32_t last = -1;
+      bool shared = false;  // tables that do not rise may be shared
+      for (int i = 0; i < a.n_trees; ++i) {
+        const esp_attn_tree& t = a.trees_host[i];
+        if (t.M <= 0 || t.P <= 0) continue;
+        pages += (int64_t(t.P) + s.bt - 1) / s.bt;
+        shared = shared || t.table <= last;
+        last = t.table;
+      }
+      e = esp::launch_diff_widen(k, a.dequant_scratch, std::min<int64_t>(pages, a.n_block_entries), shared, st, &c->launches);
       if (e != cudaSuccess) return cuda_fail(e, "diff_widen");
       w.kv = a.dequant_scratch, w.n_blocks = a.n_block_entries, w.p.kv_base = 0;
     } else if (!cached) {

@@ -190,6 +190,82 @@ def test_e4m3_steps_as_they_are_planned(HD, heads):
     _check(w, "diff_decode")
 
 
+def _apart(w, entries, fill):
+    """The same pass with `entries` table entries per tree, those that no tree reads set to `fill` (valid pages or not)."""
+    blocks = np.resize(np.asarray(fill, dtype=np.int32), len(w.trees) * entries)
+    for i, t in enumerate(w.trees):
+        n = (int(t["P"]) + w.bt - 1) // w.bt
+        blocks[i * entries:i * entries + n] = w.blocks[int(t["table"]):int(t["table"]) + n]
+        t["table"] = i * entries
+    w.blocks = blocks
+    return w
+
+
+@gpu
+@pytest.mark.parametrize("HD", [128, 256])
+def test_only_the_pages_that_are_read_are_widened(HD):
+    """A table with room for many more pages than its sequences have: the scratch of the entries behind them is left as it was; their
+    content may be anything, and what the trees read is right. Two trees share one table, one has no rows, one no cached keys."""
+    w = wl.make_pass("padded", 28, [(300, 20), (50, 0), (1000, 33), (0, 9), (300, 5)], 8, 2, HD, 16, wl.F16, wl.E4M3, scale=(HD // 2) ** -0.5)
+    w = _apart(w, 100, [0, -1, 3, w.n_blocks, 2 ** 30])
+    w.trees[4]["table"] = w.trees[0]["table"]
+    lam, norm_w = _weights(w, 3)
+    op = host.AttnOp.for_workload(w, 32)
+    dp = op.upload(w)
+    t = lambda a: torch.from_numpy(np.ascontiguousarray(a)).to(op.device)
+    O = torch.full((w.n_rows, w.q_ld), 0x1234, dtype=torch.int16, device=op.device)
+    page = 2 * w.bt * w.kv_ld * 2
+    scratch = torch.full((int(op.lib.esp_attn_dequant_scratch_bytes(C.byref(op.shape), len(w.blocks))),), 0xA5, dtype=torch.uint8, device=op.device)
+    _, opts = host.diff_plan_options(w.trees, w.H, w.Hkv, w.HD, w.kv_dtype)
+    call = op.diff_call(host.plan_tiles(w.trees, w.Hkv, **dict(opts, tile_rows=32)), w.trees, dp.Q, dp.Kb, dp.Vb, O, kv=dp.kv, kv_scales=dp.kv_scales, blocks=dp.blocks,
+                        n_blocks=w.n_blocks, desc=dp.desc, lam=t(lam), norm_w=t(norm_w), eps=EPS, out_scale=SCALE, scratch=scratch)
+    op.diff_forward(call)
+    torch.cuda.synchronize()
+    op.check_status()
+    assert op.last_kernel == "diff_umma"
+    O64, tol = diff64(w, lam, norm_w, EPS, SCALE, U16[wl.F16])
+    assert (np.abs(wl.from_bits16(O.cpu().numpy().view(np.uint16), wl.F16).astype(np.float64) - O64) <= tol).all()
+    pages = scratch[:len(w.blocks) * page].view(len(w.blocks), page)
+    left = (pages == 0xA5).all(dim=1).cpu().numpy()
+    read = np.zeros(len(w.blocks), dtype=bool)
+    for tree in w.trees:
+        if tree["M"]:
+            read[int(tree["table"]):int(tree["table"]) + (int(tree["P"]) + 15) // 16] = True
+    assert (left == ~read).all()
+    op.close()
+
+
+@gpu
+def test_widening_follows_lengths_that_change_on_the_device():
+    """A captured pass replayed after its trees and tiles were rewritten for longer sequences."""
+    short, w = [(100, 20), (40, 4)], wl.make_pass("grown", 29, [(700, 20), (333, 4)], 8, 2, 128, 16, wl.BF16, wl.E4M3, scale=0.125)
+    lam, norm_w = _weights(w, 3)
+    op = host.AttnOp.for_workload(w, 32)
+    dp = op.upload(w)
+    t = lambda a: torch.from_numpy(np.ascontiguousarray(a)).to(op.device)
+    trees = w.trees.copy()
+    trees["P"] = [p for p, _ in short]
+    plans = [host.plan_tiles(x, w.Hkv, mode=capi.ESP_PLAN_B200, split=0, tile_rows=32) for x in (trees, w.trees)]
+    assert len(plans[0].tiles) == len(plans[1].tiles)
+    O = torch.zeros((w.n_rows, w.q_ld), dtype=torch.int16, device=op.device)
+    call = op.diff_call(plans[0], trees, dp.Q, dp.Kb, dp.Vb, O, kv=dp.kv, kv_scales=dp.kv_scales, blocks=dp.blocks, n_blocks=w.n_blocks, desc=dp.desc, lam=t(lam), norm_w=t(norm_w),
+                        eps=EPS, out_scale=SCALE)
+    op.diff_forward(call)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        op.diff_forward(call)
+    tiles_dev, trees_dev = call.keep[2], call.keep[3]
+    tiles_dev.copy_(t(plans[1].tiles.view(np.int32)).view_as(tiles_dev))
+    trees_dev.copy_(t(w.trees.view(np.int32)).view_as(trees_dev))
+    g.replay()
+    torch.cuda.synchronize()
+    op.check_status()
+    O64, tol = diff64(w, lam, norm_w, EPS, SCALE, U16[wl.BF16])
+    assert (np.abs(wl.from_bits16(O.cpu().numpy().view(np.uint16), wl.BF16).astype(np.float64) - O64) <= tol).all()
+    op.close()
+
+
 # ---------------------------------------------------------------------------------------------- without a GPU
 def _append_args(**more):
     a = capi.AppendArgs(Q=0x10000, K=0x20000, V=0x30000, Qo=0x40000, Kb=0x50000, Vb=0x60000, kv=0x70000, kv_scales=0x80000, slots=0x90000, pos=0xA0000, inv_freq=0xB0000,

@@ -408,7 +408,8 @@ int esp_attn_create(esp_attn_ctx** out, int device, const esp_attn_shape* shape)
     delete c;
     return cuda_fail(e, "tcgen05 kernel setup");
   }
-  if ((e = esp::diff_decode_setup()) != cudaSuccess || (e = esp::diff_umma_setup()) != cudaSuccess) {
+  if ((e = esp::diff_decode_setup(shape->HD, c->G, shape->q_dtype, shape->kv_dtype, shape->bt)) != cudaSuccess ||
+      (e = esp::diff_umma_setup(shape->HD, c->G, shape->q_dtype, shape->kv_dtype, c->tile_rows, shape->bt)) != cudaSuccess) {
     delete c;
     return cuda_fail(e, "differential kernel setup");
   }

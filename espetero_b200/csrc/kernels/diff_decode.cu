@@ -465,12 +465,9 @@ cudaError_t setup_one() {
   return cudaFuncSetAttribute(diff_decode_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
 }
 template <int HD, int QDT>
-cudaError_t setup_types() {
-  cudaError_t e = setup_one<CfgOf<HD, QDT, QDT, 1>>();
-  if (e == cudaSuccess) e = setup_one<CfgOf<HD, QDT, QDT, 2>>();
-  if (e == cudaSuccess) e = setup_one<CfgOf<HD, ESP_E4M3, QDT, 1>>();
-  if (e == cudaSuccess) e = setup_one<CfgOf<HD, ESP_E4M3, QDT, 2>>();
-  return e;
+cudaError_t setup_types(int32_t G, int32_t kv_dtype) {
+  if (kv_dtype == ESP_E4M3) return G <= 4 ? setup_one<CfgOf<HD, ESP_E4M3, QDT, 1>>() : setup_one<CfgOf<HD, ESP_E4M3, QDT, 2>>();
+  return G <= 4 ? setup_one<CfgOf<HD, QDT, QDT, 1>>() : setup_one<CfgOf<HD, QDT, QDT, 2>>();
 }
 template <class C>
 cudaError_t launch_one(const DiffArgs& a, const CUtensorMap& m, cudaStream_t stream) {
@@ -487,12 +484,10 @@ cudaError_t launch_types(const DiffArgs& a, const CUtensorMap& m, cudaStream_t s
 
 bool diff_decode_supports(int32_t HD, int32_t G, int32_t bt) { return (HD == 128 || HD == 256) && G >= 1 && G <= 8 && bt % 16 == 0; }
 
-cudaError_t diff_decode_setup() {
-  cudaError_t e = setup_types<128, ESP_F16>();
-  if (e == cudaSuccess) e = setup_types<128, ESP_BF16>();
-  if (e == cudaSuccess) e = setup_types<256, ESP_F16>();
-  if (e == cudaSuccess) e = setup_types<256, ESP_BF16>();
-  return e;
+cudaError_t diff_decode_setup(int32_t HD, int32_t G, int32_t q_dtype, int32_t kv_dtype, int32_t bt) {
+  if (!diff_decode_supports(HD, G, bt)) return cudaSuccess;
+  if (HD == 128) return q_dtype == ESP_F16 ? setup_types<128, ESP_F16>(G, kv_dtype) : setup_types<128, ESP_BF16>(G, kv_dtype);
+  return q_dtype == ESP_F16 ? setup_types<256, ESP_F16>(G, kv_dtype) : setup_types<256, ESP_BF16>(G, kv_dtype);
 }
 
 cudaError_t launch_diff_decode(const DiffArgs& a, const CUtensorMap& pool_map, cudaStream_t stream, uint64_t* launches) {

@@ -565,13 +565,11 @@ template <int HD, int QDT, bool F8>
 cudaError_t setup_one() {
   return cudaFuncSetAttribute(diff_umma_kernel<HD, QDT, F8>, cudaFuncAttributeMaxDynamicSharedMemorySize, Geo<HD>::SMEM);
 }
-template <int HD>
-cudaError_t setup_hd() {
-  cudaError_t e = setup_one<HD, ESP_F16, false>();
-  if (e == cudaSuccess) e = setup_one<HD, ESP_BF16, false>();
-  if (e == cudaSuccess) e = setup_one<HD, ESP_F16, true>();
-  if (e == cudaSuccess) e = setup_one<HD, ESP_BF16, true>();
-  return e;
+// A pass over an E4M3 pool that reads no cached key runs without F8.
+template <int HD, int QDT>
+cudaError_t setup_types(int32_t kv_dtype) {
+  const cudaError_t e = setup_one<HD, QDT, false>();
+  return e == cudaSuccess && kv_dtype == ESP_E4M3 ? setup_one<HD, QDT, true>() : e;
 }
 template <int HD>
 cudaError_t launch_hd(const DiffArgs& a, bool f8, const CUtensorMap& pool_map, const CUtensorMap& q_map, const CUtensorMap& kb_map, const CUtensorMap& vb_map, cudaStream_t stream) {
@@ -601,9 +599,10 @@ bool diff_umma_supports(int32_t HD, int32_t G, int32_t tile_rows, int32_t bt) {
   return hpc <= G && G % hpc == 0;
 }
 
-cudaError_t diff_umma_setup() {
-  const cudaError_t e = setup_hd<128>();
-  return e == cudaSuccess ? setup_hd<256>() : e;
+cudaError_t diff_umma_setup(int32_t HD, int32_t G, int32_t q_dtype, int32_t kv_dtype, int32_t tile_rows, int32_t bt) {
+  if (!diff_umma_supports(HD, G, tile_rows, bt)) return cudaSuccess;
+  if (HD == 128) return q_dtype == ESP_F16 ? setup_types<128, ESP_F16>(kv_dtype) : setup_types<128, ESP_BF16>(kv_dtype);
+  return q_dtype == ESP_F16 ? setup_types<256, ESP_F16>(kv_dtype) : setup_types<256, ESP_BF16>(kv_dtype);
 }
 
 cudaError_t launch_diff_umma(const DiffArgs& a, bool f8, const CUtensorMap& pool_map, const CUtensorMap& q_map, const CUtensorMap& kb_map, const CUtensorMap& vb_map,

@@ -222,7 +222,7 @@ struct DiffCombineArgs {
 cudaError_t launch_diff_general(const DiffArgs& a, cudaStream_t stream, uint64_t* launches);
 // Single-row trees; pool_map is the map of the plain decode kernel.
 bool diff_decode_supports(int32_t HD, int32_t G, int32_t bt);
-cudaError_t diff_decode_setup();
+cudaError_t diff_decode_setup(int32_t HD, int32_t G, int32_t q_dtype, int32_t kv_dtype, int32_t bt);  // of what a context can launch
 cudaError_t launch_diff_decode(const DiffArgs& a, const CUtensorMap& pool_map, cudaStream_t stream, uint64_t* launches);
 // tcgen05 kernels: tiles of 16 .. 128 rows. pool_map as flash_umma's; q_map, kb_map, vb_map the same view of Q, Kb and Vb
 // with boxes of 128 rows (Vb with 256-dim heads: 64). f8: an E4M3 pool whose pages launch_diff_widen has laid out as 16-bit
@@ -230,7 +230,7 @@ cudaError_t launch_diff_decode(const DiffArgs& a, const CUtensorMap& pool_map, c
 // n_pages: of all trees; shared: some have one table
 cudaError_t launch_diff_widen(const KernelArgs& a, void* out, int64_t n_pages, bool shared, cudaStream_t stream, uint64_t* launches);
 bool diff_umma_supports(int32_t HD, int32_t G, int32_t tile_rows, int32_t bt);
-cudaError_t diff_umma_setup();
+cudaError_t diff_umma_setup(int32_t HD, int32_t G, int32_t q_dtype, int32_t kv_dtype, int32_t tile_rows, int32_t bt);
 cudaError_t launch_diff_umma(const DiffArgs& a, bool f8, const CUtensorMap& pool_map, const CUtensorMap& q_map, const CUtensorMap& kb_map, const CUtensorMap& vb_map,
                              cudaStream_t stream, uint64_t* launches);
 cudaError_t launch_diff_combine(const DiffCombineArgs& a, cudaStream_t stream, uint64_t* launches);

@@ -266,6 +266,60 @@ def test_widening_follows_lengths_that_change_on_the_device():
     op.close()
 
 
+LAYOUTS = [  # trees (P, M), H, Hkv, options, tile_rows, split, kernel
+    ("decode", [(100, 1), (0, 1), (333, 1)], 8, 2, None, 8, 32, "diff_decode"),
+    ("rows", [(100, 20), (0, 140), (333, 7)], 8, 2, None, 128, 0, "diff_umma"),
+    ("rows split", [(400, 20), (333, 7)], 8, 1, None, 16, 64, "diff_umma"),
+    ("general", [(100, 3), (0, 9), (333, 1)], 8, 2, GENERAL, 8, 64, "diff_general"),
+]
+
+
+@gpu
+@pytest.mark.parametrize("pool", [None, wl.E4M3], ids=["16-bit", "e4m3"])
+@pytest.mark.parametrize("HD", [128, 256])
+@pytest.mark.parametrize("case", LAYOUTS, ids=[c[0] for c in LAYOUTS])
+def test_a_layer_inside_a_wider_pool(case, HD, pool):
+    """The second of three layers of a pool whose rows, like the queries', the batch keys' and the output's, lie further apart than they are
+    wide. Everything beside them is NaN, and stays as it was."""
+    name, trees, H, Hkv, options, tile_rows, split, kernel = case
+    w = wl.make_pass(name, 30, trees, H, Hkv, HD, 16, wl.BF16, pool, scale=(HD // 2) ** -0.5)
+    q_ld, kv_ld, kv = w.q_ld + 72, w.kv_ld + 128, w.kv.reshape(-1, w.kv_ld)
+    nan16, nan_pool = 0x7FC0, 0x7FC0 if pool is None else 0x7F
+
+    def spread(x, ld, fill):
+        out = np.full((x.shape[0], ld), fill, dtype=x.dtype)
+        out[:, :x.shape[1]] = x
+        return out
+
+    lam, norm_w = _weights(w, 3)
+    op = host.AttnOp.for_workload(w, tile_rows)
+    for k, v in (options or {}).items():
+        op.set_option(k, v)
+    plan = host.plan_tiles(w.trees, Hkv, mode=capi.ESP_PLAN_B200, split=split, min_chunk=32, groups=4096 if split else 1, tile_rows=tile_rows)
+    dp = op.upload(w)
+    t = lambda a: torch.from_numpy(np.ascontiguousarray(a).view({2: np.int16, 1: np.uint8, 4: a.dtype}[a.dtype.itemsize])).to(op.device)
+    call = op.diff_call(plan, w.trees, dp.Q, dp.Kb, dp.Vb, dp.O, kv=dp.kv, kv_scales=dp.kv_scales, blocks=dp.blocks, n_blocks=w.n_blocks, desc=dp.desc, lam=t(lam),
+                        norm_w=t(norm_w), eps=EPS, out_scale=SCALE)
+    layer = spread(kv, kv_ld, nan_pool)
+    other = np.full_like(layer, nan_pool)
+    wide = dict(Q=t(spread(w.Q, q_ld, nan16)), Kb=t(spread(w.Kb, kv_ld, nan16)), Vb=t(spread(w.Vb, kv_ld, nan16)), kv=t(np.concatenate([other, layer, other])),
+                O=torch.full((w.n_rows, q_ld), 0x1234, dtype=torch.int16, device=op.device))
+    scratch = torch.empty(len(w.blocks) * (2 * w.bt * kv_ld * 2 + 4) + 256, dtype=torch.uint8, device=op.device)
+    for k, v in wide.items():
+        setattr(call.args, k, v.data_ptr())
+    call.args.p.q_ld, call.args.p.kv_ld, call.args.p.kv_base = q_ld, kv_ld, layer.size
+    call.args.dequant_scratch, call.args.dequant_scratch_bytes = scratch.data_ptr(), scratch.numel()
+    op.diff_forward(call)
+    torch.cuda.synchronize()
+    op.check_status()
+    assert op.last_kernel == kernel
+    O = wide["O"].cpu().numpy().view(np.uint16)
+    op.close()
+    assert (O[:, w.q_ld:] == 0x1234).all()
+    O64, tol = diff64(w, lam, norm_w, EPS, SCALE, _unit(w, kernel))
+    assert (np.abs(wl.from_bits16(O[:, :w.q_ld], wl.BF16).astype(np.float64) - O64) <= tol).all()
+
+
 # ---------------------------------------------------------------------------------------------- without a GPU
 def _append_args(**more):
     a = capi.AppendArgs(Q=0x10000, K=0x20000, V=0x30000, Qo=0x40000, Kb=0x50000, Vb=0x60000, kv=0x70000, kv_scales=0x80000, slots=0x90000, pos=0xA0000, inv_freq=0xB0000,

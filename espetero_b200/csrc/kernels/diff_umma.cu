@@ -30,7 +30,8 @@
 // Warps 0-7 softmax, 8 MMA issue (owns tensor memory), 9 / 10 K / V producers (TMA, one load per 16-key page and 64-dim chunk of the pool,
 // one per 64 or 128 rows of the batch; the Q tile, too, where it is 128 rows of one head), 11 idle (it
 // completes the warpgroup that hands registers over). Hand-offs by mbarrier; every wait is bounded: after a timeout the CTA records a
-// code, stops waiting, finishes its loop, frees its tensor memory and returns.
+// code, stops waiting, asks for no more copies, finishes its loop, gives copies and MMAs under way a millisecond, frees its tensor memory and
+// returns. (A flag on the MMA warp's issue cost 4 % of every pass; its queue holds few MMAs at a time.)
 // E4M3 pools (F8): the pages are 16-bit codes (diff_widen.cu); the K producer leaves each block's page scales in shared memory, the
 // K scale goes on the score and the V scale on the weight, whose reference is the largest product of the two.
 #include "diff_tile.cuh"
@@ -160,11 +161,12 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
   const bool whole_rows = tile.part < 0;
 
   auto wait_bar = [&](uint64_t* bar, uint32_t parity, int code) {
-    if (mbar_try_wait(bar, parity) || sh.dead) return;
-    if (!mbar_wait(bar, parity)) {
-      sh.dead = 1;
-      atomicExch(a.status, code);
-    }
+    if (mbar_try_wait(bar, parity)) return true;
+    if (sh.dead) return false;
+    if (mbar_wait(bar, parity)) return true;
+    sh.dead = 1;
+    atomicExch(a.status, code);
+    return false;
   };
 
   if (warp >= kMmaWarp) {
@@ -204,8 +206,9 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
               vs = a.kv_scales[(size_t(blk) * 2 + 1) * p.Hkv + kvh];
             }
             uint64_t* full = full0 + stage + part;
-            wait_bar(empty0 + stage + part, par, kStatusMmaTimeout);
-            if (kind < 0) {
+            if (!wait_bar(empty0 + stage + part, par, kStatusMmaTimeout)) {
+              // nothing is asked for any more
+            } else if (kind < 0) {
               mbar_arrive(full);
             } else if (is_v) {
               uint8_t* dst = v_sm + (stage + part) * C::V_SLOT + l * 2048;
@@ -225,8 +228,8 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
           // other trees' or none, zero past the tensor. Their scores are hidden and their V rows cleared.)
           [&](int b, int y) {
             uint64_t* full = full0 + stage + part;
-            wait_bar(empty0 + stage + part, par, kStatusMmaTimeout);
-            if (l < (is_v ? C::VC : C::QC)) {
+            if (!wait_bar(empty0 + stage + part, par, kStatusMmaTimeout)) {
+            } else if (l < (is_v ? C::VC : C::QC)) {
               mbar_arrive_expect_tx(full, is_v ? C::V_CHUNK : C::CHUNK);
               if (is_v) tma_load_3d(v_sm + (stage + part) * C::V_SLOT + l * C::V_CHUNK, &vb_map, full, 0, y + C::VK * part, kvh * C::VC + l);
               else tma_load_3d(k_sm + stage * C::K_TILE + l * C::CHUNK, &kb_map, full, 0, y, kvh * C::VC + map * C::QC + l);
@@ -558,6 +561,10 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
   }
   tc_fence_before_sync();
   __syncthreads();
+  if (sh.dead) {  // copies and MMAs still under way (the peer's half among them) land before their memory is given back
+    const uint64_t t0 = global_timer_ns();
+    while (global_timer_ns() - t0 < 1000000ull) {}
+  }
   if (warp == kMmaWarp) tmem_dealloc(sh.tmem, C::COLS);
 }
 

@@ -1179,7 +1179,7 @@ int esp::check_diff_pass(const esp_attn_shape& s, int TR, bool deep, const esp_a
   return esp::validate_pass(s, TR, deep, a);
 }
 
-// The entry points below may be called with another device current: they launch on their context's.
+// esp_kv_append and esp_diff_forward may be called with another device current: they launch on their context's.
 namespace {
 struct DeviceScope {
   int before = -1;
@@ -1247,8 +1247,9 @@ int esp_diff_plan_opts(const esp_attn_shape* s, const esp_attn_tree* trees, int3
   // of 16-row tiles; 5 rows behind 32768 keys 121 and 29. Over 75 passes of 1 .. 16 prompts and trees behind 200 .. 100000 keys (all heights,
   // 1 .. 32 parts) the choice is 1.05 times the best one's time in the geometric mean, 1.33 times at most. 700 rows behind 20001 E4M3 keys, 8 kv heads: 508 us
   // unsplit, 477 in two parts, 508 in three; it takes two. Small prompts share their tiles between heads: 4 x 33 rows, 256 dims, 24.5 us in tiles of
-  // one head, 13.0 of two; 8 x 20 .. 100 rows, 128 dims, 24.2 us of one, 21.0 of two, 13.8 of four. Near ties keep taller tiles and fewer parts
-  // (without a cached prefix ties within a tenth: 2 x 8192 and 5 x 33 .. 4001 rows measured 1 to 4 % faster in tiles of one head).
+  // one head, 13.0 of two; 8 x 20 .. 100 rows, 128 dims, 24.2 us of one, 21.0 of two, 13.8 of four. Near ties keep taller tiles and fewer parts:
+  // within 3 % with a cached prefix, within a tenth without (45 passes of prompts alone: 1.019 times the best height's time in the geometric mean, 1.38
+  // times at most, for 8 prompts of 7 and more rows; 1.016 and 1.15 at 3 %, where 325 rows of 256 dims lose 15 %).
   const bool wide = s->HD >= 256, split = cached > 2 * fresh;
   const double t_alone = wide ? 1.45 : 1.2, t_shared = wide ? 1.45 : 1.9, t_ends = 9.0;  // per 128 keys alone / sharing an SM; start and end of a CTA
   const double t_records = 40000.0;  // bytes of records that a CTA writes in a microsecond, a lane per row

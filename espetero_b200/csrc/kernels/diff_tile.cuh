@@ -1,5 +1,5 @@
-// What the two tcgen05 kernels of differential attention share: which key blocks a tile visits and what its rows see of them, the
-// pages of a block, and a few instruction wrappers.
+// Parts of the tcgen05 kernel of differential attention: which key blocks a tile visits and what its rows see of them, the pages of a block,
+// maxima and weights of a chunk of scores, and a few instruction wrappers.
 #pragma once
 
 #include <climits>

@@ -7,8 +7,8 @@
 // the rounded value over the block's scale).
 //
 // The angle: an fp32 product loses 2^-25 of up to 10^5 radians at far positions, more than a bf16 step. pos * inv_freq / 2 pi is
-// formed in double (the product of an int32 and an fp32 number is exact there), whole turns are taken off, and the rest, at most
-// half a turn, is good to fp32.
+// formed in double (the product is exact for |pos| < 2^29: 29 bits by 24), whole turns are taken off, and the rest, at most half a turn, is good to
+// fp32 for angles up to 2^29 radians: two roundings of 2^-53 leave 2^-25 of a turn there.
 //
 // HBM-bound for prompts (every byte is read and written once), latency-bound for single tokens. A warp owns one row, or a part of it when
 // rows are few. A lane's item is a rotating pair of 8-dim chunks, (d, d + rot_half), or one chunk that needs no partner; 32 lanes

@@ -459,13 +459,13 @@ int esp_attn_prep(esp_attn_ctx* ctx, void* stream, const float* X, const float* 
  * taken; 16-byte aligned rows are read fastest.
  * Rotation: each of the `maps` parts of a head (1, or 2 for differential heads; D = HD / maps dims) is rotated by itself:
  * pairs (f, f + rot_half), or with `adjacent` (2 f, 2 f + 1), f < rot_half, by the angle pos[row] * inv_freq[f], which is
- * formed exactly (any int32 position); dims from 2 * rot_half on pass through. rot_half = 0: no rotation (pos and inv_freq
+ * formed in double and good to fp32 up to 2^29 radians; dims from 2 * rot_half on pass through. rot_half = 0: no rotation (pos and inv_freq
  * are not read). Queries are then multiplied by qscale.
  * Outputs: Qo (rows q_ld apart), and - each optional, but together at least the pool or both of Kb and Vb - Kb / Vb (rows
  * kv_ld apart: the batch keys of the attention pass that follows) and the pool. slots: (block, position in block) per row;
  * block -1 = the row (padding, say) is not stored, though its Qo / Kb / Vb rows are written. A slot outside [0, n_blocks) x [0, bt)
- * is not written and sets the status word (esp_attn_check_status). Two rows with one slot: one of them is kept, unspecified
- * which. E4M3 pools take the code of the rounded 16-bit value with the block's scale, exactly as esp_kv_save would.
+ * is not written and sets the status word (esp_attn_check_status). Stored rows name distinct slots: one that two rows name
+ * ends up with parts of both. E4M3 pools take the code of the rounded 16-bit value with the block's scale, exactly as esp_kv_save would.
  * In place: Qo may be Q, Kb may be K and Vb may be V where type and row stride agree; other overlaps are not allowed.
  * Limits: HD <= 512, 2 * rot_half <= HD / maps. Nothing is allocated; one launch. */
 typedef struct esp_kv_append_args {
@@ -508,16 +508,17 @@ int esp_kv_append(esp_attn_ctx* ctx, void* stream, const esp_kv_append_args* arg
  * The page scales of an E4M3 pool are positive. `blocks` may hold entries that no tile reads (a padded table's), whatever they are.
  * Passes of one context may overlap on the GPU - two streams, two graphs - while their O, parts and dequant_scratch are apart.
  * A row that sees no key gets zeros. Rows that no tile covers are left as they were. Keys behind a tree's last row, pool rows past P and,
- * with ancestor masks, rows in nobody's mask are never mixed in, whatever they hold; keys that another row of the same tree sees must be
- * finite. tiles, trees and desc are 16-byte aligned. desc records may say "no ancestors" or "the whole tree" by any number below 0 or
- * above M, "sees nothing of the pass" by a segment start behind the row.
+ * with ancestor masks, rows in nobody's mask are never mixed in, whatever they hold; keys that another row of the same tree sees, and with
+ * desc every row of a tree, must be finite. tiles, trees and desc are 16-byte aligned. desc records may say "no ancestors" or "the whole
+ * tree" by any number below 0 or above M, "sees nothing of the pass" by a segment start behind the row.
  * Kernels: "diff_decode" (no tree has more than one row, G <= 8, HD 128 or 256, pages of 16 n keys), "diff_umma"
  * (HD 128 or 256, pages of 16 n keys, tile ranges that start at a multiple of 16) for tiles of 16, 32, 64 or 128 rows, 128 / tile_rows
- * heads of one kv head each (16-bit pools; E4M3 pools through dequant_scratch, sized as for esp_attn_forward; passes without
- * cached keys), "diff_general" for everything else and for calls without the host mirrors of tiles and trees, plus "diff_combine"
- * for split plans. esp_attn_last_kernel names the first of these. The option "attn_gqa" 0 keeps passes from diff_decode,
- * "attn_umma" 0 from diff_umma; "check_finite" scans these passes' output, too. Sums, maxima and the difference are fp32; softmax weights are rounded to the
- * pass's 16-bit type (fp16 over E4M3 pools in diff_decode, not at all in diff_general) before they meet V. */
+ * heads of one kv head each (16-bit pools; E4M3 pools through dequant_scratch, sized as for esp_attn_forward, of which the pages that
+ * the trees read are written; passes without cached keys), "diff_general" for everything else and for calls without the host mirrors
+ * of tiles and trees, plus "diff_combine" for split plans. esp_attn_last_kernel names the first of these. The option "attn_gqa" 0 keeps
+ * passes from diff_decode, "attn_umma" 0 from diff_umma; "check_finite" scans these passes' output, too. Sums, maxima and the
+ * difference are fp32; softmax weights are rounded to the pass's 16-bit type (fp16 over E4M3 pools in diff_decode, not at all in
+ * diff_general) before they meet V, in diff_umma over E4M3 pools times their page's V scale. */
 typedef struct esp_diff_args {
   const float* lam;    /* lam[row * lam_ld + h]: per head, lam_ld = 0, or per row and head, lam_ld >= H */
   const float* norm_w; /* [HD], or NULL: no norm */
@@ -533,7 +534,7 @@ size_t esp_diff_parts_floats(const esp_attn_shape* shape, int32_t n_parts);
  * kv_dtype of the shape. */
 int esp_diff_plan_opts(const esp_attn_shape* shape, const esp_attn_tree* trees_host, int32_t n_trees, esp_plan_opts* opts);
 /* lam[h] = exp(q1_h . k1_h) - exp(q2_h . k2_h) + lambda_init for h < H, from the layer's learned vectors ([H][dim] fp32, rows
- * ld elements apart; ld = 0: one vector for every head). Once per model load. One launch. */
+ * ld elements apart; ld = 0: one vector for every head). Once per model load. One launch, on the current device. */
 int esp_diff_lambda(void* stream, const float* q1, const float* k1, const float* q2, const float* k2, int32_t H, int32_t dim, int32_t ld,
                     float lambda_init, float* lam);
 

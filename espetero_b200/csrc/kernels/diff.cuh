@@ -24,6 +24,9 @@ __device__ __forceinline__ int4 row_record(const KernelArgs& a, int row, int M) 
   return d;
 }
 
+// log2 of a (positive) page scale, rounded down, within what references and their differences can hold.
+__device__ __forceinline__ float log2_floor(float v) { return fminf(fmaxf(float(int((__float_as_uint(v) >> 23) & 0xFFu) - 127), -100.0f), 100.0f); }
+
 __device__ __forceinline__ float diff_lam(const DiffArgs& a, int row, int h) { return a.lam[size_t(row) * a.lam_ld + h]; }
 
 // The factor that turns D into the normalised row (before the weight), from the sum of D^2 over the head.

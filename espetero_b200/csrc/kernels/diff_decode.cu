@@ -12,8 +12,8 @@
 // V and K arrive by TMA (two bulk tensor loads per block, 128-byte swizzle, rows through the page table) in rings that belong to
 // single warps, so nothing in the loop waits for another warp. Softmax in the exp2 domain over the key lanes; P^T re-enters as the
 // B operand (movmatrix), rounded to 16 bits: what the MMA takes; sums and the rows' totals stay fp32 and unrounded. E4M3 codes
-// are widened to fp16 in registers (exact), and bf16 queries scaled into its range, the K scale goes on the score, the V scale on the block's
-// P . V: p is rounded as it is, and the largest, 1, exactly.
+// are widened to fp16 in registers (exact), and bf16 queries scaled into its range, the K scale goes on the score, the power of
+// two in the V scale on the weight and the rest on the block's P . V: the largest weight, 1, is exact.
 // 32 sequences of 512 .. 32768 keys, H32 / Hkv4 / HD128, bf16: 92 us with the join = 5.7 TB/s, 0.87 of the copy peak; 131072 keys, Hkv8 / HD256, E4M3:
 // 94 us = 5.7 TB/s. 16 x 8192 E4M3 keys of 128 dims: 72 us = 3.7 TB/s, bound by the widening's instructions.
 // All waits are bounded; a CTA that gives up writes empty records and says so in the status word.
@@ -253,6 +253,10 @@ __global__ void __launch_bounds__(C::NW * 32, C::CTAS) diff_decode_kernel(const 
       }
     }
     const float sc = sl2 * kscale;
+    // What is rounded to 16 bits is the weight times the power of two in the V scale, and the reference the largest of these: neither a page of
+    // small values that is well attended nor one of large values that is hardly attended loses its weights. The rest of the scale,
+    // 1 .. 2, goes on the product.
+    const float v_log2 = C::FP8 ? log2_floor(vscale) : 0.0f, v_inv = C::FP8 ? __uint_as_float(uint32_t(127 - int(v_log2)) << 23) : 1.0f;
     const bool out_lo = g >= n_valid || g < n_skip, out_hi = g + 8 >= n_valid || g + 8 < n_skip;
     uint32_t pb[NT][2];
     float corr[NT][2];
@@ -260,8 +264,9 @@ __global__ void __launch_bounds__(C::NW * 32, C::CTAS) diff_decode_kernel(const 
     for (int n = 0; n < NT; ++n) {
       // lane: (key g, columns 2t, 2t + 1), (key g + 8, the same)
       const float sc0 = C::SCALED_Q ? sc * q_back[n][0] : sc, sc1 = C::SCALED_Q ? sc * q_back[n][1] : sc;
-      float s0 = (s[n][0][0] + s[n][1][0]) * sc0, s1 = (s[n][0][1] + s[n][1][1]) * sc1;
-      float s2 = (s[n][0][2] + s[n][1][2]) * sc0, s3 = (s[n][0][3] + s[n][1][3]) * sc1;
+      float s0 = s[n][0][0] + s[n][1][0], s1 = s[n][0][1] + s[n][1][1], s2 = s[n][0][2] + s[n][1][2], s3 = s[n][0][3] + s[n][1][3];
+      if constexpr (C::FP8) s0 = fmaf(s0, sc0, v_log2), s1 = fmaf(s1, sc1, v_log2), s2 = fmaf(s2, sc0, v_log2), s3 = fmaf(s3, sc1, v_log2);
+      else s0 *= sc0, s1 *= sc1, s2 *= sc0, s3 *= sc1;
       if (out_lo) s0 = s1 = -INFINITY;
       if (out_hi) s2 = s3 = -INFINITY;
       float x0 = fmaxf(s0, s2), x1 = fmaxf(s1, s3);
@@ -273,8 +278,8 @@ __global__ void __launch_bounds__(C::NW * 32, C::CTAS) diff_decode_kernel(const 
       const float n0 = fmaxf(m[n][0], x0), n1 = fmaxf(m[n][1], x1);  // a block has a live key
       corr[n][0] = fast_exp2(m[n][0] - n0), corr[n][1] = fast_exp2(m[n][1] - n1);
       const float p0 = fast_exp2(s0 - n0), p1 = fast_exp2(s1 - n1), p2 = fast_exp2(s2 - n0), p3 = fast_exp2(s3 - n1);
-      l[n][0] = fmaf(l[n][0], corr[n][0], p0 + p2);
-      l[n][1] = fmaf(l[n][1], corr[n][1], p1 + p3);
+      l[n][0] = fmaf(l[n][0], corr[n][0], C::FP8 ? (p0 + p2) * v_inv : p0 + p2);
+      l[n][1] = fmaf(l[n][1], corr[n][1], C::FP8 ? (p1 + p3) * v_inv : p1 + p3);
       m[n][0] = n0, m[n][1] = n1;
       pb[n][0] = movmatrix_trans(CE::pack2(p0, p1));
       pb[n][1] = movmatrix_trans(CE::pack2(p2, p3));
@@ -294,6 +299,7 @@ __global__ void __launch_bounds__(C::NW * 32, C::CTAS) diff_decode_kernel(const 
         }
       }
     } else {
+      const float v_rest = vscale * v_inv;
       // A maximum grows less and less often: the sums are only moved when one of the warp's has.
       bool grown = false;
 #pragma unroll
@@ -324,7 +330,7 @@ __global__ void __launch_bounds__(C::NW * 32, C::CTAS) diff_decode_kernel(const 
           mma_16816<C::CDT>(dx, fa, pb[n][0], pb[n][1]);
           mma_16816<C::CDT>(dy, fb, pb[n][0], pb[n][1]);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) x[i] = fmaf(dx[i], vscale, x[i]), y[i] = fmaf(dy[i], vscale, y[i]);
+          for (int i = 0; i < 4; ++i) x[i] = fmaf(dx[i], v_rest, x[i]), y[i] = fmaf(dy[i], v_rest, y[i]);
         }
       }
     }

@@ -213,8 +213,7 @@ __device__ __forceinline__ float chunk_max(const uint32_t (&s)[32]) {
 // Over an E4M3 pool a row's reference is the largest scaled score + log2 of the page's V scale: the scale of a page goes on the weights before
 // they are rounded to 16 bits, and what has to stay in fp16's range is their product. (Against the scores' maximum alone, a page of large values
 // that a row hardly attends would push the weights of the others under fp16's.) k0, k1 = scale of the softmax, in log2 units, times the
-// (positive) K scales of the chunk's two pages, v0, v1 their log2_scale.
-__device__ __forceinline__ float log2_scale(float v) { return fminf(fmaxf(float(int((__float_as_uint(v) >> 23) & 0xFFu) - 127), -100.0f), 100.0f); }  // rounded down
+// (positive) K scales of the chunk's two pages, v0, v1 their log2_floor.
 __device__ __forceinline__ float chunk_max(const uint32_t (&s)[32], float k0, float k1, float v0, float v1) {
   float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll

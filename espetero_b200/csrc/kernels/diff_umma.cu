@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::CTAS)
       auto shape = [&](uint32_t (&x)[32], int i) {
         if (!whole) hide(x, visible32(L, b, c0 + 32 * i, dsc, am, use_anc, rr));
       };
-      auto top = [&](const uint32_t (&x)[32], int i) { return F8 ? chunk_max(x, ks[2 * i], ks[2 * i + 1], log2_scale(vs[2 * i]), log2_scale(vs[2 * i + 1])) : sl2 * chunk_max(x); };  // scale > 0
+      auto top = [&](const uint32_t (&x)[32], int i) { return F8 ? chunk_max(x, ks[2 * i], ks[2 * i + 1], log2_floor(vs[2 * i]), log2_floor(vs[2 * i + 1])) : sl2 * chunk_max(x); };  // scale > 0
       constexpr int HELD = C::HOLD ? NS : 1;
       uint32_t s[HELD][32];
       float mx = -INFINITY;

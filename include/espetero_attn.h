@@ -518,7 +518,8 @@ int esp_kv_append(esp_attn_ctx* ctx, void* stream, const esp_kv_append_args* arg
  * of tiles and trees, plus "diff_combine" for split plans. esp_attn_last_kernel names the first of these. The option "attn_gqa" 0 keeps
  * passes from diff_decode, "attn_umma" 0 from diff_umma; "check_finite" scans these passes' output, too. Sums, maxima and the
  * difference are fp32; softmax weights are rounded to the pass's 16-bit type (fp16 over E4M3 pools in diff_decode, not at all in
- * diff_general) before they meet V, in diff_umma over E4M3 pools times their page's V scale. */
+ * diff_general) before they meet V: over E4M3 pools times their page's V scale (diff_umma) or the power of two in it (diff_decode),
+ * so that what a key adds to its row decides how many of its bits are kept. */
 typedef struct esp_diff_args {
   const float* lam;    /* lam[row * lam_ld + h]: per head, lam_ld = 0, or per row and head, lam_ld >= H */
   const float* norm_w; /* [HD], or NULL: no norm */

@@ -107,7 +107,8 @@ def _check_rows(name: str, t, device, dtypes, rows: int, width: int, ld: int | N
 
 @dataclass
 class Call:
-    """Arguments of one call and what they point to (device tensors, host records), kept alive together."""
+    """Arguments of one call and what they point to (device tensors, host records), kept alive together: until the work is done, where that runs on
+    another stream than the tensors'."""
     args: C.Structure
     more: C.Structure | None
     keep: tuple

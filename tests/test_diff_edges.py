@@ -251,6 +251,18 @@ def test_only_the_pages_that_are_read_are_widened(HD):
 
 
 @gpu
+@pytest.mark.parametrize("apart", [0, 20], ids=["tight", "padded"])
+def test_many_trees_over_e4m3(apart):
+    """More trees than a warp sums up at once, some without rows, some without cached keys, every seventh with its neighbour's table."""
+    w = wl.make_pass("many", 31, [((37 * i) % 290, (0, 1, 2, 5)[i % 4]) for i in range(75)], 4, 2, 128, 16, wl.F16, wl.E4M3, scale=0.125)
+    if apart:
+        w = _apart(w, apart, [-1, 0, 2 ** 30])
+    for i in range(7, 75, 7):
+        w.trees[i]["table"], w.trees[i]["P"] = w.trees[i - 1]["table"], min(int(w.trees[i]["P"]), int(w.trees[i - 1]["P"]))
+    _check(w, "diff_umma", tile_rows=64)
+
+
+@gpu
 def test_widening_follows_lengths_that_change_on_the_device():
     """A captured pass replayed after its trees and tiles were rewritten for longer sequences."""
     short, w = [(100, 20), (40, 4)], wl.make_pass("grown", 29, [(700, 20), (333, 4)], 8, 2, 128, 16, wl.BF16, wl.E4M3, scale=0.125)
